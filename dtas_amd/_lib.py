@@ -115,10 +115,16 @@ SIGNATURES = {
     "dtas_take_q8_f16": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _cfg, _vp],
     "dtas_gemv_q8_f32": [_vp, _vp, _vp, _vp, _i64, _i64, _cfg, _vp],
     "dtas_gemm_q8_f16_fused": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_int32, _cfg, _vp],
+    "dtas_gemv_q4_f16": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_int32, ctypes.c_int32, _vp],
+    "dtas_attn_tree_f16": [_vp] * 8 + [_i64] * 7 + [ctypes.c_float, _vp],
+    "dtas_verify_tree_f32": [_vp] * 9 + [_i64] * 3 + [_vp],
+    "dtas_cache_append_f16": [_vp] * 7 + [_i64] * 7 + [_vp],
 }
 
 # entry points that builds of this ABI version from before them lack: such a build (DTAS_LIBRARY) serves everything else
-LATER = {"dtas_builtin_gemm"}
+LATER = {"dtas_builtin_gemm", "dtas_gemv_q4_f16", "dtas_attn_tree_f16", "dtas_verify_tree_f32", "dtas_cache_append_f16"}
+
+MAX_TREE_NODES = 64
 
 _lib = None
 

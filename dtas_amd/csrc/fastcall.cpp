@@ -11,6 +11,9 @@
 #include <Python.h>
 #include <pthread.h>
 
+#include <cmath>
+#include <initializer_list>
+
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -27,8 +30,11 @@ namespace {
   X(dtas_attn_scores_f16_f32) X(dtas_attn_pv_f16) X(dtas_decode_q8_f16) X(dtas_attn_mask_f16)                            \
   X(dtas_softmax_temperature_f32) X(dtas_split3_f16) X(dtas_swap_axes_f16) X(dtas_rotary_f16) X(dtas_take_f16)           \
   X(dtas_take_q8_f16) X(dtas_gemv_q8_f32) X(dtas_gemv_q8_f16) X(dtas_gemm_q8_f16_fused) X(dtas_last_error)
+// entry points that older builds of the library lack: null there, and the function leaves its calls to the Python body
+#define DTAS_LATER_ENTRIES(X) X(dtas_gemv_q4_f16) X(dtas_attn_tree_f16) X(dtas_verify_tree_f32) X(dtas_cache_append_f16)
 #define DTAS_DECLARE(name) decltype(&::name) p_##name = nullptr;
 DTAS_ENTRIES(DTAS_DECLARE)
+DTAS_LATER_ENTRIES(DTAS_DECLARE)
 #undef DTAS_DECLARE
 PyObject* g_error = nullptr;  // dtas_amd._lib.DtasError
 bool g_bound = false;
@@ -332,6 +338,76 @@ DTAS_FUNCTION(gemm_q8, 8, {
   }
 })
 
+// ---- a decoding step with drafted tokens.  (Their names begin with an underscore: the list of the others is closed.)  All tensors
+// of a call have to lie on the current device, whose stream the launch goes to; a call from elsewhere is the Python body's, which
+// changes the device for it.
+bool here(std::initializer_list<const at::Tensor*> tensors) {
+  const auto device = c10::hip::current_device();
+  for (auto* t : tensors)
+    if (t && t->device().index() != device) return false;
+  return true;
+}
+bool shaped(const at::Tensor* t, std::initializer_list<int64_t> sizes) { return t->sizes() == at::IntArrayRef(sizes); }
+
+// x, Wq, scale, bias, y, epilogue, res1, res2
+DTAS_FUNCTION(_gemv_q4, 8, {
+  const int64_t epilogue = a.integer(5);
+  auto *x = a.tensor(0, F16), *Wq = a.tensor(1), *scale = a.tensor(2, F16), *y = a.tensor(4, epilogue == DTAS_EPI_BIAS_ADD2_CAST_F32 ? F32 : F16);
+  if (a.ok && p_dtas_gemv_q4_f16 && Wq->dim() == 2 && (Wq->scalar_type() == at::kInt || Wq->scalar_type() == at::kUInt32) && scale->dim() == 2 &&
+      x->dim() > 0 && y->dim() > 0) {
+    const int64_t N = Wq->size(0), K = Wq->size(1) * 8, group = K / scale->size(1), M = x->numel() / K;
+    auto *bias = a.optional(3, F16, N), *res1 = a.optional(6, F16, M * N), *res2 = a.optional(7, F16, M * N);
+    if (a.require(scale->size(0) == N && (group == 32 || group == 64 || group == 128) && K == group * scale->size(1) && x->size(-1) == K &&
+                  y->size(-1) == N && y->numel() == M * N && epilogue == static_cast<int32_t>(epilogue) && here({x, Wq, scale, bias, y, res1, res2})))
+      return DTAS_CALL(dtas_gemv_q4_f16, ptr(x), ptr(Wq), ptr(scale), ptr(bias), ptr(res1), ptr(res2), ptr(y), M, N, K, static_cast<int32_t>(group),
+                       static_cast<int32_t>(epilogue));
+  }
+})
+
+// Q, K, V, K_cache, V_cache, lens, parents, out, scale (None: 1 / sqrt(d))
+DTAS_FUNCTION(_attn_tree, 9, {
+  auto *Q = a.tensor(0, F16), *K = a.tensor(1, F16), *V = a.tensor(2, F16), *Kc = a.tensor(3, F16), *Vc = a.tensor(4, F16);
+  auto *lens = a.tensor(5, at::kInt), *parents = a.tensor(6, at::kInt), *out = a.tensor(7, F16);
+  if (a.ok && p_dtas_attn_tree_f16 && Q->dim() == 4 && K->dim() == 4 && Kc->dim() == 4) {
+    const int64_t B = Q->size(0), rows = Q->size(1), heads = Q->size(2), d = Q->size(3), nodes = K->size(1), kv_heads = K->size(2), C = Kc->size(2);
+    const float scale = argv[8] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(d))) : a.number(8);
+    if (a.require(shaped(K, {B, nodes, kv_heads, d}) && V->sizes() == K->sizes() && shaped(Kc, {B, kv_heads, C, d}) && Vc->sizes() == Kc->sizes() &&
+                  out->sizes() == Q->sizes() && shaped(lens, {B}) && shaped(parents, {B, nodes}) && here({Q, K, V, Kc, Vc, lens, parents, out})))
+      return DTAS_CALL(dtas_attn_tree_f16, ptr(Q), ptr(K), ptr(V), ptr(Kc), ptr(Vc), ptr(lens), ptr(parents), ptr(out), B, nodes, rows, heads, kv_heads,
+                       d, C, scale);
+  }
+})
+
+// target, draft, tokens, parents, accept, sample, path, count, next_token
+DTAS_FUNCTION(_verify_tree, 9, {
+  auto *target = a.tensor(0, F32), *draft = a.tensor(1, F32), *tokens = a.tensor(2, at::kInt), *parents = a.tensor(3, at::kInt);
+  auto *accept = a.tensor(4, F32), *sample = a.tensor(5, F32), *path = a.tensor(6, at::kInt), *count = a.tensor(7, at::kInt), *next = a.tensor(8, at::kInt);
+  if (a.ok && p_dtas_verify_tree_f32 && target->dim() == 3 && draft->sizes() == target->sizes()) {
+    const int64_t B = target->size(0), nodes = target->size(1), V = target->size(2);
+    for (auto* t : {tokens, parents, accept, path}) a.require(shaped(t, {B, nodes}));
+    for (auto* t : {sample, count, next}) a.require(shaped(t, {B}));
+    if (a.ok && here({target, draft, tokens, parents, accept, sample, path, count, next}))
+      return DTAS_CALL(dtas_verify_tree_f32, ptr(target), ptr(draft), ptr(tokens), ptr(parents), ptr(accept), ptr(sample), ptr(path), ptr(count),
+                       ptr(next), B, nodes, V);
+  }
+})
+
+// K, V, path, count, K_cache, V_cache, lens
+DTAS_FUNCTION(_cache_append, 7, {
+  auto *K = a.tensor(0, F16), *V = a.tensor(1, F16), *Kc = a.tensor(4, F16), *Vc = a.tensor(5, F16), *lens = a.tensor(6, at::kInt);
+  if (a.ok && p_dtas_cache_append_f16 && K->dim() >= 4 && Kc->dim() == K->dim() && V->sizes() == K->sizes() && Vc->sizes() == Kc->sizes()) {
+    const int64_t B = K->size(-4), nodes = K->size(-3), kv_heads = K->size(-2), d = K->size(-1), C = Kc->size(-2);
+    auto* path = argv[2] == Py_None ? nullptr : a.tensor(2, at::kInt);
+    auto* count = a.optional(3, at::kInt, B);
+    a.require((path == nullptr) == (count == nullptr) && Kc->size(-4) == B && Kc->size(-3) == kv_heads && Kc->size(-1) == d && shaped(lens, {B}));
+    a.require(!path || !count || (path->dim() == 2 && path->size(0) == B && count->dim() == 1));
+    for (int64_t i = 0; i + 4 < K->dim(); ++i) a.require(K->size(i) == Kc->size(i));
+    if (a.ok && here({K, V, path, count, Kc, Vc, lens}))
+      return DTAS_CALL(dtas_cache_append_f16, ptr(K), ptr(V), ptr(path), ptr(count), ptr(Kc), ptr(Vc), ptr(lens), K->numel() / (B * nodes * kv_heads * d), B,
+                       nodes, path ? path->size(1) : nodes, kv_heads, d, C);
+  }
+})
+
 // bind({entry point: address}, DtasError)
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *addresses, *error;
@@ -345,6 +421,14 @@ PyObject* bind(PyObject*, PyObject* args) {
   }
   DTAS_ENTRIES(DTAS_BIND)
 #undef DTAS_BIND
+#define DTAS_BIND_LATER(name)                                                                \
+  {                                                                                          \
+    PyObject* v = PyDict_GetItemString(addresses, #name);                                    \
+    p_##name = v ? reinterpret_cast<decltype(p_##name)>(PyLong_AsVoidPtr(v)) : nullptr;      \
+    if (PyErr_Occurred()) return nullptr;                                                    \
+  }
+  DTAS_LATER_ENTRIES(DTAS_BIND_LATER)
+#undef DTAS_BIND_LATER
   Py_INCREF(error);
   Py_XDECREF(g_error);
   g_error = error;
@@ -358,6 +442,7 @@ PyMethodDef methods[] = {DTAS_METHOD(add), DTAS_METHOD(copy), DTAS_METHOD(cast),
                          DTAS_METHOD(attn_scores), DTAS_METHOD(attn_pv), DTAS_METHOD(decode_q8), DTAS_METHOD(attn_mask),
                          DTAS_METHOD(softmax_temperature), DTAS_METHOD(split3), DTAS_METHOD(swap_axes), DTAS_METHOD(rotary),
                          DTAS_METHOD(take), DTAS_METHOD(take_q8), DTAS_METHOD(gemv_q8_f32), DTAS_METHOD(gemv_q8), DTAS_METHOD(gemm_q8),
+                         DTAS_METHOD(_gemv_q4), DTAS_METHOD(_attn_tree), DTAS_METHOD(_verify_tree), DTAS_METHOD(_cache_append),
                          {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

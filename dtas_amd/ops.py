@@ -507,3 +507,125 @@ def gemm_q8(A: torch.Tensor, Wq: torch.Tensor, scale: torch.Tensor, bias: Option
         raise ValueError("gemm_q8: shape mismatch")
     check(lib().dtas_gemm_q8_f16_fused(_p(A), _p(Wq), _p(scale), _p(bias), _p(res1), _p(res2), _p(C), M, N, K, epilogue,
                                        _cfg(cfg), _stream()), "dtas_gemm_q8_f16_fused")
+
+
+def _one_device(what: str, *tensors: Optional[torch.Tensor]):
+    """All tensors on one device: that device, made current for the launch (its current stream is the one the kernel goes on)."""
+    _dev(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"{what}: the tensors are on {len(devices)} devices")
+    return torch.cuda.device(devices.pop())
+
+
+def _ints(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if any(t is not None and t.dtype != torch.int32 for t in tensors):
+        raise ValueError(f"{what}: indices, lengths and counts are int32")
+
+
+def gemv_q4(x: torch.Tensor, Wq: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor], y: torch.Tensor,
+            epilogue: int = 0, res1: Optional[torch.Tensor] = None, res2: Optional[torch.Tensor] = None) -> None:
+    """y (..., N) = epilogue(x (..., K) . W^T) for the rows of x, with 4-bit weights W = (nibble - 7) * scale: element k of a row
+    of W is bits 4 (k % 8) .. + 3 of word k / 8 of Wq[N, K/8], scale [N, K/group] fp16 with groups of 32, 64 or 128.  Epilogues as
+    ``gemm``, in fp32 with one rounding.  For one row and the few of a tree of drafted tokens: W is read once per 64 rows."""
+    if _fastcall._gemv_q4(x, Wq, scale, bias, y, epilogue, res1, res2):
+        return
+    with _one_device("gemv_q4", x, Wq, scale, bias, y, res1, res2):
+        if Wq.dim() != 2 or Wq.dtype not in (torch.int32, torch.uint32) or scale.dim() != 2 or scale.dtype != torch.float16:
+            raise ValueError("gemv_q4: expects 32-bit words [N, K/8] and float16 scales [N, K/group]")
+        N, K = Wq.shape[0], Wq.shape[1] * 8
+        group = K // scale.shape[1] if scale.shape[1] else 32
+        if scale.shape[0] != N or group not in (32, 64, 128) or K != group * scale.shape[1]:
+            raise ValueError(f"gemv_q4: K = {K} and scales {tuple(scale.shape)} do not form groups of 32, 64 or 128")
+        if x.dim() == 0 or y.dim() == 0 or x.shape[-1] != K or y.shape[-1] != N:
+            raise ValueError("gemv_q4: inner extents differ")
+        M = x.numel() // K if K else y.numel() // max(N, 1)
+        want_out = torch.float32 if epilogue == _lib.EPI_BIAS_ADD2_CAST_F32 else torch.float16
+        if x.dtype != torch.float16 or y.dtype != want_out or any(t is not None and t.dtype != torch.float16 for t in (bias, res1, res2)):
+            raise ValueError("gemv_q4: expects fp16 x, bias and residuals (and an fp32 y for the cast epilogue)")
+        if y.numel() != M * N or (bias is not None and bias.numel() != N) or any(t is not None and t.numel() != M * N for t in (res1, res2)):
+            raise ValueError("gemv_q4: shape mismatch")
+        check(lib().dtas_gemv_q4_f16(_p(x), _p(Wq), _p(scale), _p(bias), _p(res1), _p(res2), _p(y), M, N, K, group, epilogue, _stream()),
+              "dtas_gemv_q4_f16")
+
+
+def attn_tree(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, K_cache: torch.Tensor, V_cache: torch.Tensor, lens: torch.Tensor,
+              parents: torch.Tensor, out: torch.Tensor, scale: Optional[float] = None) -> None:
+    """Attention of a tree of drafted tokens over a cache: out [b, t, h] = softmax(scale * Q[b, t, h] . keys) . values, where a row sees
+    the first lens[b] rows of the cache, the nodes above its own and its own.  Q and out (B, rows, heads, d), the nodes' own K and V
+    (B, nodes, kv_heads, d), the caches (B, kv_heads, capacity, d), all fp16; lens int32 (B), parents int32 (B, nodes), at most 64
+    nodes: the parent of node i lies in [0, i), any other value (-1) leaves it without one.  Row t is node nodes - rows + t: the last
+    `rows` nodes ask, all of them if there are as many.  `heads` is a multiple of `kv_heads`; scale 1 / sqrt(d) if None.  One node of
+    one row is the decode step.  ``take`` and ``rotary`` turn queries and keys of a tree: the tables' rows at the nodes' positions
+    (length + depth) taken first, then `rotary` over all rows with them."""
+    if _fastcall._attn_tree(Q, K, V, K_cache, V_cache, lens, parents, out, scale):
+        return
+    with _one_device("attn_tree", Q, K, V, K_cache, V_cache, lens, parents, out):
+        if any(t.dtype != torch.float16 for t in (Q, K, V, K_cache, V_cache, out)):
+            raise ValueError("attn_tree: expects fp16 queries, keys, values, caches and output")
+        _ints("attn_tree", lens, parents)
+        if any(t.dim() != 4 for t in (Q, K, K_cache)):
+            raise ValueError("attn_tree: expects Q (B, rows, heads, d), K (B, nodes, kv_heads, d) and caches (B, kv_heads, capacity, d)")
+        B, rows, heads, d = Q.shape
+        nodes, kv_heads, capacity = K.shape[1], K.shape[2], K_cache.shape[2]
+        if tuple(K.shape) != (B, nodes, kv_heads, d) or V.shape != K.shape or tuple(K_cache.shape) != (B, kv_heads, capacity, d) \
+                or V_cache.shape != K_cache.shape or out.shape != Q.shape or tuple(lens.shape) != (B,) or tuple(parents.shape) != (B, nodes):
+            raise ValueError("attn_tree: shape mismatch")
+        check(lib().dtas_attn_tree_f16(_p(Q), _p(K), _p(V), _p(K_cache), _p(V_cache), _p(lens), _p(parents), _p(out), B, nodes, rows, heads,
+                                       kv_heads, d, capacity, d ** -0.5 if scale is None and d else float(scale or 0.0), _stream()),
+              "dtas_attn_tree_f16")
+
+
+def verify_tree(target: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, accept: torch.Tensor,
+                sample: torch.Tensor, path: torch.Tensor, count: torch.Tensor, next_token: torch.Tensor) -> None:
+    """Which nodes of a tree of drafted tokens the target accepts.  target and draft (B, nodes, V) fp32: the distributions behind each node
+    (``softmax_temperature`` writes them), of the model that is served and of the one that the node's children were drawn from;
+    tokens, parents int32 (B, nodes), accept fp32 (B, nodes) and sample fp32 (B) uniform in [0, 1).  Node 0 is the last token already
+    chosen.  The children of a node are offered in the order of their index; a child with token x is accepted if accept * q(x) < p'(x),
+    p' the target's row at first; one that is refused leaves p' = max(p' - q, 0) / its sum.  Where none is accepted, next_token int32
+    (B) is the first token whose prefix sum of p' exceeds sample * the sum of p'.  path int32 (B, nodes) gets the nodes on the way, node 0
+    first and -1 behind the last, count int32 (B) their number.  A token outside [0, V) is never offered (padding: -1)."""
+    if _fastcall._verify_tree(target, draft, tokens, parents, accept, sample, path, count, next_token):
+        return
+    with _one_device("verify_tree", target, draft, tokens, parents, accept, sample, path, count, next_token):
+        if any(t.dtype != torch.float32 for t in (target, draft, accept, sample)):
+            raise ValueError("verify_tree: expects fp32 distributions and random numbers")
+        _ints("verify_tree", tokens, parents, path, count, next_token)
+        if target.dim() != 3 or draft.shape != target.shape:
+            raise ValueError("verify_tree: expects target and draft (B, nodes, V)")
+        B, nodes, V = target.shape
+        if any(tuple(t.shape) != (B, nodes) for t in (tokens, parents, accept, path)) or any(tuple(t.shape) != (B,) for t in (sample, count, next_token)):
+            raise ValueError("verify_tree: shape mismatch")
+        check(lib().dtas_verify_tree_f32(_p(target), _p(draft), _p(tokens), _p(parents), _p(accept), _p(sample), _p(path), _p(count),
+                                         _p(next_token), B, nodes, V, _stream()), "dtas_verify_tree_f32")
+
+
+def cache_append(K: torch.Tensor, V: torch.Tensor, path: Optional[torch.Tensor], count: Optional[torch.Tensor], K_cache: torch.Tensor,
+                 V_cache: torch.Tensor, lens: torch.Tensor) -> None:
+    """The rows that a step keeps, into the caches of all layers: K_cache[..., b, h, lens[b] + j, :] = K[..., b, path[b, j], h, :] for
+    j < count[b], and V alike.  K and V (..., B, nodes, kv_heads, d), the caches (..., B, kv_heads, capacity, d), fp16, with the same
+    leading extents (the layers); path int32 (B, slots) and count int32 (B) as ``verify_tree`` writes them, or both None: all rows
+    in their order (a prompt, a decoded token).  lens int32 (B) is read, not changed.  Rows that would fall outside the capacity, and
+    path entries outside [0, nodes), are left out."""
+    if _fastcall._cache_append(K, V, path, count, K_cache, V_cache, lens):
+        return
+    with _one_device("cache_append", K, V, path, count, K_cache, V_cache, lens):
+        if any(t.dtype != torch.float16 for t in (K, V, K_cache, V_cache)):
+            raise ValueError("cache_append: expects fp16 keys, values and caches")
+        _ints("cache_append", path, count, lens)
+        if K.dim() < 4 or K_cache.dim() != K.dim():
+            raise ValueError("cache_append: expects K (..., B, nodes, kv_heads, d) and caches (..., B, kv_heads, capacity, d)")
+        B, nodes, kv_heads, d = K.shape[-4:]
+        capacity = K_cache.shape[-2]
+        if V.shape != K.shape or V_cache.shape != K_cache.shape or tuple(K_cache.shape) != (*K.shape[:-4], B, kv_heads, capacity, d) \
+                or tuple(lens.shape) != (B,):
+            raise ValueError("cache_append: shape mismatch")
+        if (path is None) != (count is None):
+            raise ValueError("cache_append: path and count go together")
+        if path is not None and (path.dim() != 2 or path.shape[0] != B or tuple(count.shape) != (B,)):
+            raise ValueError("cache_append: shape mismatch")
+        layers = 1
+        for extent in K.shape[:-4]:
+            layers *= extent
+        check(lib().dtas_cache_append_f16(_p(K), _p(V), _p(path), _p(count), _p(K_cache), _p(V_cache), _p(lens), layers, B, nodes,
+                                          nodes if path is None else path.shape[1], kv_heads, d, capacity, _stream()), "dtas_cache_append_f16")

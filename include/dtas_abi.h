@@ -414,6 +414,56 @@ int dtas_decode_q8_f16(const void* Wq, const void* scale, void* W, int64_t N, in
 int dtas_gemv_q8_f16(const void* x, const void* Wq, const void* scale, const void* bias, void* y,
                      int64_t N, int64_t K, int32_t epilogue, const dtas_config* cfg, void* stream);
 
+/* ==== one decoding step with drafted tokens ====================================================================
+ * No PrimFunc of the reference: its model graphs decode row by row, against a cache that its runtime keeps.  The entry points
+ * below are what a step needs beside them that checks a tree of drafted tokens in one pass: the products of a drafting model
+ * in 4 bits, attention of the tree over the cache, the choice of a path, and its rows into the cache.
+ *
+ * A tree holds up to DTAS_MAX_TREE_NODES nodes per sequence, parents first: the parent of node i is parents[i] where that lies in
+ * [0, i); any other value leaves i without one.  Device buffers of counts and indices (lens, parents, tokens, path, count) are
+ * int32; values outside their range are treated as stated, never followed. */
+#define DTAS_MAX_TREE_NODES 64
+
+/* ---- 4-bit weights with fp16 group scales: y[M,N] = epilogue(x[M,K] . W^T), W[n,k] = (nibble - 7) * scale[n, k/group] ----
+ * Wq[N, K/8] uint32: element k of a row is bits 4 (k % 8) .. + 3 of word k / 8; scale[N, K/group] fp16, group 32, 64 or 128, K a
+ * multiple of it.  The weights are not rounded: a group's products are summed in fp32 and scaled there.  bias[N] or NULL;
+ * epilogues as dtas_gemm_f16_fused (res1, res2 [M,N] with the ADD2 kinds, NULL otherwise; y fp32 with ADD2_CAST_F32), but in
+ * fp32 with one rounding at the end, GELU by erfc.  Made for one row and the few of a tree: W is read again for every 64 rows. */
+int dtas_gemv_q4_f16(const void* x, const void* Wq, const void* scale, const void* bias, const void* res1, const void* res2, void* y,
+                     int64_t M, int64_t N, int64_t K, int32_t group, int32_t epilogue, void* stream);
+
+/* ---- attention of a tree over a cache ----
+ * out[b,t,h,:] = sum_j softmax_j(scale * Q[b,t,h,:] . k_j) v_j over the keys j that the row sees: [0, lens[b]) of the cache and, among
+ * the nodes' own, its node and the nodes above it.  Row t is node nodes - rows + t (the last `rows` nodes ask; rows == nodes: all).
+ * Q and out [batch, rows, heads, d], K and V [batch, nodes, kv_heads, d] (the nodes' own), K_cache and V_cache
+ * [batch, kv_heads, capacity, d], all fp16; lens[batch] (clipped to [0, capacity]), parents[batch, nodes].  heads is a multiple of
+ * kv_heads; query head h reads key head h / (heads / kv_heads).  d up to 256; multiples of 8 on 16-byte boundaries run on the matrix
+ * cores, others element by element.  fp32 scores and sums.  Keys are shared over workgroups that meet in the split-K workspace. */
+int dtas_attn_tree_f16(const void* Q, const void* K, const void* V, const void* K_cache, const void* V_cache, const void* lens,
+                       const void* parents, void* out, int64_t batch, int64_t nodes, int64_t rows, int64_t heads, int64_t kv_heads,
+                       int64_t d, int64_t capacity, float scale, void* stream);
+
+/* ---- which drafted tokens the target accepts, and the token behind them ----
+ * target and draft [batch, nodes, V] fp32: the distributions behind each node (rows that sum to one), of the large model and of the one
+ * that the node's children were drawn from, independently of each other; tokens, parents, accept (uniform in [0, 1))
+ * [batch, nodes]; sample (uniform in [0, 1)) [batch].  Node 0 is the last token already chosen.  From there on, with
+ * p' the target's row of the node: its children in the order of their index; one with token x is accepted if
+ * accept * q(x) < p'(x), and the walk goes on behind it; one that is refused leaves p' = max(p' - q, 0) / its sum.  Where no child is
+ * accepted the next token is the first whose prefix sum of p' exceeds sample * the sum of p' (p itself where nothing is left of p', -1
+ * where that is zero too).  Nodes with a token outside [0, V) or without a parent are not offered.
+ * path[batch, nodes]: the nodes on the way, node 0 first, -1 behind the last; count[batch]: how many; next[batch].  64-bit sums. */
+int dtas_verify_tree_f32(const void* target, const void* draft, const void* tokens, const void* parents, const void* accept,
+                         const void* sample, void* path, void* count, void* next, int64_t batch, int64_t nodes, int64_t V, void* stream);
+
+/* ---- rows into the caches of all layers ----
+ * K_cache[l,b,h,lens[b]+j,:] = K[l,b,path[b,j],h,:] for j < count[b], and V alike: K and V [layers, batch, nodes, kv_heads, d], the caches
+ * [layers, batch, kv_heads, capacity, d], fp16; path[batch, slots], count[batch] (as dtas_verify_tree_f32 writes them), or both NULL:
+ * all rows in their order (slots == nodes).  lens[batch] is read, not changed.  Rows that would fall outside [0, capacity), and path entries
+ * outside [0, nodes), are left out; everything else in the caches stays as it was.  nodes is not limited here. */
+int dtas_cache_append_f16(const void* K, const void* V, const void* path, const void* count, void* K_cache, void* V_cache, const void* lens,
+                          int64_t layers, int64_t batch, int64_t nodes, int64_t slots, int64_t kv_heads, int64_t d, int64_t capacity,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif
