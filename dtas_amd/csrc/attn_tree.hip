@@ -143,14 +143,14 @@ __device__ __forceinline__ void read_v(unsigned at, f16x4 (&lo)[N], f16x4 (&hi)[
         : "memory");
 }
 
-template <int DP, int RT>
-__global__ void __launch_bounds__(256) attn_tree_kernel(TreeArgs a, int row_groups, int nsplit, float* __restrict__ ws,
+template <int DP, int RT, int W>
+__global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_groups, int nsplit, float* __restrict__ ws,
                                                         unsigned* __restrict__ arrivals) {
   constexpr int KS = DP / 32, DT = DP / 16, VL = DP / 16;  // k steps, channel tiles, 16-byte pieces of V per lane and block
   constexpr int kRows = 16 * RT, kChunks = DP / 8;
   constexpr int kPartial = kRows * (DP + 2);               // floats of a split's share: sums, then maxima, then weights
-  __shared__ __attribute__((aligned(16))) char lds[4 * wave_bytes(DP)];
-  __shared__ float stat_m[4][kRows], stat_l[4][kRows];
+  __shared__ __attribute__((aligned(16))) char lds[W * wave_bytes(DP)];
+  __shared__ float stat_m[W][kRows], stat_l[W][kRows];
   __shared__ int last_flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
   const int g = a.heads / a.kv_heads, R = a.Tq * g;
@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(TreeArgs a, int row_grou
   const int bh = unit / nsplit, z = unit % nsplit, b = bh / a.kv_heads, hk = bh % a.kv_heads;
   const int64_t len = clamp_len(a.lens[b], a.capacity);
   const int cached_blocks = static_cast<int>((len + kBlockKeys - 1) / kBlockKeys), blocks = cached_blocks + (a.T + kBlockKeys - 1) / kBlockKeys;
-  // a split takes at least four blocks, one per wavefront; splits beyond what that leaves have nothing to do
-  int splits = (blocks + 3) / 4;
+  // a split takes at least a block per wavefront; splits beyond what that leaves have nothing to do
+  int splits = (blocks + W - 1) / W;
   splits = splits < nsplit ? splits : nsplit;
   if (z >= splits) return;
   const int first = static_cast<int>(static_cast<int64_t>(blocks) * z / splits), end = static_cast<int>(static_cast<int64_t>(blocks) * (z + 1) / splits);
@@ -343,11 +343,11 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(TreeArgs a, int row_grou
     load_k(s);
     load_v(s);
   }
-  for (; blk < end && blk < cached_blocks; blk += 4)
-    visit(std::false_type{}, static_cast<int>(len - static_cast<int64_t>(blk) * kBlockKeys), 0, blk + 4 < end, blk + 4);
+  for (; blk < end && blk < cached_blocks; blk += W)
+    visit(std::false_type{}, static_cast<int>(len - static_cast<int64_t>(blk) * kBlockKeys), 0, blk + W < end, blk + W);
   if (blk < end) visit(std::true_type{}, 0, (blk - cached_blocks) * kBlockKeys, false, 0);
 
-  // ---- the four wavefronts' shares, joined in their order
+  // ---- the wavefronts' shares, joined in their order
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     sum[rt] = sum_of_row(sum[rt]);
@@ -358,7 +358,13 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(TreeArgs a, int row_grou
   }
   __syncthreads();
   auto weight_of = [](float m, float best) { return best == -INFINITY ? 0.f : exp2_fast(m - best); };
-  const int tile = bh * row_groups + rg;
+  auto best_of = [&](int r) {
+    float best = stat_m[0][r];
+#pragma unroll
+    for (int w = 1; w < W; ++w) best = fmaxf(best, stat_m[w][r]);
+    return best;
+  };
+  const int tile = bh * row_groups + rg, my_rows = R - rg * kRows < kRows ? R - rg * kRows : kRows;
   float* share = ws + (static_cast<int64_t>(tile) * nsplit + z) * kPartial;
   auto out_row = [&](int r) -> half_t* {
     return a.out + ((static_cast<int64_t>(b) * a.Tq + r / g) * a.heads + hk * g + r % g) * a.d;
@@ -368,36 +374,37 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(TreeArgs a, int row_grou
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row0 = rt * 16;
+    if (row0 >= my_rows) break;
     {
-      const int r = row0 + i16;
-      const float best = fmaxf(fmaxf(stat_m[0][r], stat_m[1][r]), fmaxf(stat_m[2][r], stat_m[3][r])), w = weight_of(top[rt], best);
+      const float w = weight_of(top[rt], best_of(row0 + i16));
       float* to = reinterpret_cast<float*>(mine) + i16 * kPitch + 4 * quarter;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(to + dt * 16) = f32x4{o[rt][dt][0] * w, o[rt][dt][1] * w, o[rt][dt][2] * w, o[rt][dt][3] * w};
     }
     __syncthreads();
-    for (int at = tid; at < 16 * (DP / 4); at += 256) {
-      const int i = at / (DP / 4), c = 4 * (at % (DP / 4)), r = rg * kRows + row0 + i;
+    for (int at = tid; at < 16 * (DP / 4); at += 64 * W) {
+      const int i = at / (DP / 4), c = 4 * (at % (DP / 4)), r = row0 + i;
+      if (r >= my_rows || c >= a.d) continue;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
       float l = 0.f;
-      const float best = fmaxf(fmaxf(stat_m[0][row0 + i], stat_m[1][row0 + i]), fmaxf(stat_m[2][row0 + i], stat_m[3][row0 + i]));
+      const float best = best_of(r);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < W; ++w) {
         const f32x4 part = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * wave_bytes(DP)) + i * kPitch + c);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += part[j];
-        l += stat_l[w][row0 + i] * weight_of(stat_m[w][row0 + i], best);
+        l += stat_l[w][r] * weight_of(stat_m[w][r], best);
       }
       if (splits > 1) {
-        store_out(v, reinterpret_cast<f32x4*>(share + (row0 + i) * DP + c), true);
+        store_out(v, reinterpret_cast<f32x4*>(share + r * DP + c), true);
         if (c == 0)
-          __hip_atomic_store(reinterpret_cast<uint64_t*>(share + kRows * DP) + row0 + i,
+          __hip_atomic_store(reinterpret_cast<uint64_t*>(share + kRows * DP) + r,
                              static_cast<uint64_t>(__builtin_bit_cast(unsigned, best)) | static_cast<uint64_t>(__builtin_bit_cast(unsigned, l)) << 32,
                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      } else if (r < R && c < a.d) {
+      } else {
         const float inv = 1.f / l;
-        *reinterpret_cast<f16x4*>(out_row(r) + c) = f16x4{static_cast<half_t>(v[0] * inv), static_cast<half_t>(v[1] * inv),
-                                                          static_cast<half_t>(v[2] * inv), static_cast<half_t>(v[3] * inv)};
+        *reinterpret_cast<f16x4*>(out_row(rg * kRows + r) + c) = f16x4{static_cast<half_t>(v[0] * inv), static_cast<half_t>(v[1] * inv),
+                                                                       static_cast<half_t>(v[2] * inv), static_cast<half_t>(v[3] * inv)};
       }
     }
     __syncthreads();
@@ -416,54 +423,66 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(TreeArgs a, int row_grou
   __syncthreads();
   if (!last_flag) return;
   const float* shares = ws + static_cast<int64_t>(tile) * nsplit * kPartial;
-  uint64_t* stats = reinterpret_cast<uint64_t*>(lds);  // [split][row]: maximum and sum
-  for (int at = tid; at < splits * kRows; at += 256)
-    stats[at] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(at / kRows) * kPartial + kRows * DP) + at % kRows,
-                                  __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  uint64_t* stats = reinterpret_cast<uint64_t*>(lds);  // [split][row]: maximum and sum; the sum turns into the split's weight
+  for (int at = tid; at < splits * kRows; at += 64 * W)
+    if (at % kRows < my_rows)
+      stats[at] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(at / kRows) * kPartial + kRows * DP) + at % kRows,
+                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  for (int at = tid; at < kRows * (DP / 4); at += 256) {
-    const int i = at / (DP / 4), c = 4 * (at % (DP / 4)), r = rg * kRows + i;
-    if (r >= R || c >= a.d) continue;
+  for (int at = tid; at < my_rows * (DP / 4); at += 64 * W) {
+    const int i = at / (DP / 4), c = 4 * (at % (DP / 4));
+    if (c >= a.d) continue;
     float best = -INFINITY, l = 0.f;
     for (int y = 0; y < splits; ++y) best = fmaxf(best, __builtin_bit_cast(float, static_cast<unsigned>(stats[y * kRows + i])));
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int y = 0; y < splits; ++y) {
-      const uint64_t two = stats[y * kRows + i];
-      const float w = weight_of(__builtin_bit_cast(float, static_cast<unsigned>(two)), best);
-      const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(y) * kPartial + i * DP + c);
-      const uint64_t one = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const uint64_t other = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      l = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(two >> 32)), l);
-      v[0] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one)), v[0]);
-      v[1] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one >> 32)), v[1]);
-      v[2] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other)), v[2]);
-      v[3] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other >> 32)), v[3]);
+    constexpr int kAtOnce = 8;  // shares requested before the first is used: a trip to memory per eight splits
+    for (int y0 = 0; y0 < splits; y0 += kAtOnce) {
+      uint64_t one[kAtOnce], other[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int y = y0 + u < splits ? y0 + u : splits - 1;
+        const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(y) * kPartial + i * DP + c);
+        one[u] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        other[u] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (y0 + u >= splits) break;
+        const uint64_t two = stats[(y0 + u) * kRows + i];
+        const float w = weight_of(__builtin_bit_cast(float, static_cast<unsigned>(two)), best);
+        l = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(two >> 32)), l);
+        v[0] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u])), v[0]);
+        v[1] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u] >> 32)), v[1]);
+        v[2] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u])), v[2]);
+        v[3] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u] >> 32)), v[3]);
+      }
     }
     const float inv = 1.f / l;
-    *reinterpret_cast<f16x4*>(out_row(r) + c) = f16x4{static_cast<half_t>(v[0] * inv), static_cast<half_t>(v[1] * inv),
-                                                      static_cast<half_t>(v[2] * inv), static_cast<half_t>(v[3] * inv)};
+    *reinterpret_cast<f16x4*>(out_row(rg * kRows + i) + c) = f16x4{static_cast<half_t>(v[0] * inv), static_cast<half_t>(v[1] * inv),
+                                                                   static_cast<half_t>(v[2] * inv), static_cast<half_t>(v[3] * inv)};
   }
 }
 
-template <int DP, int RT>
+template <int DP, int RT, int W>
 int launch_tree(const TreeArgs& a, int64_t batch, hipStream_t s) {
   constexpr int kRows = 16 * RT;
   const int64_t groups = ceil_div(static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads), kRows), tiles = batch * a.kv_heads * groups;
-  // two workgroups for each CU, while a split keeps four blocks of keys and the statistics of all splits fit the LDS
+  // a workgroup for each CU, while a split keeps a block of keys per wavefront and the statistics of all splits fit the LDS
   constexpr int kMostSplits = 64 / RT;
-  int64_t nsplit = ceil_div(2 * kNumCU, tiles);
-  const int64_t blocks = ceil_div(a.capacity, kBlockKeys) + ceil_div(a.T, kBlockKeys), useful = ceil_div(blocks, 4);
+  int64_t nsplit = kNumCU / tiles;
+  const int64_t blocks = ceil_div(a.capacity, kBlockKeys) + ceil_div(a.T, kBlockKeys), useful = ceil_div(blocks, W);
   nsplit = nsplit > useful ? useful : nsplit;
   nsplit = nsplit > kMostSplits ? kMostSplits : nsplit;
+  nsplit = nsplit < 1 ? 1 : nsplit;
   if (tiles * nsplit > INT32_MAX) return fail("attn_tree: the launch has too many workgroups");
-  static_assert(kMostSplits * kRows * 8 <= 4 * wave_bytes(DP), "the splits' statistics fit the LDS");
+  static_assert(kMostSplits * kRows * 8 <= W * wave_bytes(DP), "the splits' statistics fit the LDS");
   float* partials = nullptr;
   unsigned* arrivals = nullptr;
   std::unique_lock<std::recursive_mutex> lock;
   if (nsplit > 1 && split_scratch(s, static_cast<size_t>(tiles * nsplit) * kRows * (DP + 2) * sizeof(float), static_cast<size_t>(tiles),
                                   static_cast<int>(nsplit), &partials, &arrivals, &lock) != 0)
     return -1;
-  hipLaunchKernelGGL((attn_tree_kernel<DP, RT>), dim3(static_cast<unsigned>(tiles * nsplit)), dim3(256), 0, s, a, static_cast<int>(groups),
+  hipLaunchKernelGGL((attn_tree_kernel<DP, RT, W>), dim3(static_cast<unsigned>(tiles * nsplit)), dim3(64 * W), 0, s, a, static_cast<int>(groups),
                      static_cast<int>(nsplit), partials, arrivals);
   return check_launch("attn_tree");
 }
@@ -471,9 +490,9 @@ int launch_tree(const TreeArgs& a, int64_t batch, hipStream_t s) {
 template <int DP>
 int launch_tree_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
-  if (rows <= 16) return launch_tree<DP, 1>(a, batch, s);
-  if (rows <= 32 || DP > 128) return launch_tree<DP, 2>(a, batch, s);  // (more sums than 512 registers hold, beyond 128 channels)
-  if constexpr (DP <= 128) return launch_tree<DP, 4>(a, batch, s);
+  if (rows <= 16) return launch_tree<DP, 1, (DP <= 128 ? 8 : 4)>(a, batch, s);
+  if (rows <= 32 || DP > 128) return launch_tree<DP, 2, (DP <= 128 ? 8 : 4)>(a, batch, s);  // (more sums than 512 registers hold, beyond 128 channels)
+  if constexpr (DP <= 128) return launch_tree<DP, 4, 4>(a, batch, s);
 }
 
 }  // namespace
