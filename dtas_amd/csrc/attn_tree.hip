@@ -18,7 +18,8 @@ struct TreeArgs {
   half_t* out;
   int T, Tq, heads, kv_heads, d;
   int64_t capacity;
-  float scale_log2;  // scale * log2(e): the softmax is taken in powers of two
+  float scale_log2;  // |scale| * log2(e): the softmax is taken in powers of two
+  half_t sign;       // the scale's: 1, -1, or 0 (scale_log2 is 1 then)
 };
 
 __device__ __forceinline__ int64_t clamp_len(int len, int64_t capacity) {
@@ -43,7 +44,7 @@ __global__ void __launch_bounds__(64) attn_tree_scalar_kernel(TreeArgs a, int64_
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (lane + 64 * i < a.d) s = fmaf(qv[i], static_cast<float>(k[lane + 64 * i]), s);
-      s = wave_sum(s) * a.scale_log2;
+      s = wave_sum(s) * static_cast<float>(a.sign) * a.scale_log2;
       const float next = fmaxf(top, s);
       const float keep = next == -INFINITY ? 1.f : exp2f(top - next), p = next == -INFINITY ? 0.f : exp2f(s - next);
       top = next;
@@ -68,17 +69,20 @@ __global__ void __launch_bounds__(64) attn_tree_scalar_kernel(TreeArgs a, int64_
 }
 
 // ---- head dimensions that are multiples of 8, data on 16-byte boundaries: the matrix cores -----------------------------------
-// A workgroup serves up to 16 RT rows of one key head (its query heads' rows of all nodes: they read the same keys) and a run of
-// the keys; its four wavefronts take blocks of 32 keys in turn, each for all the rows and without a barrier until the end.
-//   S^T = K Q^T   A = 16 keys: a lane's 8 channels of one key are 16 contiguous bytes, loaded from memory straight into the operand's
-//                 registers; B = 16 rows.  Lane l holds keys 4 (l >> 4) .. + 3 of row l & 15.
-//   O^T = V^T P^T B = P^T as the scores' lanes hold it, its 8 keys per lane being 4 (l >> 4) .. + 3 of the block's two halves: the order of
+// The query heads' rows of one key head (of all nodes) read the same keys and form one problem of R = Tq * heads / kv_heads rows.
+//   S^T = K Q^T   A = 16 keys, B = 16 rows: lane l holds keys 4 (l >> 4) .. + 3 of row l & 15, so a row's maximum and sum take
+//                 the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+//   O^T = V^T P^T B = P^T as the scores' lanes hold it, its 8 keys per lane being 4 (l >> 4) .. + 3 of two key tiles: the order of
 //                 the keys inside an MFMA is free, so P never moves.  A = V^T in the same order: 4 keys of one channel per
-//                 transposing LDS read, from the block's V rows (32 bytes longer than a row: eight rows fall on different banks).
-// A wavefront holds one block of K and one of V on their way in registers while it works on the block before.
-constexpr int kBlockKeys = 32;
+//                 transposing LDS read, from V's rows (32 bytes longer than a row: eight rows fall on different banks).
+// P is rounded to fp16 for its product (half a step, 2^-11 of each weight); scores, maxima, sums and O stay in fp32.
+// Two kernels: up to 16 (32) rows the wavefronts of a workgroup share the keys and load K's operands straight from memory; with more rows
+// they share the rows and every key passes through the LDS once.
 constexpr int v_row_bytes(int DP) { return 2 * DP + 32; }
-constexpr int wave_bytes(int DP) { return kBlockKeys * v_row_bytes(DP); }
+// A kernel for DP channels serves head dimensions above `below(DP)`: a lane whose channels lie behind the head's last reads that head's last
+// ones instead, and what it read of K and Q is cleared (of V it only reaches sums that are not stored).
+constexpr int below(int DP) { return DP == 64 ? 0 : DP == 96 ? 64 : DP == 128 ? 96 : DP == 192 ? 128 : 192; }
+constexpr int k_row_bytes(int DP) { return 2 * DP + 16; }  // (the same 16 bytes of sixteen keys fall on different banks)
 
 // a value's maximum (sum) over the four lanes that hold the same row, l, l ^ 16, l ^ 32, l ^ 48.  The swaps exchange halves (and
 // quarters) of two registers; of a value and its copy, whose origin is hidden (given one value twice the compiler takes the two results for one)
@@ -97,9 +101,8 @@ __device__ __forceinline__ float sum_of_row(float v) { return over_row(v, [](flo
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// the nodes on the path of node `lane` up to a root, its own included, by doubling the reach six times
-__device__ __forceinline__ uint64_t ancestors(const int* parents, int T, int lane) {
-  int up = lane < T ? parents[lane] : -1;
+// the nodes on the path of node `lane`, with parent `up`, to a root, its own included, by doubling the reach six times
+__device__ __forceinline__ uint64_t ancestors(int up, int lane) {
   if (up < 0 || up >= lane) up = -1;
   uint64_t line = uint64_t{1} << lane;
 #pragma unroll
@@ -143,45 +146,342 @@ __device__ __forceinline__ void read_v(unsigned at, f16x4 (&lo)[N], f16x4 (&hi)[
         : "memory");
 }
 
-template <int DP, int RT, int W>
-__global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_groups, int nsplit, float* __restrict__ ws,
-                                                        unsigned* __restrict__ arrivals) {
-  constexpr int KS = DP / 32, DT = DP / 16, VL = DP / 16;  // k steps, channel tiles, 16-byte pieces of V per lane and block
-  constexpr int kRows = 16 * RT, kChunks = DP / 8;
-  constexpr int kPartial = kRows * (DP + 2);               // floats of a split's share: sums, then maxima, then weights
-  __shared__ __attribute__((aligned(16))) char lds[W * wave_bytes(DP)];
-  __shared__ float stat_m[W][kRows], stat_l[W][kRows];
-  __shared__ int last_flag;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
-  const int g = a.heads / a.kv_heads, R = a.Tq * g;
-  const unsigned units = gridDim.x / row_groups;           // (key head, split) pairs; the row groups of one meet on one XCD
-  const int rg = static_cast<int>(blockIdx.x / units), unit = static_cast<int>(blockIdx.x % units);
-  const int bh = unit / nsplit, z = unit % nsplit, b = bh / a.kv_heads, hk = bh % a.kv_heads;
-  const int64_t len = clamp_len(a.lens[b], a.capacity);
-  const int cached_blocks = static_cast<int>((len + kBlockKeys - 1) / kBlockKeys), blocks = cached_blocks + (a.T + kBlockKeys - 1) / kBlockKeys;
-  // a split takes at least a block per wavefront; splits beyond what that leaves have nothing to do
-  int splits = (blocks + W - 1) / W;
-  splits = splits < nsplit ? splits : nsplit;
-  if (z >= splits) return;
-  const int first = static_cast<int>(static_cast<int64_t>(blocks) * z / splits), end = static_cast<int>(static_cast<int64_t>(blocks) * (z + 1) / splits);
+// (maxima are those of the products, before the scale)
+__device__ __forceinline__ float weight_of(float m, float best, float scale_log2) { return best == -INFINITY ? 0.f : exp2_fast((m - best) * scale_log2); }
 
-  // ---- the rows: operands of Q, and which nodes each sees
-  f16x8 q[RT][KS];
-  uint64_t sees[RT];
-  const uint64_t line = end > cached_blocks ? ancestors(a.parents + static_cast<int64_t>(b) * a.T, a.T, lane) : 0;
+// the nodes that the row tiles see, from every lane's node
+template <int RT>
+__device__ __forceinline__ void see(uint64_t (&sees)[RT], int up, int lane, int row0, int R, int g, int T, int Tq) {
+  const uint64_t line = ancestors(up, lane);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    int r = rg * kRows + rt * 16 + i16;
-    r = r < R ? r : R - 1;
-    const int t = r / g;
-    const half_t* row = a.Q + ((static_cast<int64_t>(b) * a.Tq + t) * a.heads + hk * g + r % g) * a.d;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int at = ks * 32 + quarter * 8;
-      q[rt][ks] = at < a.d ? *reinterpret_cast<const f16x8*>(row + at) : f16x8{};
-    }
-    sees[rt] = __shfl(static_cast<unsigned long long>(line), a.T - a.Tq + t);
+    const int r = row0 + rt * 16 + (lane & 15);
+    sees[rt] = __shfl(static_cast<unsigned long long>(line), T - Tq + (r < R ? r : R - 1) / g);
   }
+}
+
+// ---- Which part of which sequence a workgroup has.  A sequence's units of keys (the blocks of its cache, those of the nodes behind) are cut into runs of
+// `per` units at most, the smallest `per` (and `least` at least) with which all sequences together make no more than `budget` parts, and a
+// sequence no more than `most`; its parts take consecutive slots.
+struct Part {
+  int b, z, parts, first;  // sequence, which of its parts, of how many, the sequence's first slot; b < 0: nothing to do
+};
+__device__ __forceinline__ int units_of(int len, int64_t capacity, int unit, int T) {
+  return static_cast<int>((clamp_len(len, capacity) + unit - 1) / unit) + (T + unit - 1) / unit;
+}
+// sums over the lanes up to this one
+__device__ __forceinline__ int sum_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(sum_upto(v), 63); }
+__device__ __forceinline__ int wave_most(int v) {
+  auto join = [&](int w) { v = v > w ? v : w; };
+  join(__builtin_amdgcn_update_dpp(v, v, 0x111, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(v, v, 0x112, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(v, v, 0x114, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(v, v, 0x118, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+// (the lanes hold the units of the first 64 sequences: lengths are read once unless there are more)
+struct Sequences {
+  const int* lens;
+  int batch, unit, T;
+  int64_t capacity;
+  int units0;
+  __device__ __forceinline__ Sequences(const TreeArgs& a, int batch_, int unit_, int lane)
+      : lens(a.lens), batch(batch_), unit(unit_), T(a.T), capacity(a.capacity), units0(lane < batch_ ? units_of(a.lens[lane], a.capacity, unit_, a.T) : 0) {}
+  __device__ __forceinline__ int units(int c, int lane) const { return c == 0 ? units0 : c + lane < batch ? units_of(lens[c + lane], capacity, unit, T) : 0; }
+};
+__device__ __forceinline__ int deal(const Sequences& s, int budget, int least, int most, int lane) {
+  int total = 0, longest = 0;
+  for (int c = 0; c < s.batch; c += 64) {
+    const int units = s.units(c, lane);
+    total += wave_total(units);
+    const int top = wave_most(units);
+    longest = longest > top ? longest : top;
+  }
+  int per = (total + budget - 1) / budget;
+  per = per > least ? per : least;
+  per = per > (longest + most - 1) / most ? per : (longest + most - 1) / most;
+  for (;;) {  // (per grows until the parts fit; with per = longest every sequence is one part, and budget >= batch)
+    int parts = 0;
+    for (int c = 0; c < s.batch; c += 64) parts += wave_total((s.units(c, lane) + per - 1) / per);
+    if (parts <= budget || per >= longest) return per > longest ? longest : per;
+    const int more = static_cast<int>(static_cast<float>(per) * parts / budget);
+    per = more > per ? more : per + 1;
+  }
+}
+// the part that has `slot`, or (slot < 0) the parts of sequence b
+__device__ __forceinline__ Part find_part(const TreeArgs& a, int batch, int unit, int slot, int b, int budget, int least, int most, int lane) {
+  if (budget == 0) return slot >= 0 ? Part{slot, 0, 1, slot} : Part{b, 0, 1, b};
+  if (batch == 1) {
+    const int units = units_of(a.lens[0], a.capacity, unit, a.T);
+    int per = (units + budget - 1) / budget;
+    per = per > least ? per : least;
+    const int parts = (units + per - 1) / per;
+    return Part{slot < parts ? 0 : -1, slot, parts, 0};
+  }
+  const Sequences s(a, batch, unit, lane);
+  const int per = deal(s, budget, least, most, lane);
+  int base = 0;
+  for (int c = 0; c < batch; c += 64) {
+    const int parts = (s.units(c, lane) + per - 1) / per;
+    const int upto = sum_upto(parts);
+    const uint64_t here = slot >= 0 ? __builtin_amdgcn_ballot_w64(slot >= base + upto - parts && slot < base + upto) : b < c + 64 ? uint64_t{1} << (b - c) : 0;
+    if (here) {
+      const int l = __builtin_ctzll(here);
+      const int n = __builtin_amdgcn_readlane(parts, l), first = base + __builtin_amdgcn_readlane(upto, l) - n;
+      return Part{c + l, slot - first, n, first};
+    }
+    base += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return Part{-1, 0, 0, 0};
+}
+
+// Where a unit of keys lies: in the cache, or among the nodes' own.  Rows behind the last valid key repeat that one.
+struct Keys {
+  const char *k, *v;
+  unsigned stride;  // bytes between keys (a unit's rows lie within 4 GiB)
+  int valid;
+};
+template <int UNIT>
+__device__ __forceinline__ Keys keys_of(const TreeArgs& a, int b, int hk, int64_t len, int cached, int at) {
+  if (at < cached) {
+    const int64_t from = ((static_cast<int64_t>(b) * a.kv_heads + hk) * a.capacity + static_cast<int64_t>(at) * UNIT) * a.d;
+    return {reinterpret_cast<const char*>(a.Kc + from), reinterpret_cast<const char*>(a.Vc + from), 2u * a.d, static_cast<int>(len - static_cast<int64_t>(at) * UNIT)};
+  }
+  const int node = (at - cached) * UNIT;
+  const int64_t from = ((static_cast<int64_t>(b) * a.T + node) * a.kv_heads + hk) * a.d;
+  return {reinterpret_cast<const char*>(a.K + from), reinterpret_cast<const char*>(a.V + from), 2u * a.kv_heads * a.d, a.T - node};
+}
+
+// The 8 channels of k step `ks` that a lane of `quarter` holds
+template <int DP>
+__device__ __forceinline__ f16x8 load_channels(const char* row, int ks, int quarter, int d) {
+  const int at = ks * 32 + quarter * 8;
+  if (ks * 32 + 32 <= below(DP)) return *reinterpret_cast<const f16x8*>(row + at * 2);
+  const f16x8 v = *reinterpret_cast<const f16x8*>(row + (at < d ? at : d - 8) * 2);
+  return at < d ? v : f16x8{};
+}
+
+// Q's 8 channels, with the scale's sign: the scale itself is positive (one, where it was nought), so that a row's largest product has its largest score
+template <int DP>
+__device__ __forceinline__ f16x8 load_query(const half_t* row, int ks, int quarter, int d, half_t sign) {
+  return load_channels<DP>(reinterpret_cast<const char*>(row), ks, quarter, d) * sign;
+}
+
+// A weight per key from the products of one row tile, NK key tiles: mask, running maximum and sum, O rescaled where the maximum moved.
+// `shown` says which of the keys 16 kt + 4 (lane >> 4) + j the row sees (bit 16 kt + ..), all: none is hidden.
+template <int NK, int DT>
+__device__ __forceinline__ void weigh(f32x4 (&s)[NK], bool all, uint64_t shown, int quarter, float scale_log2, float& top, float& sum, f32x4 (&o)[DT]) {
+  float best = -INFINITY;
+  if (!all) {
+    const uint64_t mine = shown >> (4 * quarter);
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[kt][j] = (mine >> (16 * kt + j)) & 1 ? s[kt][j] : -INFINITY;
+  }
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) best = fmaxf(best, s[kt][j]);
+  best = fmaxf(max_of_row(best), top);
+  if (__builtin_amdgcn_ballot_w64(best > top) != 0) {
+    const float keep = best == -INFINITY ? 1.f : exp2_fast((top - best) * scale_log2);
+    sum *= keep;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[dt][j] *= keep;
+    top = best;
+  }
+  const float from = best == -INFINITY ? 0.f : -best * scale_log2;
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[kt][j] = exp2_fast(fmaf(s[kt][j], scale_log2, from));
+      sum += s[kt][j];
+    }
+}
+__device__ __forceinline__ f16x8 weights_f16(const f32x4& a, const f32x4& b) {
+  return f16x8{static_cast<half_t>(a[0]), static_cast<half_t>(a[1]), static_cast<half_t>(a[2]), static_cast<half_t>(a[3]),
+               static_cast<half_t>(b[0]), static_cast<half_t>(b[1]), static_cast<half_t>(b[2]), static_cast<half_t>(b[3])};
+}
+__device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1; }
+
+// A value that is no number, in the 16 bytes of a piece
+__device__ __forceinline__ bool no_number(const u32x4& v) {
+  bool bad = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) bad = bad || (v[w] & 0x7c00u) == 0x7c00u || (v[w] & 0x7c000000u) == 0x7c000000u;
+  return bad;
+}
+// Values of a node that are no numbers must not meet the zero weights of the rows that do not see it: such nodes (rare) are multiplied out
+// key by key, a row adding up what it sees.  32 nodes from `base` on; s: their weights; `room`: 2 KiB of the LDS, the wavefront's own.
+template <int DT>
+__device__ __forceinline__ void add_key_by_key(const TreeArgs& a, int b, int hk, int base, const f32x4& s0, const f32x4& s1, uint64_t sees, float* room,
+                                               int lane, f32x4 (&o)[DT]) {
+  const int quarter = lane >> 4, i16 = lane & 15;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    room[(4 * quarter + j) * 16 + i16] = s0[j];
+    room[(16 + 4 * quarter + j) * 16 + i16] = s1[j];
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int key = 0; key < 32 && base + key < a.T; ++key) {
+    const float weight = room[key * 16 + i16];
+    const half_t* v = a.V + ((static_cast<int64_t>(b) * a.T + base + key) * a.kv_heads + hk) * a.d;
+    if ((sees >> (base + key)) & 1) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (dt * 16 + 4 * quarter < a.d) o[dt][j] = fmaf(weight, static_cast<float>(v[dt * 16 + 4 * quarter + j]), o[dt][j]);
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+__device__ __forceinline__ half_t* out_row(const TreeArgs& a, int b, int hk, int g, int r) {
+  return a.out + ((static_cast<int64_t>(b) * a.Tq + r / g) * a.heads + hk * g + r % g) * a.d;
+}
+__device__ __forceinline__ void store_row4(half_t* to, const f32x4& v, float inv) {
+  *reinterpret_cast<f16x4*>(to) = f16x4{static_cast<half_t>(v[0] * inv), static_cast<half_t>(v[1] * inv), static_cast<half_t>(v[2] * inv), static_cast<half_t>(v[3] * inv)};
+}
+// ---- parts of a sequence's keys: each leaves its rows' sums, and behind them their maxima and weights, in the workspace; whoever arrives last
+// joins them in their order.  The shares pass the L2 (the XCDs' are not coherent): once a part's stores have drained they are visible everywhere, and
+// only then is its arrival counted.
+__device__ __forceinline__ void store_stat(float* share, int rows, int DP, int r, float top, float sum) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(share + rows * DP) + r,
+                     static_cast<uint64_t>(__builtin_bit_cast(unsigned, top)) | static_cast<uint64_t>(__builtin_bit_cast(unsigned, sum)) << 32, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool last_to_arrive(unsigned* counter, int parts, int* flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = before == static_cast<unsigned>(parts) - 1;
+    if (*flag) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed for the next launch
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+template <int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void join_parts(const TreeArgs& a, int b, int hk, int g, int row0, int my_rows, const float* shares, int parts, uint64_t* stats) {
+  constexpr int kShare = ROWS * (DP + 2);
+  const int tid = threadIdx.x;
+  for (int at = tid; at < parts * ROWS; at += THREADS)
+    if (at % ROWS < my_rows)
+      stats[at] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(at / ROWS) * kShare + ROWS * DP) + at % ROWS, __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  for (int at = tid; at < my_rows * (DP / 4); at += THREADS) {
+    const int i = at / (DP / 4), c = 4 * (at % (DP / 4));
+    if (c >= a.d) continue;
+    float best = -INFINITY, l = 0.f;
+    for (int y = 0; y < parts; ++y) best = fmaxf(best, __builtin_bit_cast(float, static_cast<unsigned>(stats[y * ROWS + i])));
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kAtOnce = 8;  // shares requested before the first is used: a trip to memory per eight parts
+    for (int y0 = 0; y0 < parts; y0 += kAtOnce) {
+      uint64_t one[kAtOnce], other[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int y = y0 + u < parts ? y0 + u : parts - 1;
+        const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(y) * kShare + i * DP + c);
+        one[u] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        other[u] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (y0 + u >= parts) break;
+        const uint64_t two = stats[(y0 + u) * ROWS + i];
+        const float w = weight_of(__builtin_bit_cast(float, static_cast<unsigned>(two)), best, a.scale_log2);
+        l = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(two >> 32)), l);
+        v[0] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u])), v[0]);
+        v[1] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u] >> 32)), v[1]);
+        v[2] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u])), v[2]);
+        v[3] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u] >> 32)), v[3]);
+      }
+    }
+    store_row4(out_row(a, b, hk, g, row0 + i) + c, v, 1.f / l);
+  }
+}
+
+// What a launch is made of: workgroup u has slot u % slots of key head (u / slots) % kv_heads and rows from (u / slots / kv_heads) on.
+struct TreeGrid {
+  int batch, slots, budget, row_groups;
+  float* ws;
+  unsigned* arrivals;
+};
+
+// ---- few rows: the W wavefronts take blocks of 32 keys in turn, each for all 16 RT rows and without a barrier until the end.  A lane's 8 channels
+// of one key are 16 contiguous bytes, K's operand as it lies in memory; V passes through a piece of the LDS that is the wavefront's
+// own.  One block of K and one of V are on their way in registers while the block before is worked on.
+template <int DP, int RT, int W>
+__global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid grid) {
+  constexpr int KS = DP / 32, DT = DP / 16, VL = DP / 16, kBlock = 32;  // k steps, channel tiles, 16-byte pieces of V per lane, keys
+  constexpr int kRows = 16 * RT, kChunks = DP / 8, kWave = kBlock * v_row_bytes(DP);
+  __shared__ __attribute__((aligned(16))) char lds[W * kWave];
+  __shared__ float stat_m[W][kRows], stat_l[W][kRows];
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
+  const int g = a.heads / a.kv_heads, R = a.Tq * g;
+  const int slot = static_cast<int>(blockIdx.x % grid.slots), hk = static_cast<int>(blockIdx.x / grid.slots % a.kv_heads), rg = static_cast<int>(blockIdx.x / grid.slots / a.kv_heads);
+  const Part part = find_part(a, grid.batch, kBlock, slot, 0, grid.budget, W, 64 / RT, lane);
+  if (part.b < 0) return;
+  const int b = part.b;
+  const int64_t len = clamp_len(a.lens[b], a.capacity);
+  const int cached = static_cast<int>((len + kBlock - 1) / kBlock), blocks = cached + (a.T + kBlock - 1) / kBlock;
+  const int first = static_cast<int>(static_cast<int64_t>(blocks) * part.z / part.parts), end = static_cast<int>(static_cast<int64_t>(blocks) * (part.z + 1) / part.parts);
+  const int up = lane < a.T ? a.parents[static_cast<int64_t>(b) * a.T + lane] : -1;
+
+  f16x8 kf[2][KS];
+  u32x4 vf[VL];
+  auto load_k = [&](const Keys& s) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int row = kt * 16 + i16;
+      const unsigned at = static_cast<unsigned>(row < s.valid ? row : s.valid - 1) * s.stride;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = load_channels<DP>(s.k + at, ks, quarter, a.d);
+    }
+  };
+  auto load_v = [&](const Keys& s) {
+#pragma unroll
+    for (int n = 0; n < VL; ++n) {
+      const int id = n * 64 + lane, row = id / kChunks, c = id % kChunks;
+      const unsigned at = static_cast<unsigned>(row < s.valid ? row : s.valid - 1) * s.stride + (c * 8 < a.d ? c : a.d / 8 - 1) * 16;
+      vf[n] = *reinterpret_cast<const u32x4*>(s.v + at);
+    }
+  };
+  // the tree's blocks, two at most, are the last ones: a wavefront has one of them at most, as its last
+  int blk = first + wave;
+  if (blk < end) {
+    const Keys s = keys_of<kBlock>(a, b, hk, len, cached, blk);
+    load_k(s);
+    load_v(s);
+  }
+  f16x8 q[RT][KS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rg * kRows + rt * 16 + i16, have = r < R ? r : R - 1;
+    const half_t* row = a.Q + ((static_cast<int64_t>(b) * a.Tq + have / g) * a.heads + hk * g + have % g) * a.d;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[rt][ks] = load_query<DP>(row, ks, quarter, a.d, a.sign);
+  }
+  uint64_t sees[RT] = {};
+  if (end > cached) see(sees, up, lane, rg * kRows, R, g, a.T, a.Tq);
 
   f32x4 o[RT][DT];
   float top[RT], sum[RT];
@@ -192,44 +492,10 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_g
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-
-  char* mine = lds + wave * wave_bytes(DP);
+  char* mine = lds + wave * kWave;
   const unsigned tr_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)mine)) +
                          (4 * quarter + (i16 >> 2)) * v_row_bytes(DP) + (i16 & 3) * 8;
-  f16x8 kf[2][KS];
-  u32x4 vf[VL];
-  // block `blk`: of the cache, or of the nodes' own keys; rows behind its last valid key repeat that one.  A block's rows lie within 4 GiB
-  struct Block {
-    const char *k, *v;
-    unsigned stride;  // bytes between keys
-    int valid;
-  };
-  auto source = [&](int blk) -> Block {
-    if (blk < cached_blocks) {
-      const int64_t at = (static_cast<int64_t>(bh) * a.capacity + static_cast<int64_t>(blk) * kBlockKeys) * a.d;
-      return {reinterpret_cast<const char*>(a.Kc + at), reinterpret_cast<const char*>(a.Vc + at), 2u * a.d, static_cast<int>(len - static_cast<int64_t>(blk) * kBlockKeys)};
-    }
-    const int node = (blk - cached_blocks) * kBlockKeys;
-    const int64_t at = ((static_cast<int64_t>(b) * a.T + node) * a.kv_heads + hk) * a.d;
-    return {reinterpret_cast<const char*>(a.K + at), reinterpret_cast<const char*>(a.V + at), 2u * a.kv_heads * a.d, a.T - node};
-  };
-  auto load_k = [&](const Block& s) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const int row = kt * 16 + i16;
-      const unsigned at = static_cast<unsigned>(row < s.valid ? row : s.valid - 1) * s.stride + quarter * 16;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = ks * 32 + quarter * 8 < a.d ? *reinterpret_cast<const f16x8*>(s.k + (at + ks * 64)) : f16x8{};
-    }
-  };
-  auto load_v = [&](const Block& s) {
-#pragma unroll
-    for (int n = 0; n < VL; ++n) {
-      const int id = n * 64 + lane, row = id / kChunks, c = id % kChunks;
-      const unsigned at = static_cast<unsigned>(row < s.valid ? row : s.valid - 1) * s.stride + c * 16;
-      vf[n] = c * 8 < a.d ? *reinterpret_cast<const u32x4*>(s.v + at) : u32x4{0u, 0u, 0u, 0u};
-    }
-  };
+
   // one block: the scores from kf, the next block on its way (if there is one), V by way of the LDS
   auto visit = [&](auto tree_tag, int valid, int base, bool more, int next) {
     constexpr bool TREE = decltype(tree_tag)::value;
@@ -242,19 +508,15 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_g
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][ks], q[rt][ks], s[rt][kt], 0, 0, 0);
       }
-    Block coming{};
+    Keys coming{};
     if (!TREE && more) {
-      coming = source(next);
+      coming = keys_of<kBlock>(a, b, hk, len, cached, next);
       load_k(coming);
     }
-    // A value of a node that is no number must not meet the zero weights of the rows that do not see it: such a block (rare) is
-    // multiplied out key by key instead
     bool odd = false;
     if (TREE) {
 #pragma unroll
-      for (int n = 0; n < VL; ++n)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) odd = odd || (vf[n][w] & 0x7c00u) == 0x7c00u || (vf[n][w] & 0x7c000000u) == 0x7c000000u;
+      for (int n = 0; n < VL; ++n) odd = odd || no_number(vf[n]);
       odd = __builtin_amdgcn_ballot_w64(odd) != 0;
     }
     if (!odd) {
@@ -265,55 +527,13 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_g
       }
     }
     if (!TREE && more) load_v(coming);
-
     f16x8 p[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float x[8], best = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = s[rt][e >> 2][e & 3] * a.scale_log2;
-        const int key = (e >> 2) * 16 + 4 * quarter + (e & 3);
-        if (TREE) x[e] = (sees[rt] >> (base + key)) & 1 ? x[e] : -INFINITY;
-        else if (valid < kBlockKeys) x[e] = key < valid ? x[e] : -INFINITY;
-        best = fmaxf(best, x[e]);
-      }
-      best = fmaxf(max_of_row(best), top[rt]);
-      if (__builtin_amdgcn_ballot_w64(best > top[rt]) != 0) {
-        const float keep = best == -INFINITY ? 1.f : exp2_fast(top[rt] - best);
-        sum[rt] *= keep;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[rt][dt][j] *= keep;
-        top[rt] = best;
-      }
-      const float from = best == -INFINITY ? 0.f : best;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = exp2_fast(x[e] - from);
-        sum[rt] += x[e];
-        p[rt][e] = static_cast<half_t>(x[e]);
-      }
-      if (TREE && odd) {
-        // P by way of the LDS; a row adds up the values that it sees
-        float* at_p = reinterpret_cast<float*>(mine);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) at_p[((e >> 2) * 16 + 4 * quarter + (e & 3)) * 16 + i16] = x[e];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        for (int key = 0; key < kBlockKeys && base + key < a.T; ++key) {
-          const float weight = at_p[key * 16 + i16];
-          const half_t* v = a.V + ((static_cast<int64_t>(b) * a.T + base + key) * a.kv_heads + hk) * a.d;
-          if ((sees[rt] >> (base + key)) & 1) {
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (dt * 16 + 4 * quarter < a.d) o[rt][dt][j] = fmaf(weight, static_cast<float>(v[dt * 16 + 4 * quarter + j]), o[rt][dt][j]);
-          }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
+      if (TREE) weigh<2, DT>(s[rt], false, sees[rt] >> base, quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
+      else weigh<2, DT>(s[rt], valid >= kBlock, first_bits(valid), quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
+      p[rt] = weights_f16(s[rt][0], s[rt][1]);
+      if (TREE && odd) add_key_by_key<DT>(a, b, hk, base, s[rt][0], s[rt][1], sees[rt], reinterpret_cast<float*>(mine), lane, o[rt]);
     }
     if (odd) return;
     auto add = [&](int dt, const f16x4& lo, const f16x4& hi) {
@@ -335,17 +555,9 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_g
       add(DT - 1, lo[1], hi[1]);
     }
   };
-
-  // The tree's blocks, two at most, are the last ones: a wavefront has one of them at most, as its last
-  int blk = first + wave;
-  if (blk < end) {
-    const Block s = source(blk);
-    load_k(s);
-    load_v(s);
-  }
-  for (; blk < end && blk < cached_blocks; blk += W)
-    visit(std::false_type{}, static_cast<int>(len - static_cast<int64_t>(blk) * kBlockKeys), 0, blk + W < end, blk + W);
-  if (blk < end) visit(std::true_type{}, 0, (blk - cached_blocks) * kBlockKeys, false, 0);
+  for (; blk < end && blk < cached; blk += W)
+    visit(std::false_type{}, static_cast<int>(len - static_cast<int64_t>(blk) * kBlock < kBlock ? len - static_cast<int64_t>(blk) * kBlock : kBlock), 0, blk + W < end, blk + W);
+  if (blk < end) visit(std::true_type{}, 0, (blk - cached) * kBlock, false, 0);
 
   // ---- the wavefronts' shares, joined in their order
 #pragma unroll
@@ -357,26 +569,23 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_g
     }
   }
   __syncthreads();
-  auto weight_of = [](float m, float best) { return best == -INFINITY ? 0.f : exp2_fast(m - best); };
   auto best_of = [&](int r) {
     float best = stat_m[0][r];
 #pragma unroll
     for (int w = 1; w < W; ++w) best = fmaxf(best, stat_m[w][r]);
     return best;
   };
-  const int tile = bh * row_groups + rg, my_rows = R - rg * kRows < kRows ? R - rg * kRows : kRows;
-  float* share = ws + (static_cast<int64_t>(tile) * nsplit + z) * kPartial;
-  auto out_row = [&](int r) -> half_t* {
-    return a.out + ((static_cast<int64_t>(b) * a.Tq + r / g) * a.heads + hk * g + r % g) * a.d;
-  };
+  const int my_rows = R - rg * kRows < kRows ? R - rg * kRows : kRows, problem = hk * grid.row_groups + rg;
+  float* shares = grid.ws + (static_cast<int64_t>(problem) * grid.slots + part.first) * (kRows * (DP + 2));
+  float* share = shares + static_cast<int64_t>(part.z) * (kRows * (DP + 2));
   constexpr int kPitch = DP + 4;  // floats: the sixteen rows of a store start 16 bytes apart in the banks
-  static_assert(16 * kPitch * 4 <= wave_bytes(DP), "a wavefront's sums of sixteen rows fit its piece of the LDS");
+  static_assert(16 * kPitch * 4 <= kWave, "a wavefront's sums of sixteen rows fit its piece of the LDS");
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row0 = rt * 16;
     if (row0 >= my_rows) break;
     {
-      const float w = weight_of(top[rt], best_of(row0 + i16));
+      const float w = weight_of(top[rt], best_of(row0 + i16), a.scale_log2);
       float* to = reinterpret_cast<float*>(mine) + i16 * kPitch + 4 * quarter;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(to + dt * 16) = f32x4{o[rt][dt][0] * w, o[rt][dt][1] * w, o[rt][dt][2] * w, o[rt][dt][3] * w};
@@ -390,109 +599,277 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, int row_g
       const float best = best_of(r);
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const f32x4 part = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * wave_bytes(DP)) + i * kPitch + c);
+        const f32x4 some = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * kWave) + i * kPitch + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += part[j];
-        l += stat_l[w][r] * weight_of(stat_m[w][r], best);
+        for (int j = 0; j < 4; ++j) v[j] += some[j];
+        l += stat_l[w][r] * weight_of(stat_m[w][r], best, a.scale_log2);
       }
-      if (splits > 1) {
+      if (part.parts > 1) {
         store_out(v, reinterpret_cast<f32x4*>(share + r * DP + c), true);
-        if (c == 0)
-          __hip_atomic_store(reinterpret_cast<uint64_t*>(share + kRows * DP) + r,
-                             static_cast<uint64_t>(__builtin_bit_cast(unsigned, best)) | static_cast<uint64_t>(__builtin_bit_cast(unsigned, l)) << 32,
-                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (c == 0) store_stat(share, kRows, DP, r, best, l);
       } else {
-        const float inv = 1.f / l;
-        *reinterpret_cast<f16x4*>(out_row(rg * kRows + r) + c) = f16x4{static_cast<half_t>(v[0] * inv), static_cast<half_t>(v[1] * inv),
-                                                                       static_cast<half_t>(v[2] * inv), static_cast<half_t>(v[3] * inv)};
+        store_row4(out_row(a, b, hk, g, rg * kRows + r) + c, v, 1.f / l);
       }
     }
     __syncthreads();
   }
-  if (splits == 1) return;
+  if (part.parts == 1 || !last_to_arrive(grid.arrivals + static_cast<int64_t>(problem) * grid.batch + b, part.parts, &flag)) return;
+  static_assert(64 / RT * kRows * 8 <= W * kWave, "the parts' statistics fit the LDS");
+  join_parts<DP, kRows, 64 * W>(a, b, hk, g, rg * kRows, my_rows, shares, part.parts, reinterpret_cast<uint64_t*>(lds));
+}
 
-  // ---- the splits' shares, joined in their order by whoever arrives last.  The shares pass the L2 (the XCDs' are not coherent): once the
-  // stores have drained they are visible everywhere, and only then is the arrival counted
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) {
-    const unsigned before = __hip_atomic_fetch_add(arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last_flag = before == static_cast<unsigned>(splits) - 1;
-    if (last_flag) __hip_atomic_store(arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed for the next launch
+// ---- many rows: each of the W wavefronts has 16 RT rows of its own and sees all the part's keys, 64 at a time, through the LDS, where one tile is
+// worked on while the next is on its way in registers: K and V are read once for up to 16 RT W rows, and no sum crosses wavefronts.
+template <int DP, int RT, int W>
+__global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_kernel(TreeArgs a, TreeGrid grid) {
+  constexpr int KS = DP / 32, DT = DP / 16, kTile = 64, kChunks = DP / 8, kRows = 16 * RT * W;
+  constexpr int kPieces = (kTile * kChunks + 64 * W - 1) / (64 * W);  // 16-byte pieces of K (and of V) per thread and tile
+  constexpr bool kEven = kTile * kChunks % (64 * W) == 0;
+  constexpr int kK = kTile * k_row_bytes(DP), kStage = kK + kTile * v_row_bytes(DP);
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+  __shared__ int odd_values;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
+  const int g = a.heads / a.kv_heads, R = a.Tq * g;
+  const int slot = static_cast<int>(blockIdx.x % grid.slots), hk = static_cast<int>(blockIdx.x / grid.slots % a.kv_heads), rg = static_cast<int>(blockIdx.x / grid.slots / a.kv_heads);
+  const Part part = find_part(a, grid.batch, kTile, slot, 0, grid.budget, 2, 64, lane);
+  if (part.b < 0) return;
+  const int b = part.b;
+  const int64_t len = clamp_len(a.lens[b], a.capacity);
+  const int cached = static_cast<int>((len + kTile - 1) / kTile), tiles = cached + 1;  // (the tree is one tile, the last)
+  const int first = static_cast<int>(static_cast<int64_t>(tiles) * part.z / part.parts), end = static_cast<int>(static_cast<int64_t>(tiles) * (part.z + 1) / part.parts);
+  const int up = lane < a.T ? a.parents[static_cast<int64_t>(b) * a.T + lane] : -1;
+
+  u32x4 kf[kPieces], vf[kPieces];
+  auto load = [&](int at) {
+    const Keys s = keys_of<kTile>(a, b, hk, len, cached, at);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      const int id = n * 64 * W + tid, row = id / kChunks, c = id % kChunks;
+      const bool there = c * 8 < a.d;
+      const unsigned from = static_cast<unsigned>(row < s.valid ? row : s.valid - 1) * s.stride + (there ? c : a.d / 8 - 1) * 16;
+      kf[n] = *reinterpret_cast<const u32x4*>(s.k + from);
+      if (!there) kf[n] = u32x4{0u, 0u, 0u, 0u};
+      vf[n] = *reinterpret_cast<const u32x4*>(s.v + from);
+    }
+  };
+  auto keep = [&](char* stage, bool tree) {
+    bool odd = false;
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      const int id = n * 64 * W + tid, row = id / kChunks, c = id % kChunks;
+      if (!kEven && row >= kTile) break;
+      *reinterpret_cast<u32x4*>(stage + row * k_row_bytes(DP) + c * 16) = kf[n];
+      *reinterpret_cast<u32x4*>(stage + kK + row * v_row_bytes(DP) + c * 16) = vf[n];
+      if (tree) odd = odd || no_number(vf[n]);
+    }
+    if (odd) odd_values = 1;
+  };
+  if (first < end) load(first);
+  const int row0 = rg * kRows + wave * 16 * RT;  // the wavefront's first row
+  f16x8 q[RT][KS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + rt * 16 + i16, have = r < R ? r : R - 1;
+    const half_t* row = a.Q + ((static_cast<int64_t>(b) * a.Tq + have / g) * a.heads + hk * g + have % g) * a.d;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[rt][ks] = load_query<DP>(row, ks, quarter, a.d, a.sign);
   }
-  __syncthreads();
-  if (!last_flag) return;
-  const float* shares = ws + static_cast<int64_t>(tile) * nsplit * kPartial;
-  uint64_t* stats = reinterpret_cast<uint64_t*>(lds);  // [split][row]: maximum and sum; the sum turns into the split's weight
-  for (int at = tid; at < splits * kRows; at += 64 * W)
-    if (at % kRows < my_rows)
-      stats[at] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(at / kRows) * kPartial + kRows * DP) + at % kRows,
-                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  for (int at = tid; at < my_rows * (DP / 4); at += 64 * W) {
-    const int i = at / (DP / 4), c = 4 * (at % (DP / 4));
-    if (c >= a.d) continue;
-    float best = -INFINITY, l = 0.f;
-    for (int y = 0; y < splits; ++y) best = fmaxf(best, __builtin_bit_cast(float, static_cast<unsigned>(stats[y * kRows + i])));
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    constexpr int kAtOnce = 8;  // shares requested before the first is used: a trip to memory per eight splits
-    for (int y0 = 0; y0 < splits; y0 += kAtOnce) {
-      uint64_t one[kAtOnce], other[kAtOnce];
+  if (tid == 0) odd_values = 0;
+  uint64_t sees[RT] = {};
+  if (end > cached) see(sees, up, lane, row0, R, g, a.T, a.Tq);
+  f32x4 o[RT][DT];
+  float top[RT], sum[RT];
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const int y = y0 + u < splits ? y0 + u : splits - 1;
-        const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(y) * kPartial + i * DP + c);
-        one[u] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        other[u] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+  for (int rt = 0; rt < RT; ++rt) {
+    top[rt] = -INFINITY;
+    sum[rt] = 0.f;
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        if (y0 + u >= splits) break;
-        const uint64_t two = stats[(y0 + u) * kRows + i];
-        const float w = weight_of(__builtin_bit_cast(float, static_cast<unsigned>(two)), best);
-        l = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(two >> 32)), l);
-        v[0] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u])), v[0]);
-        v[1] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u] >> 32)), v[1]);
-        v[2] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u])), v[2]);
-        v[3] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u] >> 32)), v[3]);
+    for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // the LDS is written, and read again, behind this; loads of the next tile stay on their way
+  auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  meet();
+  keep(lds, first >= cached);
+  if (first + 1 < end) load(first + 1);
+  meet();
+  const bool has_rows = row0 < R;
+  const unsigned lds_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+  auto visit = [&](auto tree_tag, int valid, int stage, bool odd) {
+    constexpr bool TREE = decltype(tree_tag)::value;
+    const char* k_at = lds + stage * kStage + i16 * k_row_bytes(DP) + quarter * 16;
+    const unsigned tr_at = lds_at + stage * kStage + kK + (4 * quarter + (i16 >> 2)) * v_row_bytes(DP) + (i16 & 3) * 8;
+    f32x4 s[RT][4];
+    f16x8 k[2][KS];  // the operands of two key tiles; the statements between keep more of them from being read ahead
+    auto read_k = [&](int kt) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) k[kt & 1][ks] = *reinterpret_cast<const f16x8*>(k_at + kt * 16 * k_row_bytes(DP) + ks * 64);
+    };
+    read_k(0);
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      asm volatile("" ::: "memory");
+      if (kt < 3) read_k(kt + 1);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[kt & 1][ks], q[rt][ks], s[rt][kt], 0, 0, 0);
+    }
+    f16x8 p[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (TREE) weigh<4, DT>(s[rt], false, sees[rt], quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
+      else weigh<4, DT>(s[rt], valid >= kTile, first_bits(valid), quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
+      p[rt][0] = weights_f16(s[rt][0], s[rt][1]);
+      p[rt][1] = weights_f16(s[rt][2], s[rt][3]);
+      if (TREE && odd) {
+        // (the other stage is free: the tree's tile is the last)
+        float* room = reinterpret_cast<float*>(lds + (stage ^ 1) * kStage) + wave * 512;
+        static_assert(W * 2048 <= kStage, "the wavefronts' weights of 32 keys fit a stage");
+        add_key_by_key<DT>(a, b, hk, 0, s[rt][0], s[rt][1], sees[rt], room, lane, o[rt]);
+        add_key_by_key<DT>(a, b, hk, 32, s[rt][2], s[rt][3], sees[rt], room, lane, o[rt]);
       }
     }
-    const float inv = 1.f / l;
-    *reinterpret_cast<f16x4*>(out_row(rg * kRows + i) + c) = f16x4{static_cast<half_t>(v[0] * inv), static_cast<half_t>(v[1] * inv),
-                                                                   static_cast<half_t>(v[2] * inv), static_cast<half_t>(v[3] * inv)};
+    if (TREE && odd) return;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const unsigned at = tr_at + half * 32 * v_row_bytes(DP);
+      auto add = [&](int dt, const f16x4& lo, const f16x4& hi) {
+        const f16x8 vt = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p[rt][half], o[rt][dt], 0, 0, 0);
+      };
+#pragma unroll
+      for (int dt = 0; dt + 4 <= DT; dt += 4) {
+        f16x4 lo[4], hi[4];
+        read_v<DP>(at + dt * 32, lo, hi);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) add(dt + u, lo[u], hi[u]);
+      }
+      if constexpr (DT % 4 == 2) {
+        f16x4 lo[2], hi[2];
+        read_v<DP>(at + (DT - 2) * 32, lo, hi);
+        add(DT - 2, lo[0], hi[0]);
+        add(DT - 1, lo[1], hi[1]);
+      }
+    }
+  };
+  int stage = 0, at = first;
+  for (; at < end && at < cached; ++at, stage ^= 1) {
+    // the next tile, requested a tile ago, into the other stage; the one behind it on its way; then this one's work
+    if (at + 1 < end) keep(lds + (stage ^ 1) * kStage, at + 1 >= cached);
+    if (at + 2 < end) load(at + 2);
+    if (has_rows) visit(std::false_type{}, static_cast<int>(len - static_cast<int64_t>(at) * kTile < kTile ? len - static_cast<int64_t>(at) * kTile : kTile), stage, false);
+    meet();
+  }
+  if (at < end && has_rows) visit(std::true_type{}, 0, stage, odd_values != 0);
+
+  const int my_rows = R - rg * kRows < kRows ? R - rg * kRows : kRows, problem = hk * grid.row_groups + rg;
+  float* shares = grid.ws + (static_cast<int64_t>(problem) * grid.slots + part.first) * (kRows * (DP + 2));
+  float* share = shares + static_cast<int64_t>(part.z) * (kRows * (DP + 2));
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = wave * 16 * RT + rt * 16 + i16;
+    sum[rt] = sum_of_row(sum[rt]);
+    if (r >= my_rows) continue;
+    const float inv = 1.f / sum[rt];
+    half_t* row = out_row(a, b, hk, g, rg * kRows + r);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int c = dt * 16 + 4 * quarter;
+      if (c >= a.d) continue;
+      if (part.parts > 1) *reinterpret_cast<f32x4*>(share + r * DP + c) = o[rt][dt];
+      else store_row4(row + c, o[rt][dt], inv);
+    }
+    if (part.parts > 1 && quarter == 0)
+      *(reinterpret_cast<uint64_t*>(share + kRows * DP) + r) = static_cast<uint64_t>(__builtin_bit_cast(unsigned, top[rt])) |
+                                                               static_cast<uint64_t>(__builtin_bit_cast(unsigned, sum[rt])) << 32;
   }
 }
 
-template <int DP, int RT, int W>
-int launch_tree(const TreeArgs& a, int64_t batch, hipStream_t s) {
-  constexpr int kRows = 16 * RT;
-  const int64_t groups = ceil_div(static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads), kRows), tiles = batch * a.kv_heads * groups;
-  // a workgroup for each CU, while a split keeps a block of keys per wavefront and the statistics of all splits fit the LDS
-  constexpr int kMostSplits = 64 / RT;
-  int64_t nsplit = kNumCU / tiles;
-  const int64_t blocks = ceil_div(a.capacity, kBlockKeys) + ceil_div(a.T, kBlockKeys), useful = ceil_div(blocks, W);
-  nsplit = nsplit > useful ? useful : nsplit;
-  nsplit = nsplit > kMostSplits ? kMostSplits : nsplit;
-  nsplit = nsplit < 1 ? 1 : nsplit;
-  if (tiles * nsplit > INT32_MAX) return fail("attn_tree: the launch has too many workgroups");
-  static_assert(kMostSplits * kRows * 8 <= W * wave_bytes(DP), "the splits' statistics fit the LDS");
-  float* partials = nullptr;
-  unsigned* arrivals = nullptr;
-  std::unique_lock<std::recursive_mutex> lock;
-  if (nsplit > 1 && split_scratch(s, static_cast<size_t>(tiles * nsplit) * kRows * (DP + 2) * sizeof(float), static_cast<size_t>(tiles),
-                                  static_cast<int>(nsplit), &partials, &arrivals, &lock) != 0)
+// The parts of many rows joined: four rows of one problem and sequence per workgroup, a wavefront each
+template <int DP>
+__global__ void __launch_bounds__(256) attn_tree_join_kernel(TreeArgs a, TreeGrid grid, int rows, int unit, int least, int most) {
+  const int lane = threadIdx.x & 63, g = a.heads / a.kv_heads, R = a.Tq * g;
+  const int r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), hk = blockIdx.y, b = blockIdx.z;
+  const Part part = find_part(a, grid.batch, unit, -1, b, grid.budget, least, most, lane);
+  if (part.parts == 1 || r >= R) return;
+  const int share_size = rows * (DP + 2), i = r % rows;
+  const float* shares = grid.ws + (static_cast<int64_t>(hk * grid.row_groups + r / rows) * grid.slots + part.first) * share_size;
+  // a lane holds a part's maximum and sum (at most 64 parts), then 4 channels
+  uint64_t two = 0xff800000u;
+  if (lane < part.parts) two = *(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(lane) * share_size + rows * DP) + i);
+  const float top = __builtin_bit_cast(float, static_cast<unsigned>(two)), best = wave_max(top), w = weight_of(top, best, a.scale_log2);
+  const float total = wave_sum(w * __builtin_bit_cast(float, static_cast<unsigned>(two >> 32)));
+  const float* from = shares + static_cast<int64_t>(i) * DP + 4 * lane;
+  if (4 * lane >= a.d) from = shares;  // (read, not used)
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  constexpr int kAtOnce = 8;
+  for (int y0 = 0; y0 < part.parts; y0 += kAtOnce) {
+    f32x4 some[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) some[u] = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(y0 + u < part.parts ? y0 + u : part.parts - 1) * share_size);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (y0 + u >= part.parts) break;
+      const float wy = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), y0 + u));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = fmaf(wy, some[u][j], v[j]);
+    }
+  }
+  if (4 * lane < a.d) store_row4(out_row(a, b, hk, g, r) + 4 * lane, v, 1.f / total);
+}
+
+// The launch of a kernel for `rows` rows and `threads` threads per workgroup and parts of at least `least` units of `unit` keys, at most `most` of
+// a sequence: `fill` workgroups for the whole chip
+struct TreeShape {
+  int rows, threads, unit, least, most, fill;
+};
+template <typename Kernel>
+int launch_tree(Kernel kernel, const TreeArgs& a, int64_t batch, int DP, const TreeShape& shape, bool counts, hipStream_t s, TreeGrid* grid, std::unique_lock<std::recursive_mutex>* lock) {
+  const int64_t groups = ceil_div(static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads), shape.rows), problems = a.kv_heads * groups;
+  int64_t budget = shape.fill / problems;
+  const int64_t useful = batch * ceil_div(ceil_div(a.capacity, shape.unit) + ceil_div(a.T, shape.unit), shape.least), limit = batch * shape.most;
+  budget = budget > useful ? useful : budget;
+  budget = budget > limit ? limit : budget;
+  if (budget <= batch) budget = 0;  // every sequence in one piece
+  const int64_t slots = budget == 0 ? batch : budget;
+  if (batch > INT32_MAX || problems * slots > INT32_MAX) return fail("attn_tree: the launch has too many workgroups");
+  *grid = TreeGrid{static_cast<int>(batch), static_cast<int>(slots), static_cast<int>(budget), static_cast<int>(groups), nullptr, nullptr};
+  if (budget > 0 && split_scratch(s, static_cast<size_t>(problems * slots) * shape.rows * (DP + 2) * sizeof(float), counts ? static_cast<size_t>(problems * batch) : 1,
+                                  static_cast<int>(budget), &grid->ws, &grid->arrivals, lock) != 0)
     return -1;
-  hipLaunchKernelGGL((attn_tree_kernel<DP, RT, W>), dim3(static_cast<unsigned>(tiles * nsplit)), dim3(64 * W), 0, s, a, static_cast<int>(groups),
-                     static_cast<int>(nsplit), partials, arrivals);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(problems * slots)), dim3(shape.threads), 0, s, a, *grid);
+  return check_launch("attn_tree");
+}
+template <int DP, int RT, int W>
+int launch_few(const TreeArgs& a, int64_t batch, hipStream_t s) {
+  TreeGrid grid;
+  std::unique_lock<std::recursive_mutex> lock;
+  return launch_tree(attn_tree_kernel<DP, RT, W>, a, batch, DP, TreeShape{16 * RT, 64 * W, 32, W, 64 / RT, kNumCU}, true, s, &grid, &lock);
+}
+template <int DP, int RT, int W>
+int launch_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
+  TreeGrid grid;
+  std::unique_lock<std::recursive_mutex> lock;  // (held until the kernel that joins the parts is enqueued as well)
+  const TreeShape shape{16 * RT * W, 64 * W, 64, 2, 64, kNumCU};
+  if (launch_tree(attn_tree_rows_kernel<DP, RT, W>, a, batch, DP, shape, false, s, &grid, &lock) != 0) return -1;
+  if (grid.budget == 0) return 0;
+  const int64_t rows = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
+  hipLaunchKernelGGL(attn_tree_join_kernel<DP>, dim3(static_cast<unsigned>(ceil_div(rows, 4)), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
+                     dim3(256), 0, s, a, grid, shape.rows, shape.unit, shape.least, shape.most);
   return check_launch("attn_tree");
 }
 
 template <int DP>
 int launch_tree_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
-  if (rows <= 16) return launch_tree<DP, 1, (DP <= 128 ? 8 : 4)>(a, batch, s);
-  if (rows <= 32 || DP > 128) return launch_tree<DP, 2, (DP <= 128 ? 8 : 4)>(a, batch, s);  // (more sums than 512 registers hold, beyond 128 channels)
-  if constexpr (DP <= 128) return launch_tree<DP, 4, 4>(a, batch, s);
+  if (rows <= 16) return launch_few<DP, 1, (DP <= 128 ? 8 : 4)>(a, batch, s);
+  if (rows <= 32) return launch_few<DP, 2, (DP <= 128 ? 8 : 4)>(a, batch, s);
+  if (rows <= 64) return launch_rows<DP, 1, 4>(a, batch, s);
+  if (rows <= 128 || DP > 128) return launch_rows<DP, 1, 8>(a, batch, s);
+  if constexpr (DP <= 128) return launch_rows<DP, 2, 8>(a, batch, s);
 }
 
 }  // namespace
@@ -525,7 +902,7 @@ extern "C" int dtas_attn_tree_f16(const void* Q, const void* K, const void* V, c
   TreeArgs a{static_cast<const half_t*>(Q), static_cast<const half_t*>(K), static_cast<const half_t*>(V), static_cast<const half_t*>(K_cache),
              static_cast<const half_t*>(V_cache), static_cast<const int*>(lens), static_cast<const int*>(parents), static_cast<half_t*>(out),
              static_cast<int>(nodes), static_cast<int>(rows), static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(d), capacity,
-             scale * 1.4426950408889634f};
+             scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f, static_cast<half_t>(scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (d % 8 == 0 && aligned(Q, 16) && aligned(K, 16) && aligned(V, 16) && aligned(K_cache, 16) && aligned(V_cache, 16) && aligned(out, 16)) {
     if (d <= 64) return launch_tree_rows<64>(a, batch, s);
