@@ -294,8 +294,11 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[NK], bool all, uint64_t shown, 
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) best = fmaxf(best, s[kt][j]);
+  // The sums are kept relative to a maximum that moves only when a row's largest score leaves it behind by more than 2^8: weights of up to 256 fit fp16 as
+  // well as those up to 1 (and the sums fp32), and O is rescaled in few tiles instead of in most.
+  constexpr float kAhead = 8.f;
   best = fmaxf(max_of_row(best), top);
-  if (__builtin_amdgcn_ballot_w64(best > top) != 0) {
+  if (__builtin_amdgcn_ballot_w64((best - top) * scale_log2 > kAhead) != 0) {
     const float keep = best == -INFINITY ? 1.f : exp2_fast((top - best) * scale_log2);
     sum *= keep;
 #pragma unroll
@@ -304,7 +307,7 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[NK], bool all, uint64_t shown, 
       for (int j = 0; j < 4; ++j) o[dt][j] *= keep;
     top = best;
   }
-  const float from = best == -INFINITY ? 0.f : -best * scale_log2;
+  const float from = top == -INFINITY ? 0.f : -top * scale_log2;
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
@@ -428,6 +431,12 @@ struct TreeGrid {
 // ---- few rows: the W wavefronts take blocks of 32 keys in turn, each for all 16 RT rows and without a barrier until the end.  A lane's 8 channels
 // of one key are 16 contiguous bytes, K's operand as it lies in memory; V passes through a piece of the LDS that is the wavefront's
 // own.  One block of K and one of V are on their way in registers while the block before is worked on.
+// 4 keys of one channel, from 8 bytes of the LDS that each lane names
+__device__ __forceinline__ f16x4 read_transposed(const char* at) {
+  typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 fp16x4;
+  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)at));
+}
+
 template <int DP, int RT, int W>
 __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid grid) {
   constexpr int KS = DP / 32, DT = DP / 16, VL = DP / 16, kBlock = 32;  // k steps, channel tiles, 16-byte pieces of V per lane, keys
@@ -618,15 +627,21 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid 
   join_parts<DP, kRows, 64 * W>(a, b, hk, g, rg * kRows, my_rows, shares, part.parts, reinterpret_cast<uint64_t*>(lds));
 }
 
-// ---- many rows: each of the W wavefronts has 16 RT rows of its own and sees all the part's keys, 64 at a time, through the LDS, where one tile is
-// worked on while the next is on its way in registers: K and V are read once for up to 16 RT W rows, and no sum crosses wavefronts.
+// ---- many rows: each of the W wavefronts has 16 RT rows of its own and sees all the part's keys, 64 at a time, through the LDS (two stages of K, two
+// of V): K and V are read once for up to 16 RT W rows, and no sum crosses wavefronts.  A tile is two steps: V(t) turns its scores into weights
+// (vector instructions), M(t) multiplies them with its values and the next tile's keys with Q (the matrix cores).  With eight wavefronts the second four
+// run one step behind the first, so that each SIMD has one wavefront in either step; left to themselves the two do the same at the same
+// time (256 rows of 128 against 65533 keys, 8 key heads: 118 us, with the turns 101 .. 110).
+//   tile t's keys are read in M(t - 1), its values in M(t): steps 2 t - 1 and 2 t + 1 of the first four, one later of the others.  What a wavefront
+//   loaded of K it stores in V(t) for tile t + 1 (the others: t + 2), of V for tile t (t + 1): behind the last reads of the tile that had the
+//   stage before, and a barrier ahead of the first of its own.
 template <int DP, int RT, int W>
 __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_kernel(TreeArgs a, TreeGrid grid) {
   constexpr int KS = DP / 32, DT = DP / 16, kTile = 64, kChunks = DP / 8, kRows = 16 * RT * W;
   constexpr int kPieces = (kTile * kChunks + 64 * W - 1) / (64 * W);  // 16-byte pieces of K (and of V) per thread and tile
-  constexpr bool kEven = kTile * kChunks % (64 * W) == 0;
-  constexpr int kK = kTile * k_row_bytes(DP), kStage = kK + kTile * v_row_bytes(DP);
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+  constexpr bool kEven = kTile * kChunks % (64 * W) == 0, kTurns = W == 8;
+  constexpr int kK = kTile * k_row_bytes(DP), kV = kTile * v_row_bytes(DP);
+  __shared__ __attribute__((aligned(16))) char lds_k[2 * kK], lds_v[2 * kV];
   __shared__ int odd_values;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
   const int g = a.heads / a.kv_heads, R = a.Tq * g;
@@ -639,32 +654,53 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * part.z / part.parts), end = static_cast<int>(static_cast<int64_t>(tiles) * (part.z + 1) / part.parts);
   const int up = lane < a.T ? a.parents[static_cast<int64_t>(b) * a.T + lane] : -1;
 
+  // A thread's pieces of a tile: the same rows and channels of every tile.  Whole tiles of the cache follow each other at one distance; channels behind the
+  // head's last repeat its last ones and are not stored (K's are cleared once, V's reach no sum that is stored).
   u32x4 kf[kPieces], vf[kPieces];
-  auto load = [&](int at) {
+  unsigned from_at[kPieces];
+  const char* cache_k = reinterpret_cast<const char*>(a.Kc + (static_cast<int64_t>(b) * a.kv_heads + hk) * a.capacity * a.d);
+  const char* cache_v = reinterpret_cast<const char*>(a.Vc + (static_cast<int64_t>(b) * a.kv_heads + hk) * a.capacity * a.d);
+#pragma unroll
+  for (int n = 0; n < kPieces; ++n) {
+    const int id = n * 64 * W + tid, row = id / kChunks, c = id % kChunks;
+    from_at[n] = static_cast<unsigned>(row < kTile ? row : kTile - 1) * 2u * a.d + (c * 8 < a.d ? c : a.d / 8 - 1) * 16;
+  }
+  auto load = [&](u32x4 (&into)[kPieces], bool values, int at) {
+    if (static_cast<int64_t>(at + 1) * kTile <= len) {
+      const char* from = (values ? cache_v : cache_k) + static_cast<int64_t>(at) * (kTile * 2 * a.d);
+#pragma unroll
+      for (int n = 0; n < kPieces; ++n) into[n] = *reinterpret_cast<const u32x4*>(from + from_at[n]);
+      return;
+    }
     const Keys s = keys_of<kTile>(a, b, hk, len, cached, at);
+    const char* from = values ? s.v : s.k;
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
       const int id = n * 64 * W + tid, row = id / kChunks, c = id % kChunks;
-      const bool there = c * 8 < a.d;
-      const unsigned from = static_cast<unsigned>(row < s.valid ? row : s.valid - 1) * s.stride + (there ? c : a.d / 8 - 1) * 16;
-      kf[n] = *reinterpret_cast<const u32x4*>(s.k + from);
-      if (!there) kf[n] = u32x4{0u, 0u, 0u, 0u};
-      vf[n] = *reinterpret_cast<const u32x4*>(s.v + from);
+      into[n] = *reinterpret_cast<const u32x4*>(from + (static_cast<unsigned>(row < s.valid ? row : s.valid - 1) * s.stride + (c * 8 < a.d ? c : a.d / 8 - 1) * 16));
     }
   };
-  auto keep = [&](char* stage, bool tree) {
-    bool odd = false;
+  auto keep = [&](char* stage, int row_bytes, const u32x4 (&what)[kPieces]) {
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
       const int id = n * 64 * W + tid, row = id / kChunks, c = id % kChunks;
       if (!kEven && row >= kTile) break;
-      *reinterpret_cast<u32x4*>(stage + row * k_row_bytes(DP) + c * 16) = kf[n];
-      *reinterpret_cast<u32x4*>(stage + kK + row * v_row_bytes(DP) + c * 16) = vf[n];
-      if (tree) odd = odd || no_number(vf[n]);
+      if (c * 8 < a.d) *reinterpret_cast<u32x4*>(stage + row * row_bytes + c * 16) = what[n];
     }
-    if (odd) odd_values = 1;
   };
-  if (first < end) load(first);
+  auto keep_k = [&](int at) { keep(lds_k + (at & 1) * kK, k_row_bytes(DP), kf); };
+  auto keep_v = [&](int at) {
+    keep(lds_v + (at & 1) * kV, v_row_bytes(DP), vf);
+    if (at >= cached) {
+      bool odd = false;
+#pragma unroll
+      for (int n = 0; n < kPieces; ++n) odd = odd || no_number(vf[n]);
+      if (odd) odd_values = 1;
+    }
+  };
+  const int behind = kTurns ? wave / (W / 2) : 0;  // 1: one step behind
+  load(kf, false, first);
+  load(vf, true, first);
   const int row0 = rg * kRows + wave * 16 * RT;  // the wavefront's first row
   f16x8 q[RT][KS];
 #pragma unroll
@@ -675,6 +711,8 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
     for (int ks = 0; ks < KS; ++ks) q[rt][ks] = load_query<DP>(row, ks, quarter, a.d, a.sign);
   }
   if (tid == 0) odd_values = 0;
+  if (a.d < DP)
+    for (int at = tid; at < 2 * kK / 16; at += 64 * W) reinterpret_cast<u32x4*>(lds_k)[at] = u32x4{0u, 0u, 0u, 0u};
   uint64_t sees[RT] = {};
   if (end > cached) see(sees, up, lane, row0, R, g, a.T, a.Tq);
   f32x4 o[RT][DT];
@@ -686,84 +724,133 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // the LDS is written, and read again, behind this; loads of the next tile stay on their way
+  // the LDS is written, and read again, behind this; loads of the next tiles stay on their way
   auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   meet();
-  keep(lds, first >= cached);
-  if (first + 1 < end) load(first + 1);
+  keep_k(first);
+  if (first + 1 < end) load(kf, false, first + 1);
+  if (behind) {
+    keep_v(first);
+    if (first + 1 < end) {
+      load(vf, true, first + 1);
+      keep_k(first + 1);
+      if (first + 2 < end) load(kf, false, first + 2);
+    }
+  }
   meet();
   const bool has_rows = row0 < R;
-  const unsigned lds_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-  auto visit = [&](auto tree_tag, int valid, int stage, bool odd) {
-    constexpr bool TREE = decltype(tree_tag)::value;
-    const char* k_at = lds + stage * kStage + i16 * k_row_bytes(DP) + quarter * 16;
-    const unsigned tr_at = lds_at + stage * kStage + kK + (4 * quarter + (i16 >> 2)) * v_row_bytes(DP) + (i16 & 3) * 8;
-    f32x4 s[RT][4];
-    f16x8 k[2][KS];  // the operands of two key tiles; the statements between keep more of them from being read ahead
-    auto read_k = [&](int kt) {
+  const char* k_at = lds_k + i16 * k_row_bytes(DP) + quarter * 16;
+  const char* v_at = lds_v + (4 * quarter + (i16 >> 2)) * v_row_bytes(DP) + (i16 & 3) * 8;
+  f32x4 s[RT][4];
+  f16x8 p[RT][2];
+  // Step M's two halves as one chain: each batch of operands (channel tiles of V^T, a key tile of K) is read ahead of the MFMAs of the batch before it,
+  // and waited for behind them; the barriers to the scheduler keep it so.
+  constexpr int kBatch = DT % 4 == 0 ? 4 : 2, kBatches = 2 * DT / kBatch;  // channel tiles per batch, batches of both halves
+  f16x4 vt[2][kBatch][2];
+  f16x8 kt[2][KS];
+  auto read_v_batch = [&](int at, int n) {
+    const char* from = v_at + (at & 1) * kV + (n / (DT / kBatch)) * 32 * v_row_bytes(DP) + (n % (DT / kBatch)) * kBatch * 32;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) k[kt & 1][ks] = *reinterpret_cast<const f16x8*>(k_at + kt * 16 * k_row_bytes(DP) + ks * 64);
-    };
-    read_k(0);
+    for (int u = 0; u < kBatch; ++u)
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      asm volatile("" ::: "memory");
-      if (kt < 3) read_k(kt + 1);
+      for (int h = 0; h < 2; ++h) vt[n & 1][u][h] = read_transposed(from + u * 32 + h * 16 * v_row_bytes(DP));
+  };
+  auto read_k_tile = [&](int at, int n) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ks = 0; ks < KS; ++ks) kt[n & 1][ks] = *reinterpret_cast<const f16x8*>(k_at + (at & 1) * kK + n * 16 * k_row_bytes(DP) + ks * 64);
+  };
+  auto landed = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto score = [&](int at) {  // (the first key tile of it is there)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (n < 3) read_k_tile(at, n + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[kt & 1][ks], q[rt][ks], s[rt][kt], 0, 0, 0);
+        for (int rt = 0; rt < RT; ++rt) s[rt][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kt[n & 1][ks], q[rt][ks], s[rt][n], 0, 0, 0);
+      if (n < 3) landed();
     }
-    f16x8 p[RT][2];
+  };
+  auto values = [&](int at, bool more) {
+    read_v_batch(at, 0);
+    landed();
+#pragma unroll
+    for (int n = 0; n < kBatches; ++n) {
+      if (n + 1 < kBatches) read_v_batch(at, n + 1);
+      else if (more) read_k_tile(at + 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int dt = (n % (DT / kBatch)) * kBatch + u;
+        const f16x4 lo = vt[n & 1][u][0], hi = vt[n & 1][u][1];
+        const f16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(both, p[rt][n / (DT / kBatch)], o[rt][dt], 0, 0, 0);
+      }
+      landed();
+    }
+  };
+  auto weights = [&](bool all, int64_t valid) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      if (TREE) weigh<4, DT>(s[rt], false, sees[rt], quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
-      else weigh<4, DT>(s[rt], valid >= kTile, first_bits(valid), quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
+      weigh<4, DT>(s[rt], all, valid < 0 ? sees[rt] : first_bits(static_cast<int>(valid)), quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
       p[rt][0] = weights_f16(s[rt][0], s[rt][1]);
       p[rt][1] = weights_f16(s[rt][2], s[rt][3]);
-      if (TREE && odd) {
-        // (the other stage is free: the tree's tile is the last)
-        float* room = reinterpret_cast<float*>(lds + (stage ^ 1) * kStage) + wave * 512;
-        static_assert(W * 2048 <= kStage, "the wavefronts' weights of 32 keys fit a stage");
+    }
+  };
+  // step V's part in the staging: what was loaded a tile ago into its stages, the next on its way
+  auto pass_on = [&](int at) {
+    const int tk = at + 1 + behind, tv = at + behind;
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) asm volatile("" : "+v"(kf[n]), "+v"(vf[n]));  // (they are there, whichever way the branches go)
+    if (tk < end) keep_k(tk);
+    if (tv < end) keep_v(tv);
+    if (tk + 1 < end) load(kf, false, tk + 1);
+    if (tv + 1 < end) load(vf, true, tv + 1);
+  };
+  if (has_rows) {
+    read_k_tile(first, 0);
+    landed();
+    score(first);
+  }
+  if (kTurns && behind) meet();
+  int at = first;
+  for (; at < end && at < cached; ++at) {
+    pass_on(at);
+    if (has_rows) weights(len - static_cast<int64_t>(at) * kTile >= kTile, len - static_cast<int64_t>(at) * kTile < kTile ? len - static_cast<int64_t>(at) * kTile : kTile);
+    meet();
+    if (has_rows) {
+      values(at, at + 1 < end);
+      if (at + 1 < end) score(at + 1);
+    }
+    if (kTurns) meet();
+  }
+  if (at < end) {  // the tree's tile
+    pass_on(at);
+    if (has_rows) weights(false, -1);
+    meet();
+    if (has_rows && odd_values != 0) {
+      // (no keys are read any more: their stages are free)
+      float* room = reinterpret_cast<float*>(lds_k) + wave * 512;
+      static_assert(W * 2048 <= 2 * kK, "the wavefronts' weights of 32 keys fit the stages of K");
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
         add_key_by_key<DT>(a, b, hk, 0, s[rt][0], s[rt][1], sees[rt], room, lane, o[rt]);
         add_key_by_key<DT>(a, b, hk, 32, s[rt][2], s[rt][3], sees[rt], room, lane, o[rt]);
       }
+    } else if (has_rows) {
+      values(at, false);
     }
-    if (TREE && odd) return;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const unsigned at = tr_at + half * 32 * v_row_bytes(DP);
-      auto add = [&](int dt, const f16x4& lo, const f16x4& hi) {
-        const f16x8 vt = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p[rt][half], o[rt][dt], 0, 0, 0);
-      };
-#pragma unroll
-      for (int dt = 0; dt + 4 <= DT; dt += 4) {
-        f16x4 lo[4], hi[4];
-        read_v<DP>(at + dt * 32, lo, hi);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) add(dt + u, lo[u], hi[u]);
-      }
-      if constexpr (DT % 4 == 2) {
-        f16x4 lo[2], hi[2];
-        read_v<DP>(at + (DT - 2) * 32, lo, hi);
-        add(DT - 2, lo[0], hi[0]);
-        add(DT - 1, lo[1], hi[1]);
-      }
-    }
-  };
-  int stage = 0, at = first;
-  for (; at < end && at < cached; ++at, stage ^= 1) {
-    // the next tile, requested a tile ago, into the other stage; the one behind it on its way; then this one's work
-    if (at + 1 < end) keep(lds + (stage ^ 1) * kStage, at + 1 >= cached);
-    if (at + 2 < end) load(at + 2);
-    if (has_rows) visit(std::false_type{}, static_cast<int>(len - static_cast<int64_t>(at) * kTile < kTile ? len - static_cast<int64_t>(at) * kTile : kTile), stage, false);
-    meet();
+    if (kTurns) meet();
   }
-  if (at < end && has_rows) visit(std::true_type{}, 0, stage, odd_values != 0);
+  if (kTurns && !behind) meet();
 
   const int my_rows = R - rg * kRows < kRows ? R - rg * kRows : kRows, problem = hk * grid.row_groups + rg;
   float* shares = grid.ws + (static_cast<int64_t>(problem) * grid.slots + part.first) * (kRows * (DP + 2));
