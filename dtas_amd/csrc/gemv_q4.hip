@@ -47,14 +47,15 @@ __global__ void __launch_bounds__(256) gemv_q4_scalar_kernel(const half_t* __res
 }
 
 // ---- rows on 16-byte boundaries: the matrix cores -------------------------------------------------------------------------------
-// A wavefront takes 16 NT columns and every W-th chunk of 128 k; the W wavefronts of a workgroup (and the workgroups that share a long K) join their sums at
-// the end.  A lane loads 16 bytes of one row of W, 32 weights: the four lanes of a column hold 128.  Two exchanges of halves and two of quarters
-// turn the four words around, so that word i of the four lanes is the i-th 32 weights in order, which is an operand of
-// v_mfma_f32_16x16x32_f16 once it is fp16.  Seven instructions do that: the bytes' nibbles, even and odd, and four permutes that put
-// them into halves.  A nibble as the bits of an fp16 number is nibble * 2^-24, a subnormal, which the matrix cores take as it is: no
+// A wavefront takes 16 columns and chunks of 128 k.  A lane loads 16 bytes of one row of W, 32 weights: the four lanes of a column hold a chunk.  Two
+// exchanges of halves and two of quarters turn the four words around, so that word i of the four lanes is the i-th 32 weights in order, which is an
+// operand of v_mfma_f32_16x16x32_f16 once it is fp16.  Seven instructions do that: the bytes' nibbles, even and odd, and four permutes
+// that put them into halves.  A nibble as the bits of an fp16 number is nibble * 2^-24, a subnormal, which the matrix cores take as it is: no
 // conversion, and the offset goes through them as well, as the accumulator that a first MFMA fills with -7 * 2^-24 * (the sum of x over the group) --
 // both exact, and 2^24 is part of the scale.  The group's sum leaves the accumulator with one multiply-add per row of x and group.
-// Rows of x lie at 4 (r % 4) + r / 4 of the operand: up to four rows fill one accumulator register of the lanes, up to eight two.
+// Rows of x lie at 4 (r % 4) + r / 4 of the operand: up to four rows fill one accumulator register of the lanes.
+// The scales pass through the LDS: eight bytes of each of sixteen rows, chunk by chunk, take more lines from the caches than W does
+// (1 x 50280 x 4096: 34 us).  W's loads are plain: what fits the Infinity Cache is read from there (streamed: 5 .. 10 % longer).
 constexpr int kChunk = 128;
 
 __device__ __forceinline__ f16x8 halves_of(unsigned word) {
@@ -64,8 +65,7 @@ __device__ __forceinline__ f16x8 halves_of(unsigned word) {
   return __builtin_bit_cast(f16x8, h);
 }
 __device__ __forceinline__ void turn(u32x4& w) {
-  unsigned a = w[0], b = w[1], c = w[2], d = w[3];
-  const auto ac = __builtin_amdgcn_permlane32_swap(a, c, false, false), bd = __builtin_amdgcn_permlane32_swap(b, d, false, false);
+  const auto ac = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), bd = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
   const auto ab = __builtin_amdgcn_permlane16_swap(ac[0], bd[0], false, false), cd = __builtin_amdgcn_permlane16_swap(ac[1], bd[1], false, false);
   w = u32x4{static_cast<unsigned>(ab[0]), static_cast<unsigned>(ab[1]), static_cast<unsigned>(cd[0]), static_cast<unsigned>(cd[1])};
 }
@@ -81,185 +81,320 @@ struct Q4Args {
   unsigned* arrivals;
 };
 
-// MT row tiles of x, NT column tiles, JN registers of a tile that hold rows, GS 32-blocks of k to a scale, W wavefronts
-template <int MT, int NT, int JN, int GS, int W>
-__global__ void __launch_bounds__(64 * W) gemv_q4_kernel(Q4Args a, Q4Epilogue ep) {
-  constexpr int kRows = 16 * MT, kCols = 16 * NT, kScales = 4 / GS;
-  __shared__ float sums[W][MT][NT][JN][64];
-  __shared__ int flag;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kCols, m0 = static_cast<int64_t>(blockIdx.z) * kRows;
-  const int64_t chunks = (a.K + kChunk - 1) / kChunk, lo = chunks * blockIdx.y / a.splits, hi = chunks * (blockIdx.y + 1) / a.splits;
-  const int64_t groups = a.K / (32 * GS);
-
-  const unsigned char* w_at[NT];
-  const half_t* s_at[NT];
+// One chunk of a row of W.  In the last chunk, of 32, 64 or 96, the lanes behind its end read the last 32 again: they meet zeros of x.
+__device__ __forceinline__ u32x4 load_w(const unsigned char* row, int64_t chunk, int64_t K, int quarter) {
+  const int64_t k = chunk * kChunk;
+  const int blocks = K - k >= kChunk ? 4 : static_cast<int>((K - k) / 32);
+  return *reinterpret_cast<const u32x4*>(row + k / 2 + (quarter < blocks ? quarter : blocks - 1) * 16);
+}
+// Scales of `cols` rows from n0 on, chunks [lo, hi), into the LDS: a row is an odd number of 8-byte pieces (sixteen rows fall on different banks).
+// What lies behind the row's last scale is that one again (it meets sums of zero).
+template <int GS>
+__host__ __device__ constexpr int scale_pitch(int64_t chunks) {
+  return static_cast<int>((chunks * (4 / GS) + 3) / 4) | 1;
+}
+template <int GS, int THREADS>
+__device__ __forceinline__ void stage_scales(char* lds, const Q4Args& a, int64_t n0, int cols, int64_t lo, int64_t hi) {
+  constexpr int kScales = 4 / GS;
+  const int64_t groups = a.K / (32 * GS), first = lo * kScales;
+  const int pieces = static_cast<int>(((hi - lo) * kScales + 3) / 4), pitch = scale_pitch<GS>(hi - lo);
+  for (int t = threadIdx.x; t < cols * pieces; t += THREADS) {
+    const int r = t / pieces, c = t % pieces;
+    const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1, g = first + 4 * c;
+    const half_t* from = a.S + n * groups;
+    f16x4 v;
+    if (g + 4 <= groups) {
+      __builtin_memcpy(&v, from + g, 8);
+    } else {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int64_t n = n0 + nt * 16 + i16 < a.N ? n0 + nt * 16 + i16 : a.N - 1;  // columns past N repeat the last; never stored
-    w_at[nt] = a.Wq + n * (a.K / 2) + quarter * 16;
-    s_at[nt] = a.S + n * groups;
-  }
-  const half_t* x_at[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int64_t r = m0 + mt * 16 + (i16 >> 2) + 4 * (i16 & 3);
-    x_at[mt] = a.x + (r < a.M ? r : a.M - 1) * a.K + quarter * 8;  // (rows past M repeat the last; never stored)
-  }
-  struct Chunk {
-    u32x4 w[NT];
-    f16x8 x[MT][4];
-    half_t s[NT][kScales];
-  };
-  auto load = [&](Chunk& c, int64_t at) {
-    const int64_t k = at * kChunk;
-    if (k + kChunk <= a.K) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        c.w[nt] = load_stream(reinterpret_cast<const u32x4*>(w_at[nt] + k / 2));
-        __builtin_memcpy(c.s[nt], s_at[nt] + at * kScales, sizeof c.s[nt]);
-      }
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c.x[mt][i] = *reinterpret_cast<const f16x8*>(x_at[mt] + k + 32 * i);
-    } else {  // the last 32, 64 or 96: what lies behind them is read from the last 32 again and meets zeros of x
-      const int blocks = static_cast<int>((a.K - k) / 32);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        c.w[nt] = load_stream(reinterpret_cast<const u32x4*>(w_at[nt] + k / 2 - (quarter < blocks ? 0 : (quarter - blocks + 1) * 16)));
-#pragma unroll
-        for (int i = 0; i < kScales; ++i) c.s[nt][i] = s_at[nt][at * kScales + i < groups ? at * kScales + i : groups - 1];
-      }
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c.x[mt][i] = i < blocks ? *reinterpret_cast<const f16x8*>(x_at[mt] + k + 32 * i) : f16x8{};
+      for (int i = 0; i < 4; ++i) v[i] = from[g + i < groups ? g + i : groups - 1];
     }
-  };
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    *reinterpret_cast<f16x4*>(lds + (r * pitch + c) * 8) = v;
+  }
+}
+// The products of one chunk for MT row tiles and one column tile, onto acc; x(mt, i): the operand of its i-th 32 k
+template <int MT, int JN, int GS, typename X>
+__device__ __forceinline__ void multiply(u32x4 w, X x, const char* scales, f32x4 (&acc)[MT]) {
   constexpr unsigned short kSeven = 0x8007;  // -7 * 2^-24
   const half_t seven = __builtin_bit_cast(half_t, kSeven);
   const f16x8 offset = {seven, seven, seven, seven, seven, seven, seven, seven};
-  auto use = [&](Chunk& c) {
+  turn(w);
+  half_t s[4 / GS];
+  __builtin_memcpy(s, __builtin_assume_aligned(scales, 8 / GS), sizeof s);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) turn(c.w[nt]);
-    f32x4 part[MT][NT];
+  for (int g = 0; g < 4 / GS; ++g) {
+    f32x4 part[MT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i % GS == 0) {
+    for (int mt = 0; mt < MT; ++mt) part[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          f32x4 from = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < GS; ++u) {
+      const f16x8 h = halves_of(w[g * GS + u]);
 #pragma unroll
-          for (int u = 0; u < GS; ++u) from = __builtin_amdgcn_mfma_f32_16x16x32_f16(c.x[mt][i + u], offset, from, 0, 0, 0);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) part[mt][nt] = from;
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const f16x8 w = halves_of(c.w[nt][i]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) part[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c.x[mt][i], w, part[mt][nt], 0, 0, 0);
-      }
-      if (i % GS == GS - 1) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float s = static_cast<float>(c.s[nt][i / GS]) * 16777216.f;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int j = 0; j < JN; ++j) acc[mt][nt][j] = fmaf(s, part[mt][nt][j], acc[mt][nt][j]);
-        }
+      for (int mt = 0; mt < MT; ++mt) {
+        const f16x8 v = x(mt, g * GS + u);
+        part[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, offset, part[mt], 0, 0, 0);
+        part[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, h, part[mt], 0, 0, 0);
       }
     }
-  };
-  Chunk now, next;
-  int64_t at = lo + wave;
-  if (at < hi) load(now, at);
-  for (; at < hi; at += W) {
-    if (at + W < hi) load(next, at + W);
-    use(now);
-    now = next;
+    const float scale = static_cast<float>(s[g]) * 16777216.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int j = 0; j < JN; ++j) acc[mt][j] = fmaf(scale, part[mt][j], acc[mt][j]);
   }
+}
+// Workgroups that share a long K leave their sums in the workspace; they pass the L2 (the XCDs' are not coherent) and are counted once they have drained.
+// True for whoever arrives last, and adds them up in their order.
+__device__ __forceinline__ bool last_to_arrive(const Q4Args& a, int64_t tile, int* flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned before = __hip_atomic_fetch_add(a.arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = before == static_cast<unsigned>(a.splits) - 1;
+    if (*flag) __hip_atomic_store(a.arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed for the next launch
+  }
+  __syncthreads();
+  return *flag != 0;
+}
 
-  // ---- the wavefronts' sums, in their order; a thread holds output (m, n) of register j, lane l of tile (mt, nt)
+// ---- up to four rows: the W wavefronts of a workgroup share the K of 16 columns, by pairs of chunks (the 128 bytes of a row that make a line), and
+// request D chunks before they use the first; x and the scales lie in the LDS.
+template <int GS, int W, int D>
+__global__ void __launch_bounds__(64 * W) gemv_q4_kernel(Q4Args a, Q4Epilogue ep) {
+  static_assert(D % 2 == 0, "pairs");
+  __shared__ float sums[W][64];
+  __shared__ int flag;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15, M = static_cast<int>(a.M);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t chunks = (a.K + kChunk - 1) / kChunk, lo = chunks * blockIdx.y / a.splits, hi = chunks * (blockIdx.y + 1) / a.splits;
+  const unsigned char* w_at = a.Wq + (n0 + i16 < a.N ? n0 + i16 : a.N - 1) * (a.K / 2);  // columns past N repeat the last; never stored
+  u32x4 some[D];
+  auto chunk_of = [&](int64_t base, int d) { return base + (d / 2 * W + wave) * 2 + d % 2; };
+  auto load_all = [&](int64_t base) {
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (chunk_of(base, d) < hi) some[d] = load_w(w_at, chunk_of(base, d), a.K, quarter);
+  };
+  load_all(lo);
+  const int row_bytes = static_cast<int>(hi - lo) * (kChunk * 2), pieces = row_bytes / 16;
+  for (int t = tid; t < pieces * M; t += 64 * W) {
+    const int r = t / pieces, c = t % pieces;
+    const int64_t k = lo * kChunk + c * 8;
+    reinterpret_cast<u32x4*>(lds)[t] = k < a.K ? *reinterpret_cast<const u32x4*>(a.x + r * a.K + k) : u32x4{0u, 0u, 0u, 0u};
+  }
+  char* lds_s = lds + row_bytes * M;
+  stage_scales<GS, 64 * W>(lds_s, a, n0, 16, lo, hi);
+  __syncthreads();
+  // row r of x is row 4 r of the operand; the others, never stored, repeat the last
+  const char* x_at = lds + ((i16 >> 2) < M ? i16 >> 2 : M - 1) * row_bytes + quarter * 16;
+  const char* s_at = lds_s + i16 * scale_pitch<GS>(hi - lo) * 8;
+  f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+  for (int64_t base = lo; base < hi; base += W * D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int at = static_cast<int>(chunk_of(base, d) - lo);
+      if (chunk_of(base, d) >= hi) break;
+      multiply<1, 1, GS>(some[d], [&](int, int i) { return *reinterpret_cast<const f16x8*>(x_at + at * (kChunk * 2) + i * 64); }, s_at + at * (8 / GS), acc);
+    }
+    if (base + W * D < hi) load_all(base + W * D);
+  }
+  sums[wave][lane] = acc[0][0];
+  __syncthreads();
+  if (a.splits == 1 && tid >= 64) return;
+  float sum = 0.f;
+  const int64_t n = n0 + i16;
+  float* shares = a.ws + static_cast<int64_t>(blockIdx.x) * a.splits * 64;
+  if (tid < 64) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += sums[w][lane];
+    if (a.splits > 1) __hip_atomic_store(shares + blockIdx.y * 64 + lane, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (a.splits > 1) {
+    if (!last_to_arrive(a, blockIdx.x, &flag) || tid >= 64) return;
+    sum = 0.f;
+    for (int z0 = 0; z0 < a.splits; z0 += 8) {
+      float part[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) part[u] = __hip_atomic_load(shares + (z0 + u < a.splits ? z0 + u : a.splits - 1) * 64 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += z0 + u < a.splits ? part[u] : 0.f;
+    }
+  }
+  if (quarter < M && n < a.N) finish_q4(sum, ep, a.y, quarter, n, a.N);
+}
+
+// ---- more rows: CT x KG wavefronts, CT column tiles and KG parts of every KG SL chunks.  x passes through the LDS, KG SL chunks at a time in two stages; a
+// wavefront requests W's next SL chunks, and its share of x's next stage, before it works on the present ones.
+template <int MT, int GS, int CT, int KG, int SL>
+__global__ void __launch_bounds__(64 * CT * KG) gemv_q4_rows_kernel(Q4Args a, Q4Epilogue ep) {
+  constexpr int W = CT * KG, kRows = 16 * MT, kCols = 16 * CT, kAll = KG * SL, kPitch = kChunk * 2 + 16;  // (the same 16 bytes of sixteen rows fall on different banks)
+  constexpr int kStage = kRows * kAll * kPitch, kPieces = kRows * kAll * (kChunk / 8) / (64 * W), kSums = KG * kRows * kCols * 4;
+  static_assert(kRows * kAll * (kChunk / 8) % (64 * W) == 0, "whole pieces");
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStage > kSums ? 2 * kStage : kSums];
+  __shared__ int flag;
+  extern __shared__ __attribute__((aligned(16))) char lds_s[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
+  const int ct = wave % CT, kg = wave / CT;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kCols, m0 = static_cast<int64_t>(blockIdx.z) * kRows;
+  const int64_t chunks = (a.K + kChunk - 1) / kChunk, lo = chunks * blockIdx.y / a.splits, hi = chunks * (blockIdx.y + 1) / a.splits;
+  const int64_t col = n0 + ct * 16 + i16;
+  const unsigned char* w_at = a.Wq + (col < a.N ? col : a.N - 1) * (a.K / 2);  // columns past N repeat the last; never stored
+  u32x4 w[SL], xr[kPieces];
+  auto load_all = [&](int64_t base) {
+#pragma unroll
+    for (int sl = 0; sl < SL; ++sl)
+      if (base + kg * SL + sl < hi) w[sl] = load_w(w_at, base + kg * SL + sl, a.K, quarter);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      // piece: row, then chunk, then 16 bytes; rows past M repeat the last, never stored
+      const int id = n * 64 * W + tid, c = id % (kChunk / 8), sl = id / (kChunk / 8) % kAll, r = id / (kChunk / 8 * kAll);
+      const int64_t k = (base + sl) * kChunk + c * 8, m = m0 + r < a.M ? m0 + r : a.M - 1;
+      xr[n] = base + sl < hi && k < a.K ? *reinterpret_cast<const u32x4*>(a.x + m * a.K + k) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  auto keep_x = [&](int stage) {
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      const int id = n * 64 * W + tid, c = id % (kChunk / 8), sl = id / (kChunk / 8) % kAll, r = id / (kChunk / 8 * kAll);
+      *reinterpret_cast<u32x4*>(lds + stage * kStage + (sl * kRows + r) * kPitch + c * 16) = xr[n];
+    }
+  };
+  load_all(lo);
+  stage_scales<GS, 64 * W>(lds_s, a, n0, kCols, lo, hi);
+  keep_x(0);
+  __syncthreads();
+  const char* s_at = lds_s + (ct * 16 + i16) * scale_pitch<GS>(hi - lo) * 8;
+  const char* x_at = lds + (kg * SL * kRows + (i16 >> 2) + 4 * (i16 & 3)) * kPitch + quarter * 16;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int stage = 0;
+  for (int64_t base = lo; base < hi; base += kAll, stage ^= 1) {
+    u32x4 now[SL];
+#pragma unroll
+    for (int sl = 0; sl < SL; ++sl) now[sl] = w[sl];
+    const bool more = base + kAll < hi;
+    if (more) load_all(base + kAll);
+#pragma unroll
+    for (int sl = 0; sl < SL; ++sl) {
+      const int64_t at = base + kg * SL + sl;
+      if (at >= hi) break;
+      multiply<MT, 4, GS>(now[sl], [&](int mt, int i) { return *reinterpret_cast<const f16x8*>(x_at + stage * kStage + (sl * kRows + mt * 16) * kPitch + i * 64); },
+                          s_at + static_cast<int>(at - lo) * (8 / GS), acc);
+    }
+    if (more) {
+      keep_x(stage ^ 1);
+      __syncthreads();
+    }
+  }
+  // the parts of K joined in their order, and into rows of columns
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < JN; ++j) sums[wave][mt][nt][j][lane] = acc[mt][nt][j];
+    for (int j = 0; j < 4; ++j) sums[(kg * kRows + mt * 16 + quarter + 4 * j) * kCols + ct * 16 + i16] = acc[mt][j];
   __syncthreads();
-  constexpr int kValues = MT * NT * JN * 64;
   const int64_t tile = static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x;
-  float* shares = a.ws + tile * a.splits * kValues;
-  auto finish = [&](int v, float sum) {
-    const int l = v & 63, j = v / 64 % JN, nt = v / (64 * JN) % NT, mt = v / (64 * JN * NT);
-    const int64_t m = m0 + mt * 16 + (l >> 4) + 4 * j, n = n0 + nt * 16 + (l & 15);
-    if (m < a.M && n < a.N) finish_q4(sum, ep, a.y, m, n, a.N);
-  };
-  for (int v = tid; v < kValues; v += 64 * W) {
-    float sum = 0.f;
+  constexpr int kFours = kRows * kCols / 4, kMine = (kFours + 64 * W - 1) / (64 * W);
+  f32x4 sum[kMine];
+  auto finish = [&] {
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum += (&sums[w][0][0][0][0])[v];
-    if (a.splits == 1) finish(v, sum);
-    else __hip_atomic_store(shares + static_cast<int64_t>(blockIdx.y) * kValues + v, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  if (a.splits == 1) return;
-  // ---- a long K shared by workgroups: their sums pass the L2 (the XCDs' are not coherent) and are counted once they have drained; whoever
-  // arrives last adds them up in their order
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) {
-    const unsigned before = __hip_atomic_fetch_add(a.arrivals + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    flag = before == static_cast<unsigned>(a.splits) - 1;
-    if (flag) __hip_atomic_store(a.arrivals + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed for the next launch
-  }
-  __syncthreads();
-  if (!flag) return;
-  for (int v = tid; v < kValues; v += 64 * W) {
-    float sum = 0.f;
-    for (int z0 = 0; z0 < a.splits; z0 += 8) {
-      float some[8];
+    for (int i = 0; i < kMine; ++i) {
+      const int at = 4 * (i * 64 * W + tid);
+      const int64_t m = m0 + at / kCols, n = n0 + at % kCols;
+      if (at >= 4 * kFours || m >= a.M) break;
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        some[u] = __hip_atomic_load(shares + static_cast<int64_t>(z0 + u < a.splits ? z0 + u : a.splits - 1) * kValues + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) sum += z0 + u < a.splits ? some[u] : 0.f;
+      for (int j = 0; j < 4; ++j)
+        if (n + j < a.N) finish_q4(sum[i][j], ep, a.y, m, n + j, a.N);
     }
-    finish(v, sum);
+  };
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = 4 * (i * 64 * W + tid);
+    if (at >= 4 * kFours) break;
+    sum[i] = *reinterpret_cast<const f32x4*>(sums + at);
+#pragma unroll
+    for (int k = 1; k < KG; ++k) {
+      const f32x4 part = *reinterpret_cast<const f32x4*>(sums + k * kRows * kCols + at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[i][j] += part[j];
+    }
   }
+  if (a.splits == 1) return finish();
+  float* shares = a.ws + tile * a.splits * (kRows * kCols);
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = 4 * (i * 64 * W + tid);
+    if (at < 4 * kFours) store_out(sum[i], reinterpret_cast<f32x4*>(shares + static_cast<int64_t>(blockIdx.y) * (kRows * kCols) + at), true);
+  }
+  if (!last_to_arrive(a, tile, &flag)) return;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kAtOnce = kMine >= 8 ? 1 : 8 / kMine;  // splits requested before the first is used: eight 16-byte pieces
+  for (int z0 = 0; z0 < a.splits; z0 += kAtOnce) {
+    uint64_t part[kAtOnce][kMine][2];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float* from = shares + static_cast<int64_t>(z0 + u < a.splits ? z0 + u : a.splits - 1) * (kRows * kCols);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int at = 4 * (i * 64 * W + tid);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          part[u][i][h] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from + (at < 4 * kFours ? at : 0)) + h, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (z0 + u >= a.splits) break;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] += __builtin_bit_cast(float, static_cast<unsigned>(part[u][i][j / 2] >> (32 * (j % 2))));
+    }
+  }
+  finish();
 }
 
-template <int MT, int NT, int JN, int GS, int W>
-int launch_q4(Q4Args a, const Q4Epilogue& ep, hipStream_t s) {
-  const int64_t cols = ceil_div(a.N, 16 * NT), rows = ceil_div(a.M, 16 * MT), tiles = cols * rows, chunks = ceil_div(a.K, kChunk);
-  // K shared by workgroups where the columns alone leave CUs idle, at two chunks per wavefront at least
-  int64_t splits = kNumCU / tiles;
-  const int64_t most = chunks / (2 * W);
-  splits = splits > most ? most : splits;
+// `cols` x `rows` per workgroup and K shared by workgroups: while the tiles alone are fewer than `fill`, at `least` chunks each, and as the LDS needs it
+template <typename Kernel>
+int launch_q4(Kernel kernel, Q4Args a, const Q4Epilogue& ep, int cols, int rows, int threads, int values, int64_t fill, int64_t least, int64_t lds_per_chunk, int64_t lds_fixed,
+              int64_t lds_most, hipStream_t s) {
+  const int64_t across = ceil_div(a.N, cols), down = ceil_div(a.M, rows), tiles = across * down, chunks = ceil_div(a.K, kChunk);
+  int64_t splits = fill / tiles;
+  splits = splits > chunks / least ? chunks / least : splits;
   splits = splits > 16 ? 16 : splits;
-  a.splits = static_cast<int>(splits < 1 ? 1 : splits);
-  if (cols > INT32_MAX || rows > 65535) return fail("gemv_q4: the launch has too many workgroups");
+  const int64_t needed = ceil_div(chunks, (lds_most - lds_fixed) / lds_per_chunk);
+  splits = splits < needed ? needed : splits;
+  splits = splits < 1 ? 1 : splits;
+  if (across > INT32_MAX || down > 65535 || splits > 65535) return fail("gemv_q4: the launch has too many workgroups");
+  a.splits = static_cast<int>(splits);
   std::unique_lock<std::recursive_mutex> lock;
-  if (a.splits > 1 && split_scratch(s, static_cast<size_t>(tiles * a.splits) * (MT * NT * JN * 64) * sizeof(float), static_cast<size_t>(tiles), a.splits, &a.ws, &a.arrivals, &lock) != 0)
-    return -1;
-  hipLaunchKernelGGL((gemv_q4_kernel<MT, NT, JN, GS, W>), dim3(static_cast<unsigned>(cols), static_cast<unsigned>(a.splits), static_cast<unsigned>(rows)), dim3(64 * W), 0, s, a, ep);
+  if (splits > 1 && split_scratch(s, static_cast<size_t>(tiles * splits) * values * sizeof(float), static_cast<size_t>(tiles), a.splits, &a.ws, &a.arrivals, &lock) != 0) return -1;
+  const unsigned lds = static_cast<unsigned>(ceil_div(chunks, splits) * lds_per_chunk + lds_fixed);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(across), static_cast<unsigned>(splits), static_cast<unsigned>(down)), dim3(threads), lds, s, a, ep);
   return check_launch("gemv_q4");
+}
+template <int GS, int W, int D>
+int launch_q4_few(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
+  return launch_q4(gemv_q4_kernel<GS, W, D>, a, ep, 16, 4, 64 * W, 64, kNumCU, 2 * W, a.M * kChunk * 2 + 16 * (8 / GS), 16 * 16, 60 * 1024, s);
+}
+template <int MT, int GS, int CT, int KG, int SL>
+int launch_q4_many(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
+  constexpr int kRows = 16 * MT, kCols = 16 * CT;
+  return launch_q4(gemv_q4_rows_kernel<MT, GS, CT, KG, SL>, a, ep, kCols, kRows, 64 * CT * KG, kRows * kCols, kNumCU, KG * SL, kCols * (8 / GS), kCols * 16, 20 * 1024, s);
 }
 template <int GS>
 int launch_q4_rows(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
-  if (a.M <= 4) return launch_q4<1, 1, 1, GS, 4>(a, ep, s);
-  if (a.M <= 8) return launch_q4<1, 1, 2, GS, 4>(a, ep, s);
-  if (a.M <= 16) return launch_q4<1, 1, 4, GS, 4>(a, ep, s);
-  if (a.M <= 32) return launch_q4<2, 2, 4, GS, 4>(a, ep, s);
-  return launch_q4<4, 2, 4, GS, 4>(a, ep, s);
+  // few columns: more wavefronts to each sixteen.  2560 x 10240 (160 workgroups) on 4 / 8 / 16 wavefronts 14.9 / 10.4 / 7.9 us, 7680 x 2560 (480) 7.2 / 6.2 / 6.3,
+  // 50280 x 4096 (3143) 28.8 / 31.5 / 40.5; four chunks requested at once instead of two are level to 10 % longer
+  if (a.M <= 4) return a.N <= 16 * 256 ? launch_q4_few<GS, 16, 2>(a, ep, s) : a.N <= 16 * 1024 ? launch_q4_few<GS, 8, 2>(a, ep, s) : launch_q4_few<GS, 4, 2>(a, ep, s);
+  if (a.M <= 16) return launch_q4_many<1, GS, 4, 4, 2>(a, ep, s);
+  // by 32 rows, W again for the next 32: 64 rows at once are behind but for the widest W (64 x 2560 x 10240 25.4 us against 18.3, 64 x 4096 x 4096 17.3 / 12.8,
+  // 64 x 10240 x 2560 23.0 / 17.8, 48 x 11008 x 4096 20.9 / 22.9).  Sixteen wavefronts where the columns are few, eight beyond (10240 x 2560 20.5 / 17.8, 2560 x 10240 18.3 / 20.3)
+  return a.N <= 8192 ? launch_q4_many<2, GS, 4, 4, 1>(a, ep, s) : launch_q4_many<2, GS, 4, 2, 2>(a, ep, s);
 }
 
 }  // namespace

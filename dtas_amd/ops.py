@@ -527,7 +527,7 @@ def gemv_q4(x: torch.Tensor, Wq: torch.Tensor, scale: torch.Tensor, bias: Option
             epilogue: int = 0, res1: Optional[torch.Tensor] = None, res2: Optional[torch.Tensor] = None) -> None:
     """y (..., N) = epilogue(x (..., K) . W^T) for the rows of x, with 4-bit weights W = (nibble - 7) * scale: element k of a row
     of W is bits 4 (k % 8) .. + 3 of word k / 8 of Wq[N, K/8], scale [N, K/group] fp16 with groups of 32, 64 or 128.  Epilogues as
-    ``gemm``, in fp32 with one rounding.  For one row and the few of a tree of drafted tokens: W is read once per 64 rows."""
+    ``gemm``, in fp32 with one rounding.  For one row and the few of a tree of drafted tokens: W is read once per 32 rows."""
     if _fastcall._gemv_q4(x, Wq, scale, bias, y, epilogue, res1, res2):
         return
     with _one_device("gemv_q4", x, Wq, scale, bias, y, res1, res2):

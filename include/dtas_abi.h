@@ -428,7 +428,8 @@ int dtas_gemv_q8_f16(const void* x, const void* Wq, const void* scale, const voi
  * Wq[N, K/8] uint32: element k of a row is bits 4 (k % 8) .. + 3 of word k / 8; scale[N, K/group] fp16, group 32, 64 or 128, K a
  * multiple of it.  The weights are not rounded: a group's products are summed in fp32 and scaled there.  bias[N] or NULL;
  * epilogues as dtas_gemm_f16_fused (res1, res2 [M,N] with the ADD2 kinds, NULL otherwise; y fp32 with ADD2_CAST_F32), but in
- * fp32 with one rounding at the end, GELU by erfc.  Made for one row and the few of a tree: W is read again for every 64 rows. */
+ * fp32 with one rounding at the end, GELU by erfc.  Made for one row and the few of a tree: W is read again for every 32 rows.  A long K
+ * is shared by workgroups that meet in the split-K workspace where the columns alone leave CUs idle. */
 int dtas_gemv_q4_f16(const void* x, const void* Wq, const void* scale, const void* bias, const void* res1, const void* res2, void* y,
                      int64_t M, int64_t N, int64_t K, int32_t group, int32_t epilogue, void* stream);
 
