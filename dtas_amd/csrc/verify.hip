@@ -1,6 +1,5 @@
 // Drafted tokens against the target's probabilities, and what is accepted into the key/value cache, for gfx950.
-#include "dtas_device.h"
-#include "dtas_host.h"
+#include "gemm_common.h"
 
 namespace dtas {
 namespace {
@@ -16,7 +15,12 @@ namespace {
 // so a refusal costs one sum over the rows and an acceptance none.  Where no child is accepted the next token is the first v whose
 // prefix sum of max(p - c q, 0) exceeds sample * total.  Sums and comparisons are in 64 bits: the products of two fp32 numbers are
 // exact there, and a token is chosen next to a border of the prefix sums.
-constexpr int kVerifyThreads = 1024;
+//
+// What happens at a node does not depend on the way there: a workgroup per node finds out which child is accepted there, or the token behind it, and
+// whoever is last among a sequence's workgroups follows the path.  Nodes that cannot be on it are left out beforehand: the first child of a node
+// is settled by accept * q < p alone, and a later one (c >= 1 by then) is out of the question where its first brother is accepted or p <= q.  So the rows that
+// are read are few more than those of the path (32 trees of 31 nodes over 50280 tokens: 68 us with a workgroup per tree that walked it).
+constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / 64;
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
@@ -29,99 +33,209 @@ __device__ __forceinline__ double rest_of(float p, float q, double c) {
   return w > 0.0 ? w : 0.0;  // (NaN too)
 }
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const float* __restrict__ target, const float* __restrict__ draft,
-                                                                     const int* __restrict__ tokens, const int* __restrict__ parents,
-                                                                     const float* __restrict__ accept, const float* __restrict__ sample,
-                                                                     int* __restrict__ path, int* __restrict__ count, int* __restrict__ next,
-                                                                     int T, int64_t V) {
-  constexpr int kWaves = kVerifyThreads / 64;
-  __shared__ float at_p[DTAS_MAX_TREE_NODES], at_q[DTAS_MAX_TREE_NODES], at_u[DTAS_MAX_TREE_NODES];
-  __shared__ int at_parent[DTAS_MAX_TREE_NODES];
-  __shared__ double part[2][kWaves];
-  const int64_t b = blockIdx.x;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  int phase = 0;
-  if (tid < T) {
-    const int parent = parents[b * T + tid], token = tokens[b * T + tid];
-    const bool offered = tid > 0 && parent >= 0 && parent < tid && token >= 0 && token < V;
-    at_parent[tid] = offered ? parent : -1;
-    at_u[tid] = accept[b * T + tid];
-    at_p[tid] = offered ? target[(b * T + parent) * V + token] : 0.f;
-    at_q[tid] = offered ? draft[(b * T + parent) * V + token] : 0.f;
-    path[b * T + tid] = tid == 0 ? 0 : -1;
+// four consecutive probabilities (rows of an odd vocabulary begin off 16 bytes)
+__device__ __forceinline__ f32x4 load4(const float* p) {
+  f32x4 v;
+  __builtin_memcpy(&v, __builtin_assume_aligned(p, 4), 16);
+  return v;
+}
+
+// The sum of max(p - c q, 0) over [from, to), by one wavefront; q is not read where c is 0
+__device__ __forceinline__ double sum_rest(const float* p, const float* q, double c, int64_t from, int64_t to, int lane) {
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  int64_t v = from + 4 * lane;
+  constexpr int kAtOnce = 4;
+  for (; v + 256 * (kAtOnce - 1) + 4 <= to; v += 256 * kAtOnce) {
+    f32x4 a[kAtOnce], b[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) a[u] = load4(p + v + 256 * u);
+    if (c != 0.0) {
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) b[u] = load4(q + v + 256 * u);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] += rest_of(a[u][j], b[u][j], c);
   }
+  for (; v < to; v += 256)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (v + j < to) s[j] += rest_of(p[v + j], c != 0.0 ? q[v + j] : 0.f, c);
+  return wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
+}
+
+struct VerifyArgs {
+  const float *target, *draft;
+  const int *tokens, *parents;
+  const float *accept, *sample;
+  int *path, *count, *next;
+  int T;
+  int64_t V;
+  int* outcomes;       // [batch, T]: an accepted child, or -2 - the next token
+  unsigned* arrivals;  // [batch]
+};
+
+__global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs a) {
+  __shared__ float at_p[DTAS_MAX_TREE_NODES], at_q[DTAS_MAX_TREE_NODES], at_u[DTAS_MAX_TREE_NODES];
+  __shared__ double part[2][kVerifyWaves];
+  __shared__ int flag;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, node = blockIdx.x, T = a.T;
+  const int64_t b = blockIdx.y, V = a.V;
+  // ---- every wavefront: the edges, and which nodes the walk can reach
+  const int parent = lane < T ? a.parents[b * T + lane] : -1, token = lane < T ? a.tokens[b * T + lane] : -1;
+  const bool offered = lane > 0 && parent >= 0 && parent < lane && token >= 0 && token < V;
+  const float u = offered ? a.accept[b * T + lane] : 0.f;
+  const float p0 = offered ? a.target[(b * T + parent) * V + token] : 0.f, q0 = offered ? a.draft[(b * T + parent) * V + token] : 0.f;
+  const uint64_t edges = __builtin_amdgcn_ballot_w64(offered);
+  // a node's children, as the lane of that node holds them
+  uint64_t children = 0;
+  for (uint64_t left = edges; left; left &= left - 1) {
+    const int child = __builtin_ctzll(left);
+    if (__builtin_amdgcn_readlane(parent, child) == lane) children |= uint64_t{1} << child;
+  }
+  const int eldest = children ? __builtin_ctzll(children) : -1;                              // of this lane's node
+  const int first = __shfl(eldest, offered ? parent : lane);                                 // of this lane's parent
+  const bool at_once = static_cast<double>(u) * static_cast<double>(q0) < static_cast<double>(p0 > 0.f ? p0 : 0.f);
+  const uint64_t settled = __builtin_amdgcn_ballot_w64(offered && at_once);
+  const bool can = offered && (first == lane ? at_once : !((settled >> (first < 0 ? 0 : first)) & 1) && p0 > q0);
+  uint64_t reach = 1, fresh = 1;  // from node 0 on, a generation at a time
+  const uint64_t open = __builtin_amdgcn_ballot_w64(can);
+  while (fresh) {
+    const uint64_t more = __builtin_amdgcn_ballot_w64(can && ((fresh >> (parent < 0 ? 0 : parent)) & 1)) & open & ~reach;
+    reach |= more;
+    fresh = more;
+  }
+  if (!((reach >> node) & 1)) return;
+  if (wave == 0) {
+    at_p[lane] = p0;
+    at_q[lane] = q0;
+    at_u[lane] = u;
+  }
+  uint64_t mine = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(children), node)) & 0xffffffffu;
+  mine |= static_cast<uint64_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(children >> 32), node))) << 32;
   __syncthreads();
-  // the sum of max(p - c q, 0) over [lo, hi), one contiguous piece per wavefront; every thread returns with the pieces in `part`
-  auto sums = [&](const float* p, const float* q, double c, int64_t lo, int64_t piece, int64_t hi) -> const double* {
-    double s = 0.0;
-    const int64_t from = lo + wave * piece, to = from + piece < hi ? from + piece : hi;
-    for (int64_t v = from + lane; v < to; v += 64) s += rest_of(p[v], q[v], c);
-    s = wave_sum64(s);
+
+  // ---- this node: its children in their order, then the token
+  const float* p = a.target + (b * T + node) * V;
+  const float* q = a.draft + (b * T + node) * V;
+  int phase = 0;
+  // the sums of the wavefronts' pieces of [lo, hi); every thread returns with them in `part`
+  auto sums = [&](double c, int64_t lo, int64_t piece, int64_t hi) -> const double* {
+    const int64_t from = lo + wave * piece < hi ? lo + wave * piece : hi, to = from + piece < hi ? from + piece : hi;
+    const double s = sum_rest(p, q, c, from, to, lane);
     double* bank = part[phase++ & 1];
     if (lane == 0) bank[wave] = s;
     __syncthreads();
     return bank;
   };
-  int at = 0, accepted = 1;
+  const int64_t whole = ((V + kVerifyWaves - 1) / kVerifyWaves + 3) / 4 * 4;
+  int outcome = -1;
+  bool accepted = false;
   double c = 0.0, left = 1.0;
-  for (int i = 1; i < T; ++i) {
-    if (at_parent[i] != at) continue;
-    const double q = static_cast<double>(at_q[i]), rest = rest_of(at_p[i], at_q[i], c);
-    if (static_cast<double>(at_u[i]) * q * left < rest) {
-      if (tid == 0) path[b * T + accepted] = i;
-      ++accepted;
-      at = i;
-      c = 0.0;
-      left = 1.0;
-    } else {
-      c += left;
-      const double* bank = sums(target + (b * T + at) * V, draft + (b * T + at) * V, c, 0, (V + kWaves - 1) / kWaves, V);
-      left = 0.0;
-      for (int w = 0; w < kWaves; ++w) left += bank[w];
-    }
-  }
-  const float* p = target + (b * T + at) * V;
-  const float* q = draft + (b * T + at) * V;
-  int64_t lo = 0, hi = V;
-  double goal = 0.0, base = 0.0;
-  bool first = true;
-  int chosen = -1;
-  while (hi > lo) {
-    const int64_t piece = (hi - lo + kWaves - 1) / kWaves;
-    const double* bank = sums(p, q, c, lo, piece, hi);
-    if (first) {
-      double total = 0.0;
-      for (int w = 0; w < kWaves; ++w) total += bank[w];
-      if (!(total > 0.0)) {
-        if (c == 0.0) break;  // a row of zeros: there is no token
-        c = 0.0;              // nothing is left of the target (its rows equal the draft's): the target itself
-        continue;
-      }
-      const double r = static_cast<double>(sample[b]);
-      goal = (r > 0.0 ? r < 1.0 ? r : 1.0 : 0.0) * total;
-      first = false;
-    }
-    int w_at = -1;
-    double before = base;
-    for (int w = 0; w < kWaves; ++w) {
-      if (bank[w] > 0.0) {
-        w_at = w;  // (the last one with a positive sum, where rounding leaves the goal behind all of them)
-        base = before;
-        if (before + bank[w] > goal) break;
-      }
-      before += bank[w];
-    }
-    lo += w_at * piece;
-    hi = lo + piece < hi ? lo + piece : hi;
-    if (piece == 1) {
-      chosen = static_cast<int>(lo);
+  const double* bank = nullptr;  // the pieces' sums with the present c
+  for (; mine; mine &= mine - 1) {
+    const int i = __builtin_ctzll(mine);
+    if (static_cast<double>(at_u[i]) * static_cast<double>(at_q[i]) * left < rest_of(at_p[i], at_q[i], c)) {
+      outcome = i;
+      accepted = true;
       break;
     }
+    c += left;
+    bank = sums(c, 0, whole, V);
+    left = 0.0;
+    for (int w = 0; w < kVerifyWaves; ++w) left += bank[w];
   }
+  if (!accepted) {
+    if (!bank) bank = sums(c, 0, whole, V);
+    double total = 0.0;
+    for (int w = 0; w < kVerifyWaves; ++w) total += bank[w];
+    if (!(total > 0.0) && c != 0.0) {  // nothing is left of the target (its rows equal the draft's): the target itself
+      c = 0.0;
+      bank = sums(c, 0, whole, V);
+      total = 0.0;
+      for (int w = 0; w < kVerifyWaves; ++w) total += bank[w];
+    }
+    if (total > 0.0) {  // (a row of zeros has no token: outcome -1)
+      const double r = static_cast<double>(a.sample[b]), goal = (r > 0.0 ? r < 1.0 ? r : 1.0 : 0.0) * total;
+      // the piece that the goal falls into: the first whose end lies behind it, or (where rounding leaves it behind all) the last with a sum
+      int64_t lo = 0, hi = V, piece = whole;
+      double base = 0.0;
+      for (;;) {
+        int w_at = 0;
+        double before = base, start = base;
+        for (int w = 0; w < kVerifyWaves; ++w) {
+          if (bank[w] > 0.0) {
+            w_at = w;
+            start = before;
+            if (before + bank[w] > goal) break;
+          }
+          before += bank[w];
+        }
+        base = start;
+        lo += w_at * piece;
+        hi = lo + piece < hi ? lo + piece : hi;
+        if (hi - lo <= 256) break;
+        piece = ((hi - lo + kVerifyWaves - 1) / kVerifyWaves + 3) / 4 * 4;
+        bank = sums(c, lo, piece, hi);
+      }
+      // four tokens a lane
+      double w[4], mine4 = 0.0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t v = lo + 4 * lane + j;
+        w[j] = v < hi ? rest_of(p[v], c != 0.0 ? q[v] : 0.f, c) : 0.0;
+        mine4 += w[j];
+      }
+      double upto = mine4;
+#pragma unroll
+      for (int i = 1; i < 64; i <<= 1) {
+        const double other = __shfl_up(upto, i);
+        if (lane >= i) upto += other;
+      }
+      const uint64_t some = __builtin_amdgcn_ballot_w64(mine4 > 0.0), behind = __builtin_amdgcn_ballot_w64(mine4 > 0.0 && base + upto > goal);
+      const int l = behind ? __builtin_ctzll(behind) : 63 - __builtin_clzll(some | 1);
+      double before = base + (upto - mine4);
+      int token_at = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (w[j] > 0.0 && !(token_at > 0 && before > goal)) token_at = j + 1;  // (the first whose end lies behind the goal, else the last with a weight)
+        before += w[j];
+      }
+      outcome = -2 - static_cast<int>(lo + 4 * l + __shfl(token_at, l) - 1);
+    }
+  }
+
+  // ---- whoever is last follows the path.  The outcomes pass the L2 (the XCDs' are not coherent); an arrival is counted once its own has drained
   if (tid == 0) {
-    count[b] = accepted;
-    next[b] = chosen;
+    __hip_atomic_store(a.outcomes + b * T + node, outcome, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const unsigned arrived = __hip_atomic_fetch_add(a.arrivals + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    flag = arrived == static_cast<unsigned>(__builtin_popcountll(reach)) - 1;
+    if (flag) __hip_atomic_store(a.arrivals + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // re-armed for the next launch
   }
+  if (wave != 0) return;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if (!__builtin_amdgcn_readfirstlane(flag)) return;
+  const int found = (reach >> lane) & 1 ? __hip_atomic_load(a.outcomes + b * T + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : -1;
+  int at = 0, steps = 1, way = lane == 0 ? 0 : -1;
+  for (;;) {
+    const int o = __builtin_amdgcn_readlane(found, at);
+    if (o < 1) {
+      if (lane == 0) {
+        a.next[b] = -2 - o;
+        a.count[b] = steps;
+      }
+      break;
+    }
+    at = o;
+    if (lane == steps) way = o;
+    ++steps;
+  }
+  if (lane < T) a.path[b * T + lane] = way;
 }
 
 // ---- the accepted rows into the cache -------------------------------------------------------------------------------
@@ -177,11 +291,31 @@ extern "C" int dtas_verify_tree_f32(const void* target, const void* draft, const
     for (int j = 0; j < i; ++j)
       if (overlaps(out[i].at, out[i].bytes, out[j].at, out[j].bytes)) return fail("verify_tree: the outputs overlap");
   }
-  hipLaunchKernelGGL(verify_tree_kernel, dim3(static_cast<unsigned>(batch)), dim3(kVerifyThreads), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const float*>(target), static_cast<const float*>(draft), static_cast<const int*>(tokens),
-                     static_cast<const int*>(parents), static_cast<const float*>(accept), static_cast<const float*>(sample), static_cast<int*>(path),
-                     static_cast<int*>(count), static_cast<int*>(next), static_cast<int>(nodes), V);
-  return check_launch("verify_tree");
+  VerifyArgs args{static_cast<const float*>(target), static_cast<const float*>(draft), static_cast<const int*>(tokens), static_cast<const int*>(parents),
+                  static_cast<const float*>(accept), static_cast<const float*>(sample), static_cast<int*>(path), static_cast<int*>(count), static_cast<int*>(next),
+                  static_cast<int>(nodes), V, nullptr, nullptr};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  // a grid holds 65535 sequences: more are further launches
+  for (int64_t b = 0; b < batch; b += 65535) {
+    const int64_t some = batch - b < 65535 ? batch - b : 65535;
+    float* room = nullptr;
+    std::unique_lock<std::recursive_mutex> lock;
+    if (split_scratch(s, static_cast<size_t>(some * nodes) * sizeof(int), static_cast<size_t>(some), static_cast<int>(nodes), &room, &args.arrivals, &lock) != 0) return -1;
+    args.outcomes = reinterpret_cast<int*>(room);
+    hipLaunchKernelGGL(verify_tree_kernel, dim3(static_cast<unsigned>(nodes), static_cast<unsigned>(some)), dim3(kVerifyThreads), 0, s, args);
+    if (check_launch("verify_tree") != 0) return -1;
+    const int64_t n = some * nodes;
+    args.target += n * V;
+    args.draft += n * V;
+    args.tokens += n;
+    args.parents += n;
+    args.accept += n;
+    args.sample += some;
+    args.path += n;
+    args.count += some;
+    args.next += some;
+  }
+  return 0;
 }
 
 extern "C" int dtas_cache_append_f16(const void* K, const void* V, const void* path, const void* count, void* K_cache, void* V_cache,
