@@ -22,9 +22,30 @@ namespace {
 // are read are few more than those of the path (32 trees of 31 nodes over 50280 tokens: 68 us with a workgroup per tree that walked it).
 constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / 64;
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int i = 32; i > 0; i >>= 1) v += __shfl_xor(v, i);
+// sums over the lanes up to this one, on the DPP datapath (through the LDS crossbar the six steps take six times as long); ROWS: of 16 lanes each, or of all
+template <int CTRL, int MASK>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), CTRL, MASK, 0xf, true);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), CTRL, MASK, 0xf, true);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double lane64(double v, int lane) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(bits), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), lane);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double upto16(double v) {
+  v += dpp64<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v += dpp64<0x112, 0xf>(v);
+  v += dpp64<0x114, 0xf>(v);
+  v += dpp64<0x118, 0xf>(v);
+  return v;
+}
+__device__ __forceinline__ double upto64(double v) {
+  v = upto16(v);
+  v += dpp64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
@@ -40,32 +61,32 @@ __device__ __forceinline__ f32x4 load4(const float* p) {
   return v;
 }
 
-// The sum of max(p - c q, 0) over [from, to), by one wavefront; q is not read where c is 0
+// The sum of max(p - c q, 0) over [from, to), by one wavefront; q is not read where c is 0.  `from` is a multiple of 4 of the row, and so is `to` unless it
+// is the row's end.  A pass over both rows of 50280 tokens takes a workgroup 3 us: what a CU draws from its L2 (in fp32 the sums take as long).
 __device__ __forceinline__ double sum_rest(const float* p, const float* q, double c, int64_t from, int64_t to, int lane) {
   double s[4] = {0.0, 0.0, 0.0, 0.0};
-  int64_t v = from + 4 * lane;
-  constexpr int kAtOnce = 4;
-  for (; v + 256 * (kAtOnce - 1) + 4 <= to; v += 256 * kAtOnce) {
+  constexpr int kAtOnce = 3;
+  for (int64_t base = from; base < to; base += 256 * kAtOnce) {
     f32x4 a[kAtOnce], b[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) a[u] = load4(p + v + 256 * u);
-    if (c != 0.0) {
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) b[u] = load4(q + v + 256 * u);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int64_t v = base + 256 * u + 4 * lane;
+      const bool in = v + 4 <= to;
+      a[u] = b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (base + 256 * u >= to) continue;
+      if (in) a[u] = load4(p + v);
+      if (in && c != 0.0) b[u] = load4(q + v);
     }
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u)
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (base + 256 * u >= to) break;
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[j] += rest_of(a[u][j], b[u][j], c);
+    }
   }
-  for (; v < to; v += 256)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (v + j < to) s[j] += rest_of(p[v + j], c != 0.0 ? q[v + j] : 0.f, c);
-  return wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
+  const int64_t end = to - ((to - from) & 3) + lane;  // the last one to three
+  if (end < to) s[0] += rest_of(p[end], c != 0.0 ? q[end] : 0.f, c);
+  return lane64(upto64((s[0] + s[1]) + (s[2] + s[3])), 63);
 }
 
 struct VerifyArgs {
@@ -81,62 +102,67 @@ struct VerifyArgs {
 
 __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs a) {
   __shared__ float at_p[DTAS_MAX_TREE_NODES], at_q[DTAS_MAX_TREE_NODES], at_u[DTAS_MAX_TREE_NODES];
+  __shared__ int eldest[DTAS_MAX_TREE_NODES];
+  __shared__ uint64_t at_reach, at_mine;
   __shared__ double part[2][kVerifyWaves];
   __shared__ int flag;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, node = blockIdx.x, T = a.T;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, node = blockIdx.x, T = a.T;
   const int64_t b = blockIdx.y, V = a.V;
-  // ---- every wavefront: the edges, and which nodes the walk can reach
-  const int parent = lane < T ? a.parents[b * T + lane] : -1, token = lane < T ? a.tokens[b * T + lane] : -1;
-  const bool offered = lane > 0 && parent >= 0 && parent < lane && token >= 0 && token < V;
-  const float u = offered ? a.accept[b * T + lane] : 0.f;
-  const float p0 = offered ? a.target[(b * T + parent) * V + token] : 0.f, q0 = offered ? a.draft[(b * T + parent) * V + token] : 0.f;
-  const uint64_t edges = __builtin_amdgcn_ballot_w64(offered);
-  // a node's children, as the lane of that node holds them
-  uint64_t children = 0;
-  for (uint64_t left = edges; left; left &= left - 1) {
-    const int child = __builtin_ctzll(left);
-    if (__builtin_amdgcn_readlane(parent, child) == lane) children |= uint64_t{1} << child;
-  }
-  const int eldest = children ? __builtin_ctzll(children) : -1;                              // of this lane's node
-  const int first = __shfl(eldest, offered ? parent : lane);                                 // of this lane's parent
-  const bool at_once = static_cast<double>(u) * static_cast<double>(q0) < static_cast<double>(p0 > 0.f ? p0 : 0.f);
-  const uint64_t settled = __builtin_amdgcn_ballot_w64(offered && at_once);
-  const bool can = offered && (first == lane ? at_once : !((settled >> (first < 0 ? 0 : first)) & 1) && p0 > q0);
-  uint64_t reach = 1, fresh = 1;  // from node 0 on, a generation at a time
-  const uint64_t open = __builtin_amdgcn_ballot_w64(can);
-  while (fresh) {
-    const uint64_t more = __builtin_amdgcn_ballot_w64(can && ((fresh >> (parent < 0 ? 0 : parent)) & 1)) & open & ~reach;
-    reach |= more;
-    fresh = more;
-  }
-  if (!((reach >> node) & 1)) return;
+  // ---- the edges, and which nodes the walk can reach
   if (wave == 0) {
+    const int parent = lane < T ? a.parents[b * T + lane] : -1, token = lane < T ? a.tokens[b * T + lane] : -1;
+    const float u = lane < T ? a.accept[b * T + lane] : 0.f;
+    const bool offered = lane > 0 && parent >= 0 && parent < lane && token >= 0 && token < V;
+    const int above = offered ? parent : 0;
+    const float p0 = offered ? a.target[(b * T + above) * V + token] : 0.f, q0 = offered ? a.draft[(b * T + above) * V + token] : 0.f;
+    eldest[lane] = 64;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (offered) atomicMin(&eldest[above], lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int first = eldest[above];  // (of this lane's node and its brothers)
     at_p[lane] = p0;
     at_q[lane] = q0;
     at_u[lane] = u;
+    const bool at_once = static_cast<double>(u) * static_cast<double>(q0) < static_cast<double>(p0 > 0.f ? p0 : 0.f);
+    const uint64_t settled = __builtin_amdgcn_ballot_w64(offered && at_once);
+    const bool can = offered && (first == lane ? at_once : !((settled >> (first & 63)) & 1) && p0 > q0);
+    uint64_t reach = 1, fresh = 1;  // from node 0 on, a generation at a time
+    while (fresh) {
+      const uint64_t more = __builtin_amdgcn_ballot_w64(can && ((fresh >> above) & 1)) & ~reach;
+      reach |= more;
+      fresh = more;
+    }
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(offered && parent == node);
+    if (lane == 0) {
+      at_reach = reach;
+      at_mine = mine;
+    }
   }
-  uint64_t mine = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(children), node)) & 0xffffffffu;
-  mine |= static_cast<uint64_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(children >> 32), node))) << 32;
   __syncthreads();
+  const uint64_t reach = at_reach;
+  if (!((reach >> node) & 1)) return;
+  uint64_t mine = at_mine;
 
   // ---- this node: its children in their order, then the token
   const float* p = a.target + (b * T + node) * V;
   const float* q = a.draft + (b * T + node) * V;
   int phase = 0;
-  // the sums of the wavefronts' pieces of [lo, hi); every thread returns with them in `part`
-  auto sums = [&](double c, int64_t lo, int64_t piece, int64_t hi) -> const double* {
+  // the sums of the wavefronts' pieces of [lo, hi): lane w of a row of sixteen returns with piece w's
+  auto sums = [&](double c, int64_t lo, int64_t piece, int64_t hi) -> double {
     const int64_t from = lo + wave * piece < hi ? lo + wave * piece : hi, to = from + piece < hi ? from + piece : hi;
     const double s = sum_rest(p, q, c, from, to, lane);
     double* bank = part[phase++ & 1];
     if (lane == 0) bank[wave] = s;
     __syncthreads();
-    return bank;
+    return bank[lane & 15];
   };
+  static_assert(kVerifyWaves == 16, "a row of lanes");
   const int64_t whole = ((V + kVerifyWaves - 1) / kVerifyWaves + 3) / 4 * 4;
   int outcome = -1;
   bool accepted = false;
   double c = 0.0, left = 1.0;
-  const double* bank = nullptr;  // the pieces' sums with the present c
+  double pieces = 0.0;  // with the present c: lane w of sixteen holds the sum of piece w ...
+  bool summed = false;
   for (; mine; mine &= mine - 1) {
     const int i = __builtin_ctzll(mine);
     if (static_cast<double>(at_u[i]) * static_cast<double>(at_q[i]) * left < rest_of(at_p[i], at_q[i], c)) {
@@ -145,19 +171,17 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
       break;
     }
     c += left;
-    bank = sums(c, 0, whole, V);
-    left = 0.0;
-    for (int w = 0; w < kVerifyWaves; ++w) left += bank[w];
+    pieces = sums(c, 0, whole, V);
+    summed = true;
+    left = lane64(upto16(pieces), 15);
   }
   if (!accepted) {
-    if (!bank) bank = sums(c, 0, whole, V);
-    double total = 0.0;
-    for (int w = 0; w < kVerifyWaves; ++w) total += bank[w];
+    if (!summed) pieces = sums(c, 0, whole, V);
+    double total = lane64(upto16(pieces), 15);
     if (!(total > 0.0) && c != 0.0) {  // nothing is left of the target (its rows equal the draft's): the target itself
       c = 0.0;
-      bank = sums(c, 0, whole, V);
-      total = 0.0;
-      for (int w = 0; w < kVerifyWaves; ++w) total += bank[w];
+      pieces = sums(c, 0, whole, V);
+      total = lane64(upto16(pieces), 15);
     }
     if (total > 0.0) {  // (a row of zeros has no token: outcome -1)
       const double r = static_cast<double>(a.sample[b]), goal = (r > 0.0 ? r < 1.0 ? r : 1.0 : 0.0) * total;
@@ -165,22 +189,16 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
       int64_t lo = 0, hi = V, piece = whole;
       double base = 0.0;
       for (;;) {
-        int w_at = 0;
-        double before = base, start = base;
-        for (int w = 0; w < kVerifyWaves; ++w) {
-          if (bank[w] > 0.0) {
-            w_at = w;
-            start = before;
-            if (before + bank[w] > goal) break;
-          }
-          before += bank[w];
-        }
-        base = start;
-        lo += w_at * piece;
+        const double upto = upto16(pieces);
+        const unsigned some = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(pieces > 0.0)) & 0xffffu;
+        const unsigned behind = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(pieces > 0.0 && base + upto > goal)) & 0xffffu;
+        const int at = behind ? __builtin_ctz(behind) : 31 - __builtin_clz(some | 1u);
+        if (at > 0) base += lane64(upto, at - 1);
+        lo += at * piece;
         hi = lo + piece < hi ? lo + piece : hi;
         if (hi - lo <= 256) break;
         piece = ((hi - lo + kVerifyWaves - 1) / kVerifyWaves + 3) / 4 * 4;
-        bank = sums(c, lo, piece, hi);
+        pieces = sums(c, lo, piece, hi);
       }
       // four tokens a lane
       double w[4], mine4 = 0.0;
@@ -190,12 +208,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
         w[j] = v < hi ? rest_of(p[v], c != 0.0 ? q[v] : 0.f, c) : 0.0;
         mine4 += w[j];
       }
-      double upto = mine4;
-#pragma unroll
-      for (int i = 1; i < 64; i <<= 1) {
-        const double other = __shfl_up(upto, i);
-        if (lane >= i) upto += other;
-      }
+      const double upto = upto64(mine4);
       const uint64_t some = __builtin_amdgcn_ballot_w64(mine4 > 0.0), behind = __builtin_amdgcn_ballot_w64(mine4 > 0.0 && base + upto > goal);
       const int l = behind ? __builtin_ctzll(behind) : 63 - __builtin_clzll(some | 1);
       double before = base + (upto - mine4);
@@ -240,30 +253,34 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
 
 // ---- the accepted rows into the cache -------------------------------------------------------------------------------
 // cache[l, b, h, lens[b] + j, :] = new[l, b, path[b, j], h, :] for j < count[b]; no path: all rows in their order.  Rows that would
-// fall outside [0, capacity), and path entries outside [0, T), are left out.  One thread per 16 bytes (or per element), of K
-// (blockIdx.y = 0) and V (1).
+// fall outside [0, capacity), and path entries outside [0, T), are left out.  A workgroup has `run` slots of one sequence and layer, of K and of V, in 16-byte
+// pieces (or elements): what it needs to know of the sequence are scalars, and a workgroup behind the last kept slot ends at once.
 template <typename U>
 __global__ void __launch_bounds__(256) cache_append_kernel(const U* __restrict__ K, const U* __restrict__ V, const int* __restrict__ path,
                                                            const int* __restrict__ count, U* __restrict__ Kc, U* __restrict__ Vc,
                                                            const int* __restrict__ lens, int B, int T, int slots, int H, int per_row, int64_t capacity,
-                                                           int64_t total) {
-  const U* from = blockIdx.y ? V : K;
-  U* to = blockIdx.y ? Vc : Kc;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-    // i = (((l B + b) slots + j) H + h) per_row + e
-    const int e = static_cast<int>(i % per_row);
-    int64_t r = i / per_row;
-    const int h = static_cast<int>(r % H);
-    r /= H;
-    const int j = static_cast<int>(r % slots);
-    r /= slots;
-    const int b = static_cast<int>(r % B);
-    const int64_t lb = r;
-    if (count && j >= count[b]) continue;
-    const int node = path ? path[static_cast<int64_t>(b) * slots + j] : j;
-    const int64_t row = static_cast<int64_t>(lens[b]) + j;
-    if (node < 0 || node >= T || row < 0 || row >= capacity) continue;
-    to[((lb * H + h) * capacity + row) * per_row + e] = from[((lb * T + node) * H + h) * per_row + e];
+                                                           int run, int runs) {
+  const int64_t lb = blockIdx.x / static_cast<unsigned>(runs);
+  const int b = static_cast<int>(lb % B), j0 = static_cast<int>(blockIdx.x % static_cast<unsigned>(runs)) * run;
+  int kept = slots;
+  if (count) kept = count[b] < slots ? count[b] : slots;
+  if (j0 >= kept) return;
+  const int64_t len = lens[b];
+  const int here = kept - j0 < run ? kept - j0 : run;
+  const unsigned row = static_cast<unsigned>(H) * per_row, all = static_cast<unsigned>(here) * row;
+  const U* from_k = K + lb * T * static_cast<int64_t>(row);
+  const U* from_v = V + lb * T * static_cast<int64_t>(row);
+  U* to_k = Kc + lb * H * capacity * per_row;
+  U* to_v = Vc + lb * H * capacity * per_row;
+  for (unsigned t = threadIdx.x; t < all; t += 256) {
+    const unsigned i = t / row, in_row = t - i * row, h = in_row / static_cast<unsigned>(per_row), e = in_row - h * per_row;
+    const int j = j0 + static_cast<int>(i), node = path ? path[static_cast<int64_t>(b) * slots + j] : j;
+    const int64_t at = len + j;
+    if (node < 0 || node >= T || at < 0 || at >= capacity) continue;
+    const int64_t source = static_cast<int64_t>(node) * row + in_row, sink = (static_cast<int64_t>(h) * capacity + at) * per_row + e;
+    const U k = from_k[source], v = from_v[source];
+    to_k[sink] = k;
+    to_v[sink] = v;
   }
 }
 
@@ -342,14 +359,18 @@ extern "C" int dtas_cache_append_f16(const void* K, const void* V, const void* p
       return fail("cache_append: a cache overlaps an input");
   if (overlaps(K_cache, cache_bytes, V_cache, cache_bytes)) return fail("cache_append: the caches overlap");
   const bool wide = d % 8 == 0 && aligned(K, 16) && aligned(V, 16) && aligned(K_cache, 16) && aligned(V_cache, 16);
-  const int64_t per_row = wide ? d / 8 : d, total = layers * batch * slots * kv_heads * per_row;
-  const int64_t grid = ceil_div(total, 256) < (int64_t{1} << 22) ? ceil_div(total, 256) : int64_t{1} << 22;
+  const int64_t per_row = wide ? d / 8 : d, row = kv_heads * per_row;
+  // a slot of all heads at least, two pieces (of K and V) per thread and turn where the rows are short; a workgroup's pieces are counted in 32 bits
+  if (row > INT32_MAX / 2) return fail("cache_append: the rows of a position are too long");
+  const int64_t run = row >= 256 ? 1 : 256 / row, runs = ceil_div(slots, run);
+  if (layers * batch * runs > INT32_MAX) return fail("cache_append: the launch has too many workgroups");
   auto go = [&](auto* tag) {
     using U = std::remove_pointer_t<decltype(tag)>;
-    hipLaunchKernelGGL(cache_append_kernel<U>, dim3(static_cast<unsigned>(grid), 2), dim3(256), 0, static_cast<hipStream_t>(stream),
+    hipLaunchKernelGGL(cache_append_kernel<U>, dim3(static_cast<unsigned>(layers * batch * runs)), dim3(256), 0, static_cast<hipStream_t>(stream),
                        static_cast<const U*>(K), static_cast<const U*>(V), static_cast<const int*>(path), static_cast<const int*>(count),
                        static_cast<U*>(K_cache), static_cast<U*>(V_cache), static_cast<const int*>(lens), static_cast<int>(batch),
-                       static_cast<int>(nodes), static_cast<int>(slots), static_cast<int>(kv_heads), static_cast<int>(per_row), capacity, total);
+                       static_cast<int>(nodes), static_cast<int>(slots), static_cast<int>(kv_heads), static_cast<int>(per_row), capacity, static_cast<int>(run),
+                       static_cast<int>(runs));
   };
   if (wide) go(static_cast<u32x4*>(nullptr));
   else go(static_cast<half_t*>(nullptr));
