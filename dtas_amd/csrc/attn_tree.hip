@@ -219,9 +219,8 @@ __device__ __forceinline__ int deal(const Sequences& s, int budget, int least, i
     per = more > per ? more : per + 1;
   }
 }
-// the part that has `slot`, or (slot < 0) the parts of sequence b
-__device__ __forceinline__ Part find_part(const TreeArgs& a, int batch, int unit, int slot, int b, int budget, int least, int most, int lane) {
-  if (budget == 0) return slot >= 0 ? Part{slot, 0, 1, slot} : Part{b, 0, 1, b};
+__device__ __forceinline__ Part find_part(const TreeArgs& a, int batch, int unit, int slot, int budget, int least, int most, int lane) {
+  if (budget == 0) return Part{slot, 0, 1, slot};
   if (batch == 1) {
     const int units = units_of(a.lens[0], a.capacity, unit, a.T);
     int per = (units + budget - 1) / budget;
@@ -235,7 +234,7 @@ __device__ __forceinline__ Part find_part(const TreeArgs& a, int batch, int unit
   for (int c = 0; c < batch; c += 64) {
     const int parts = (s.units(c, lane) + per - 1) / per;
     const int upto = sum_upto(parts);
-    const uint64_t here = slot >= 0 ? __builtin_amdgcn_ballot_w64(slot >= base + upto - parts && slot < base + upto) : b < c + 64 ? uint64_t{1} << (b - c) : 0;
+    const uint64_t here = __builtin_amdgcn_ballot_w64(slot >= base + upto - parts && slot < base + upto);
     if (here) {
       const int l = __builtin_ctzll(here);
       const int n = __builtin_amdgcn_readlane(parts, l), first = base + __builtin_amdgcn_readlane(upto, l) - n;
@@ -382,29 +381,35 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* counter, int parts, int
 }
 template <int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void join_parts(const TreeArgs& a, int b, int hk, int g, int row0, int my_rows, const float* shares, int parts, uint64_t* stats) {
-  constexpr int kShare = ROWS * (DP + 2);
+  constexpr int kShare = ROWS * (DP + 2), kAtOnce = 8;  // parts requested before the first is used: a trip to memory per eight
   const int tid = threadIdx.x;
+  uint64_t one[kAtOnce], other[kAtOnce];
+  auto request = [&](int at, int y0) {
+    const int i = at / (DP / 4), c = 4 * (at % (DP / 4));
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int y = y0 + u < parts ? y0 + u : parts - 1;
+      const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(y) * kShare + i * DP + c);
+      one[u] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      other[u] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  };
+  // (the thread's first sums are on their way while the statistics come)
+  const int last = my_rows * (DP / 4);
+  if (tid < last) request(tid, 0);
   for (int at = tid; at < parts * ROWS; at += THREADS)
     if (at % ROWS < my_rows)
       stats[at] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(at / ROWS) * kShare + ROWS * DP) + at % ROWS, __ATOMIC_RELAXED,
                                     __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  for (int at = tid; at < my_rows * (DP / 4); at += THREADS) {
+  for (int at = tid; at < last; at += THREADS) {
     const int i = at / (DP / 4), c = 4 * (at % (DP / 4));
-    if (c >= a.d) continue;
+    if (at != tid) request(at, 0);
     float best = -INFINITY, l = 0.f;
     for (int y = 0; y < parts; ++y) best = fmaxf(best, __builtin_bit_cast(float, static_cast<unsigned>(stats[y * ROWS + i])));
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    constexpr int kAtOnce = 8;  // shares requested before the first is used: a trip to memory per eight parts
     for (int y0 = 0; y0 < parts; y0 += kAtOnce) {
-      uint64_t one[kAtOnce], other[kAtOnce];
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const int y = y0 + u < parts ? y0 + u : parts - 1;
-        const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(y) * kShare + i * DP + c);
-        one[u] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        other[u] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+      if (y0 > 0) request(at, y0);
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
         if (y0 + u >= parts) break;
@@ -417,7 +422,7 @@ __device__ __forceinline__ void join_parts(const TreeArgs& a, int b, int hk, int
         v[3] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u] >> 32)), v[3]);
       }
     }
-    store_row4(out_row(a, b, hk, g, row0 + i) + c, v, 1.f / l);
+    if (c < a.d) store_row4(out_row(a, b, hk, g, row0 + i) + c, v, 1.f / l);
   }
 }
 
@@ -426,6 +431,7 @@ struct TreeGrid {
   int batch, slots, budget, row_groups;
   float* ws;
   unsigned* arrivals;
+  int* dealt;  // [batch][2], for the launch that joins many rows: a sequence's parts and its first slot
 };
 
 // ---- few rows: the W wavefronts take blocks of 32 keys in turn, each for all 16 RT rows and without a barrier until the end.  A lane's 8 channels
@@ -447,7 +453,7 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
   const int g = a.heads / a.kv_heads, R = a.Tq * g;
   const int slot = static_cast<int>(blockIdx.x % grid.slots), hk = static_cast<int>(blockIdx.x / grid.slots % a.kv_heads), rg = static_cast<int>(blockIdx.x / grid.slots / a.kv_heads);
-  const Part part = find_part(a, grid.batch, kBlock, slot, 0, grid.budget, W, 64 / RT, lane);
+  const Part part = find_part(a, grid.batch, kBlock, slot, grid.budget, W, 64 / RT, lane);
   if (part.b < 0) return;
   const int b = part.b;
   const int64_t len = clamp_len(a.lens[b], a.capacity);
@@ -646,9 +652,13 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
   const int g = a.heads / a.kv_heads, R = a.Tq * g;
   const int slot = static_cast<int>(blockIdx.x % grid.slots), hk = static_cast<int>(blockIdx.x / grid.slots % a.kv_heads), rg = static_cast<int>(blockIdx.x / grid.slots / a.kv_heads);
-  const Part part = find_part(a, grid.batch, kTile, slot, 0, grid.budget, 2, 64, lane);
+  const Part part = find_part(a, grid.batch, kTile, slot, grid.budget, 2, 64, lane);
   if (part.b < 0) return;
   const int b = part.b;
+  if (grid.budget > 0 && part.z == 0 && hk == 0 && rg == 0 && tid == 0) {
+    grid.dealt[2 * b] = part.parts;
+    grid.dealt[2 * b + 1] = part.first;
+  }
   const int64_t len = clamp_len(a.lens[b], a.capacity);
   const int cached = static_cast<int>((len + kTile - 1) / kTile), tiles = cached + 1;  // (the tree is one tile, the last)
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * part.z / part.parts), end = static_cast<int>(static_cast<int64_t>(tiles) * (part.z + 1) / part.parts);
@@ -875,37 +885,53 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
   }
 }
 
-// The parts of many rows joined: four rows of one problem and sequence per workgroup, a wavefront each
+// The parts of many rows joined: four rows of one problem and sequence per workgroup, a wavefront each, DP / 4 lanes to a part's row
 template <int DP>
-__global__ void __launch_bounds__(256) attn_tree_join_kernel(TreeArgs a, TreeGrid grid, int rows, int unit, int least, int most) {
+__global__ void __launch_bounds__(256) attn_tree_join_kernel(TreeArgs a, TreeGrid grid, int rows) {
+  constexpr int kLanes = DP / 4, kParts = 64 / kLanes;  // (several parts at a time)
   const int lane = threadIdx.x & 63, g = a.heads / a.kv_heads, R = a.Tq * g;
   const int r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), hk = blockIdx.y, b = blockIdx.z;
-  const Part part = find_part(a, grid.batch, unit, -1, b, grid.budget, least, most, lane);
-  if (part.parts == 1 || r >= R) return;
-  const int share_size = rows * (DP + 2), i = r % rows;
-  const float* shares = grid.ws + (static_cast<int64_t>(hk * grid.row_groups + r / rows) * grid.slots + part.first) * share_size;
-  // a lane holds a part's maximum and sum (at most 64 parts), then 4 channels
-  uint64_t two = 0xff800000u;
-  if (lane < part.parts) two = *(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(lane) * share_size + rows * DP) + i);
-  const float top = __builtin_bit_cast(float, static_cast<unsigned>(two)), best = wave_max(top), w = weight_of(top, best, a.scale_log2);
-  const float total = wave_sum(w * __builtin_bit_cast(float, static_cast<unsigned>(two >> 32)));
-  const float* from = shares + static_cast<int64_t>(i) * DP + 4 * lane;
-  if (4 * lane >= a.d) from = shares;  // (read, not used)
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (r >= R) return;
+  const int parts = grid.dealt[2 * b], share_size = rows * (DP + 2), i = r % rows;
+  if (parts == 1) return;
+  const float* shares = grid.ws + (static_cast<int64_t>(hk * grid.row_groups + r / rows) * grid.slots + grid.dealt[2 * b + 1]) * share_size;
+  const int sub = lane / kLanes, c = 4 * (lane % kLanes);
+  const float* from = shares + static_cast<int64_t>(i) * DP + c;
   constexpr int kAtOnce = 8;
-  for (int y0 = 0; y0 < part.parts; y0 += kAtOnce) {
-    f32x4 some[kAtOnce];
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) some[u] = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(y0 + u < part.parts ? y0 + u : part.parts - 1) * share_size);
+  f32x4 some[kAtOnce];
+  auto request = [&](int y0) {
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
-      if (y0 + u >= part.parts) break;
-      const float wy = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), y0 + u));
+      const int y = y0 + u * kParts + sub;
+      some[u] = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(y < parts ? y : parts - 1) * share_size);
+    }
+  };
+  request(0);
+  // a lane holds a part's maximum and sum (at most 64 parts)
+  uint64_t two = 0xff800000u;
+  if (lane < parts) two = *(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(lane) * share_size + rows * DP) + i);
+  const float top = __builtin_bit_cast(float, static_cast<unsigned>(two)), w = weight_of(top, wave_max(top), a.scale_log2);
+  const float total = wave_sum(w * __builtin_bit_cast(float, static_cast<unsigned>(two >> 32)));
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int y0 = 0; y0 < parts; y0 += kAtOnce * kParts) {
+    if (y0 > 0) request(y0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = fmaf(wy, some[u][j], v[j]);
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int y = y0 + u * kParts + sub;
+      if (y0 + u * kParts >= parts) break;
+      const float wy = __shfl(w, y & 63);
+      if (y < parts) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(wy, some[u][j], v[j]);
+      }
     }
   }
-  if (4 * lane < a.d) store_row4(out_row(a, b, hk, g, r) + 4 * lane, v, 1.f / total);
+  const f32x4 own = v;
+#pragma unroll
+  for (int k = 1; k < kParts; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += __shfl(own[j], (lane % kLanes + k * kLanes) & 63);  // (those of the first lanes, which store)
+  if (lane < kLanes && c < a.d) store_row4(out_row(a, b, hk, g, r) + c, v, 1.f / total);
 }
 
 // The launch of a kernel for `rows` rows and `threads` threads per workgroup and parts of at least `least` units of `unit` keys, at most `most` of
@@ -923,10 +949,12 @@ int launch_tree(Kernel kernel, const TreeArgs& a, int64_t batch, int DP, const T
   if (budget <= batch) budget = 0;  // every sequence in one piece
   const int64_t slots = budget == 0 ? batch : budget;
   if (batch > INT32_MAX || problems * slots > INT32_MAX) return fail("attn_tree: the launch has too many workgroups");
-  *grid = TreeGrid{static_cast<int>(batch), static_cast<int>(slots), static_cast<int>(budget), static_cast<int>(groups), nullptr, nullptr};
-  if (budget > 0 && split_scratch(s, static_cast<size_t>(problems * slots) * shape.rows * (DP + 2) * sizeof(float), counts ? static_cast<size_t>(problems * batch) : 1,
-                                  static_cast<int>(budget), &grid->ws, &grid->arrivals, lock) != 0)
+  *grid = TreeGrid{static_cast<int>(batch), static_cast<int>(slots), static_cast<int>(budget), static_cast<int>(groups), nullptr, nullptr, nullptr};
+  const size_t sums = static_cast<size_t>(problems * slots) * shape.rows * (DP + 2);
+  if (budget > 0 && split_scratch(s, (sums + 2 * static_cast<size_t>(batch)) * sizeof(float), counts ? static_cast<size_t>(problems * batch) : 1, static_cast<int>(budget), &grid->ws,
+                                  &grid->arrivals, lock) != 0)
     return -1;
+  if (budget > 0) grid->dealt = reinterpret_cast<int*>(grid->ws + sums);
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(problems * slots)), dim3(shape.threads), 0, s, a, *grid);
   return check_launch("attn_tree");
 }
@@ -945,7 +973,7 @@ int launch_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   if (grid.budget == 0) return 0;
   const int64_t rows = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
   hipLaunchKernelGGL(attn_tree_join_kernel<DP>, dim3(static_cast<unsigned>(ceil_div(rows, 4)), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
-                     dim3(256), 0, s, a, grid, shape.rows, shape.unit, shape.least, shape.most);
+                     dim3(256), 0, s, a, grid, shape.rows);
   return check_launch("attn_tree");
 }
 

@@ -423,7 +423,7 @@ extern "C" int dtas_gemv_q4_f16(const void* x, const void* Wq, const void* scale
   const half_t* xp = static_cast<const half_t*>(x);
   const half_t* sp = static_cast<const half_t*>(scale);
   const int group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
-  if (K > 0 && aligned(x, 16) && aligned(Wq, 16) && M <= 64 * int64_t{65535}) {
+  if (K > 0 && aligned(x, 16) && aligned(Wq, 16) && M <= 16 * int64_t{65535}) {
     const Q4Args a{xp, static_cast<const unsigned char*>(Wq), sp, y, M, N, K, 1, nullptr, nullptr};
     return group == 32 ? launch_q4_rows<1>(a, ep, s) : group == 64 ? launch_q4_rows<2>(a, ep, s) : launch_q4_rows<4>(a, ep, s);
   }
