@@ -207,6 +207,60 @@ def test_a_recorded_step_replays_the_eager_bits():
     assert int(eager.lens.min()) > n + 6
 
 
+class _Subclass(torch.Tensor):
+    """An object that only the Python body takes."""
+
+
+def _calls():
+    """(name, arguments, keywords, index of each output) of the operators' ordinary forms."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    half = lambda *s: torch.randn(*s, device="cuda", generator=g).half()
+    f = lambda *s: torch.rand(*s, device="cuda", generator=g)
+    z = lambda *s, dtype=torch.float16: torch.zeros(*s, device="cuda", dtype=dtype)
+    words = lambda N, K: torch.randint(-2 ** 31, 2 ** 31, (N, K // 8), device="cuda", generator=g, dtype=torch.int64).to(torch.int32)
+    i = lambda *v: torch.tensor(v, device="cuda", dtype=torch.int32)
+    yield "gemv_q4", [half(256), words(24, 256), half(24, 8).abs(), half(24), z(24)], {}, [4]
+    yield "gemv_q4", [half(1, 5, 256), words(24, 256).view(torch.uint32), half(24, 2).abs(), None, z(1, 5, 24)], {"epilogue": 3}, [4]
+    yield "gemv_q4", [half(5, 256), words(24, 256), half(24, 4).abs(), half(24), z(5, 24, dtype=torch.float32), 2, half(5, 24), half(5, 24)], {}, [4]
+    parents, lens = i(-1, 0, 0, -1, 0, 1).view(2, 3), i(9, 4)
+    tree = [half(2, 3, 4, 64), half(2, 3, 2, 64), half(2, 3, 2, 64), half(2, 2, 10, 64), half(2, 2, 10, 64), lens, parents, z(2, 3, 4, 64)]
+    yield "attn_tree", tree, {}, [7]
+    yield "attn_tree", [*tree[:7], z(2, 3, 4, 64)], {"scale": 0.5}, [7]
+    target, draft = torch.softmax(half(2, 3, 40).float(), -1), torch.softmax(half(2, 3, 40).float(), -1)
+    outs = [z(2, 3, dtype=torch.int32), z(2, dtype=torch.int32), z(2, dtype=torch.int32)]
+    yield "verify_tree", [target, draft, i(1, 7, 9, 2, 5, 39).view(2, 3), parents, f(2, 3), f(2) * 0.5 + 0.4, *outs], {}, [6, 7, 8]
+    yield "cache_append", [half(2, 2, 3, 2, 64), half(2, 2, 3, 2, 64), i(0, 2, -1, 0, 1, 2).view(2, 3), i(2, 3), z(2, 2, 2, 10, 64), z(2, 2, 2, 10, 64), i(0, 7)], {}, [4, 5]
+    yield "cache_append", [half(2, 3, 2, 64), half(2, 3, 2, 64), None, None, z(2, 2, 10, 64), z(2, 2, 10, 64), i(4, 7)], {}, [4, 5]
+
+
+def test_the_native_check_and_the_body_are_one_function(monkeypatch):
+    for name, args, kw, outs in _calls():
+        took = []
+        native = getattr(ops._fastcall, "_" + name)
+        results = []
+        for as_given in (True, False):
+            for at in outs:
+                args[at].zero_()
+            given = args if as_given else [a.as_subclass(_Subclass) if isinstance(a, torch.Tensor) else a for a in args]
+            with monkeypatch.context() as m:
+                m.setattr(ops._fastcall, "_" + name, lambda *a: took.append(native(*a)) or took[-1])
+                getattr(ops, name)(*given, **kw)
+            results.append([args[at].clone() for at in outs])
+        assert took == [True, False], name
+        for one, other in zip(*results):
+            assert one.count_nonzero() > 0 and torch.equal(one, other), name
+
+
+def test_calls_after_an_error_go_on():
+    h2 = lambda *s: torch.ones(*s, device="cuda", dtype=torch.float16)
+    i = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.int32)
+    out = h2(1, 1, 4, 64)
+    with pytest.raises(RuntimeError, match="share 3 key heads"):
+        ops.attn_tree(h2(1, 1, 4, 64), h2(1, 1, 3, 64), h2(1, 1, 3, 64), h2(1, 3, 5, 64), h2(1, 3, 5, 64), i(1), i(1, 1), out)
+    ops.attn_tree(h2(1, 1, 4, 64), h2(1, 1, 2, 64), h2(1, 1, 2, 64), h2(1, 2, 5, 64), h2(1, 2, 5, 64), i(1), i(1, 1), out)
+    assert bool((out == 1).all())
+
+
 def test_two_streams_and_two_threads_at_once():
     model = Model()
     steps = []

@@ -80,6 +80,13 @@ def test_sizes(M, N, K, group):
     check(M, N, K, group, 0)
 
 
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 65536), (4, 33, 20480), (3, 5000, 16384), (12, 50, 32768), (40, 70, 49152)])
+def test_long_k(M, N, K, group):
+    # K shared by workgroups because the LDS does not hold its scales, or x
+    check(M, N, K, group, 0)
+
+
 @pytest.mark.parametrize("epilogue", [0, 1, 2, 3])
 @pytest.mark.parametrize("M,N,K", [(1, 515, 2560), (2, 96, 512), (7, 100, 640), (24, 333, 1024), (50, 64, 2560)])
 def test_epilogues(M, N, K, epilogue):

@@ -118,6 +118,17 @@ def test_ragged_batches():
     check(make(40, 1, 1, 3, 2, 64, [7 * b for b in range(40)], 280))
 
 
+@pytest.mark.parametrize("B,Hkv,group,T", [(100, 1, 2, 1), (70, 2, 5, 8), (130, 1, 1, 3), (300, 1, 1, 1), (66, 1, 70, 1)])
+def test_many_sequences(B, Hkv, group, T):
+    # more sequences than a wavefront has lanes, their keys dealt out to the workgroups
+    check(make(B, T, T, Hkv, group, 64, [(37 * b * b) % 700 for b in range(B)], 700))
+
+
+def test_one_long_sequence_among_short_ones():
+    for group, T in ((2, 1), (8, 7)):
+        check(make(6, T, T, 1, group, 64, [3, 9001, 0, 40, 1, 700], 9001))
+
+
 def test_lengths_are_clipped_to_the_cache():
     host = make(4, 3, 3, 2, 2, 64, [-5, 1 << 30, 70, 71], 70)
     check(host)
@@ -225,6 +236,14 @@ def test_offsets_past_32_bits():
     ops.attn_tree(host["Q"].cuda(), host["K"].cuda(), host["V"].cuda(), Kc, Vc, host["lens"].cuda(), host["parents"].cuda(), out)
     want, tolerance = expected(host)
     assert bool(((out.cpu().double() - want).abs() <= tolerance).all())
+
+
+def test_what_lies_in_the_cache_and_is_seen_spreads():
+    host = make(1, 4, 4, 2, 2, 80, [100], 100, "chain")
+    host["Vc"][0, 0, 50, 3], host["Kc"][0, 1, 20, 0] = float("inf"), float("nan")
+    got = launch(host)
+    assert bool((got[0, :, :2, 3] == float("inf")).all()) and bool(torch.isfinite(got[0, :, :2, :3]).all()) and bool(torch.isfinite(got[0, :, :2, 4:]).all())
+    assert bool(torch.isnan(got[0, :, 2:]).all())
 
 
 def test_refusals():
