@@ -49,20 +49,31 @@ __global__ void __launch_bounds__(256) gemv_q4_scalar_kernel(const half_t* __res
 // ---- rows on 16-byte boundaries: the matrix cores -------------------------------------------------------------------------------
 // A wavefront takes 16 columns and chunks of 128 k.  A lane loads 16 bytes of one row of W, 32 weights: the four lanes of a column hold a chunk.  Two
 // exchanges of halves and two of quarters turn the four words around, so that word i of the four lanes is the i-th 32 weights in order, which is an
-// operand of v_mfma_f32_16x16x32_f16 once it is fp16.  Seven instructions do that: the bytes' nibbles, even and odd, and four permutes
-// that put them into halves.  A nibble as the bits of an fp16 number is nibble * 2^-24, a subnormal, which the matrix cores take as it is: no
-// conversion, and the offset goes through them as well, as the accumulator that a first MFMA fills with -7 * 2^-24 * (the sum of x over the group) --
-// both exact, and 2^24 is part of the scale.  The group's sum leaves the accumulator with one multiply-add per row of x and group.
+// operand of v_mfma_f32_16x16x32_f16 once it is fp16.  Nine instructions do that: a nibble in the low bits of the fp16 number 1024 is 1024 + nibble, or
+// 1024 + 16 nibble four bits up; one packed add (or multiply-add) leaves nibble - 7, exactly.  That pairs the weights k and k + 4 of a word, so x lies in
+// the LDS in the same order.  (The nibble as a subnormal, its offset through the matrix cores as well, takes fewer instructions and loses the sum's
+// low bits: products are aligned by the exponents of their factors, a subnormal's being 2^-14 whatever its size, and ten bits fall off.)
+// The group's sum leaves the accumulator with one multiply-add per row of x and group.
 // Rows of x lie at 4 (r % 4) + r / 4 of the operand: up to four rows fill one accumulator register of the lanes.
 // The scales pass through the LDS: eight bytes of each of sixteen rows, chunk by chunk, take more lines from the caches than W does
 // (1 x 50280 x 4096: 34 us).  W's loads are plain: what fits the Infinity Cache is read from there (streamed: 5 .. 10 % longer).
 constexpr int kChunk = 128;
 
+// weights 0 4 1 5 2 6 3 7 of a word
 __device__ __forceinline__ f16x8 halves_of(unsigned word) {
-  const unsigned even = word & 0x0f0f0f0fu, odd = (word >> 4) & 0x0f0f0f0fu;
-  const u32x4 h = {__builtin_amdgcn_perm(odd, even, 0x0c040c00u), __builtin_amdgcn_perm(odd, even, 0x0c050c01u),
-                   __builtin_amdgcn_perm(odd, even, 0x0c060c02u), __builtin_amdgcn_perm(odd, even, 0x0c070c03u)};
-  return __builtin_bit_cast(f16x8, h);
+  constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u, k1024 = 0x64006400u;
+  const f16x2 less = {-1031.f16, -1031.f16}, sixteenth = {0.0625f16, 0.0625f16}, less_high = {-71.f16, -71.f16};
+  const unsigned next = word >> 8;
+  const f16x2 a = __builtin_bit_cast(f16x2, (word & kLow) | k1024) + less;
+  const f16x2 b = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (word & kHigh) | k1024), sixteenth, less_high);
+  const f16x2 c = __builtin_bit_cast(f16x2, (next & kLow) | k1024) + less;
+  const f16x2 d = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (next & kHigh) | k1024), sixteenth, less_high);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// eight of x in the weights' order
+__device__ __forceinline__ u32x4 in_order(u32x4 x) {
+  return u32x4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
+               __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
 }
 __device__ __forceinline__ void turn(u32x4& w) {
   const auto ac = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), bd = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
@@ -115,9 +126,6 @@ __device__ __forceinline__ void stage_scales(char* lds, const Q4Args& a, int64_t
 // The products of one chunk for MT row tiles and one column tile, onto acc; x(mt, i): the operand of its i-th 32 k
 template <int MT, int JN, int GS, typename X>
 __device__ __forceinline__ void multiply(u32x4 w, X x, const char* scales, f32x4 (&acc)[MT]) {
-  constexpr unsigned short kSeven = 0x8007;  // -7 * 2^-24
-  const half_t seven = __builtin_bit_cast(half_t, kSeven);
-  const f16x8 offset = {seven, seven, seven, seven, seven, seven, seven, seven};
   turn(w);
   half_t s[4 / GS];
   __builtin_memcpy(s, __builtin_assume_aligned(scales, 8 / GS), sizeof s);
@@ -130,13 +138,9 @@ __device__ __forceinline__ void multiply(u32x4 w, X x, const char* scales, f32x4
     for (int u = 0; u < GS; ++u) {
       const f16x8 h = halves_of(w[g * GS + u]);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const f16x8 v = x(mt, g * GS + u);
-        part[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, offset, part[mt], 0, 0, 0);
-        part[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, h, part[mt], 0, 0, 0);
-      }
+      for (int mt = 0; mt < MT; ++mt) part[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x(mt, g * GS + u), h, part[mt], 0, 0, 0);
     }
-    const float scale = static_cast<float>(s[g]) * 16777216.f;
+    const float scale = static_cast<float>(s[g]);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(64 * W) gemv_q4_kernel(Q4Args a, Q4Epilogue ep
   for (int t = tid; t < pieces * M; t += 64 * W) {
     const int r = t / pieces, c = t % pieces;
     const int64_t k = lo * kChunk + c * 8;
-    reinterpret_cast<u32x4*>(lds)[t] = k < a.K ? *reinterpret_cast<const u32x4*>(a.x + r * a.K + k) : u32x4{0u, 0u, 0u, 0u};
+    reinterpret_cast<u32x4*>(lds)[t] = k < a.K ? in_order(*reinterpret_cast<const u32x4*>(a.x + r * a.K + k)) : u32x4{0u, 0u, 0u, 0u};
   }
   char* lds_s = lds + row_bytes * M;
   stage_scales<GS, 64 * W>(lds_s, a, n0, 16, lo, hi);
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(64 * CT * KG) gemv_q4_rows_kernel(Q4Args a, Q4
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
       const int id = n * 64 * W + tid, c = id % (kChunk / 8), sl = id / (kChunk / 8) % kAll, r = id / (kChunk / 8 * kAll);
-      *reinterpret_cast<u32x4*>(lds + stage * kStage + (sl * kRows + r) * kPitch + c * 16) = xr[n];
+      *reinterpret_cast<u32x4*>(lds + stage * kStage + (sl * kRows + r) * kPitch + c * 16) = in_order(xr[n]);
     }
   };
   load_all(lo);

@@ -80,6 +80,25 @@ def test_sizes(M, N, K, group):
     check(M, N, K, group, 0)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 4, 5, 16, 17, 64])
+def test_small_products_beside_a_large_row_element(M, group):
+    # x is one number of 1024 per group, which meets the weight 0, and whole numbers of 2^-10 up to 31: every product and every sum is a
+    # whole number of 2^-10 below 2^24 of them (31 * 8 * 640 < 2^18), which fp32 holds: the sum is the exact one in any order
+    N, K = 48, 640
+    g = torch.Generator().manual_seed(M)
+    nibbles = torch.randint(0, 16, (N, K), generator=g)
+    x = torch.randint(-31, 32, (M, K), generator=g).double() / 1024
+    x[:, 5::group] = 1024
+    nibbles[:, 5::group] = 7
+    words = (nibbles.view(N, K // 8, 8) << (4 * torch.arange(8))).sum(-1)
+    words = (words - (words >> 31 << 32)).to(torch.int32)
+    y = torch.empty(M, N, device="cuda")
+    zero, one = torch.zeros(M, N, dtype=torch.float16, device="cuda"), torch.ones(N, K // group, dtype=torch.float16, device="cuda")
+    ops.gemv_q4(x.half().cuda(), words.cuda(), one, None, y, _lib.EPI_BIAS_ADD2_CAST_F32, zero, zero)
+    assert torch.equal(y.cpu().double(), x @ (nibbles - 7).double().T)
+
+
 @pytest.mark.parametrize("group", [32, 128])
 @pytest.mark.parametrize("M,N,K", [(1, 40, 65536), (4, 33, 20480), (3, 5000, 16384), (12, 50, 32768), (40, 70, 49152)])
 def test_long_k(M, N, K, group):
