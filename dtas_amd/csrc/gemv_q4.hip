@@ -373,7 +373,24 @@ int launch_q4(Kernel kernel, Q4Args a, const Q4Epilogue& ep, int cols, int rows,
   const int64_t needed = ceil_div(chunks, (lds_most - lds_fixed) / lds_per_chunk);
   splits = splits < needed ? needed : splits;
   splits = splits < 1 ? 1 : splits;
-  if (across > INT32_MAX || down > 65535 || splits > 65535) return fail("gemv_q4: the launch has too many workgroups");
+  // many rows of a long K: in slabs whose parts fit the workspace well
+  constexpr int64_t kMostBytes = int64_t{256} << 20;
+  const int64_t bytes = splits > 1 ? tiles * splits * values * 4 : 0, by_bytes = ceil_div(bytes, kMostBytes), by_grid = ceil_div(down, 65535);
+  const int64_t slabs = by_bytes > by_grid ? by_bytes : by_grid;
+  if (slabs > 1 && down > 1) {
+    const int64_t step = (down / slabs > 1 ? down / slabs : 1) * rows;
+    for (int64_t m = 0; m < a.M; m += step) {
+      Q4Args part = a;
+      Q4Epilogue at = ep;
+      part.M = a.M - m < step ? a.M - m : step;
+      part.x = a.x + m * a.K;
+      part.y = static_cast<char*>(a.y) + m * a.N * (ep.kind == DTAS_EPI_BIAS_ADD2_CAST_F32 ? 4 : 2);
+      if (ep.res1) at.res1 = ep.res1 + m * a.N, at.res2 = ep.res2 + m * a.N;
+      if (launch_q4(kernel, part, at, cols, rows, threads, values, fill, least, lds_per_chunk, lds_fixed, lds_most, s) != 0) return -1;
+    }
+    return 0;
+  }
+  if (across > INT32_MAX || splits > 65535) return fail("gemv_q4: the launch has too many workgroups");
   a.splits = static_cast<int>(splits);
   std::unique_lock<std::recursive_mutex> lock;
   if (splits > 1 && split_scratch(s, static_cast<size_t>(tiles * splits) * values * sizeof(float), static_cast<size_t>(tiles), a.splits, &a.ws, &a.arrivals, &lock) != 0) return -1;
@@ -393,7 +410,7 @@ int launch_q4_many(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
 template <int GS>
 int launch_q4_rows(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
   // few columns: more wavefronts to each sixteen.  2560 x 10240 (160 workgroups) on 4 / 8 / 16 wavefronts 14.9 / 10.4 / 7.9 us, 7680 x 2560 (480) 7.2 / 6.2 / 6.3,
-  // 50280 x 4096 (3143) 28.8 / 31.5 / 40.5; four chunks requested at once instead of two are level to 10 % longer
+  // 50280 x 4096 (3143) 27.0 (28.8 when the others were measured) / 31.5 / 40.5; four chunks requested at once instead of two are level to 10 % longer
   if (a.M <= 4) return a.N <= 16 * 256 ? launch_q4_few<GS, 16, 2>(a, ep, s) : a.N <= 16 * 1024 ? launch_q4_few<GS, 8, 2>(a, ep, s) : launch_q4_few<GS, 4, 2>(a, ep, s);
   if (a.M <= 16) return launch_q4_many<1, GS, 4, 4, 2>(a, ep, s);
   // by 32 rows, W again for the next 32: 64 rows at once are behind but for the widest W (64 x 2560 x 10240 25.4 us against 18.3, 64 x 4096 x 4096 17.3 / 12.8,
@@ -427,7 +444,7 @@ extern "C" int dtas_gemv_q4_f16(const void* x, const void* Wq, const void* scale
   const half_t* xp = static_cast<const half_t*>(x);
   const half_t* sp = static_cast<const half_t*>(scale);
   const int group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
-  if (K > 0 && aligned(x, 16) && aligned(Wq, 16) && M <= 16 * int64_t{65535}) {
+  if (K > 0 && aligned(x, 16) && aligned(Wq, 16)) {
     const Q4Args a{xp, static_cast<const unsigned char*>(Wq), sp, y, M, N, K, 1, nullptr, nullptr};
     return group == 32 ? launch_q4_rows<1>(a, ep, s) : group == 64 ? launch_q4_rows<2>(a, ep, s) : launch_q4_rows<4>(a, ep, s);
   }

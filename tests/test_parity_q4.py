@@ -80,6 +80,18 @@ def test_sizes(M, N, K, group):
     check(M, N, K, group, 0)
 
 
+def test_many_rows_of_a_long_k():
+    # the parts of all rows together are more than the workspace is asked for at once: several launches
+    M, N, K, group = 4100, 8192, 5120, 32
+    host, dev = make(M, N, K, group, 1)
+    y = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    ops.gemv_q4(*dev[:4], y, _lib.EPI_BIAS_ADD2, *dev[4:])
+    for rows in ([0, 31, 32, 1023, 2015, 2016, 2047, 2048, 2049], [4063, 4064, 4095, 4096, 4099]):
+        value, slack = expected([host[0][rows], *host[1:4], host[4][rows], host[5][rows]], _lib.EPI_BIAS_ADD2)
+        assert bool(((y[rows].cpu().double() - value).abs() <= slack).all())
+    assert bool(torch.isfinite(y).all())
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("M", [1, 4, 5, 16, 17, 64])
 def test_small_products_beside_a_large_row_element(M, group):
