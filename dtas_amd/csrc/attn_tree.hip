@@ -637,7 +637,8 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid 
 // of V): K and V are read once for up to 16 RT W rows, and no sum crosses wavefronts.  A tile is two steps: V(t) turns its scores into weights
 // (vector instructions), M(t) multiplies them with its values and the next tile's keys with Q (the matrix cores).  With eight wavefronts the second four
 // run one step behind the first, so that each SIMD has one wavefront in either step; left to themselves the two do the same at the same
-// time (256 rows of 128 against 65533 keys, 8 key heads: 118 us, with the turns 101 .. 110).
+// time (256 rows of 128 against 65533 keys, 8 key heads: 118 us, with the turns 101 .. 110).  Stages that the loads write themselves, four of each, were level
+// (103 us; 84 without any loads, 69 with nothing but them).
 //   tile t's keys are read in M(t - 1), its values in M(t): steps 2 t - 1 and 2 t + 1 of the first four, one later of the others.  What a wavefront
 //   loaded of K it stores in V(t) for tile t + 1 (the others: t + 2), of V for tile t (t + 1): behind the last reads of the tile that had the
 //   stage before, and a barrier ahead of the first of its own.
@@ -1007,7 +1008,7 @@ extern "C" int dtas_attn_tree_f16(const void* Q, const void* K, const void* V, c
   constexpr int64_t kMost = int64_t{1} << 60;
   if (heads > 65535 || batch > (int64_t{1} << 31) || capacity > INT32_MAX || capacity > kMost / d / kv_heads / batch)
     return fail("attn_tree: the extents overflow");
-  if (!(scale >= -3.0e38f && scale <= 3.0e38f)) return fail("attn_tree: the scale is not a finite number");
+  if (!(scale >= -2.0e38f && scale <= 2.0e38f)) return fail("attn_tree: the scale is not a finite number up to 2e38");
   if (!Q || !K || !V || !lens || !parents || !out || (capacity > 0 && (!K_cache || !V_cache))) return fail("attn_tree: NULL buffer");
   const int64_t out_bytes = batch * rows * heads * d * 2, new_bytes = batch * nodes * kv_heads * d * 2, cache_bytes = batch * kv_heads * capacity * d * 2;
   if (overlaps(out, out_bytes, Q, out_bytes) || overlaps(out, out_bytes, K, new_bytes) || overlaps(out, out_bytes, V, new_bytes) ||

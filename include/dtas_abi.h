@@ -421,15 +421,15 @@ int dtas_gemv_q8_f16(const void* x, const void* Wq, const void* scale, const voi
  *
  * A tree holds up to DTAS_MAX_TREE_NODES nodes per sequence, parents first: the parent of node i is parents[i] where that lies in
  * [0, i); any other value leaves i without one.  Device buffers of counts and indices (lens, parents, tokens, path, count) are
- * int32; values outside their range are treated as stated, never followed. */
+ * int32; values outside their range are treated as stated, never followed.  The first three use the split-K workspace, under the rules
+ * stated at the top of this file. */
 #define DTAS_MAX_TREE_NODES 64
 
 /* ---- 4-bit weights with fp16 group scales: y[M,N] = epilogue(x[M,K] . W^T), W[n,k] = (nibble - 7) * scale[n, k/group] ----
  * Wq[N, K/8] uint32: element k of a row is bits 4 (k % 8) .. + 3 of word k / 8; scale[N, K/group] fp16, group 32, 64 or 128, K a
  * multiple of it.  The weights are not rounded: a group's products are summed in fp32 and scaled there.  bias[N] or NULL;
  * epilogues as dtas_gemm_f16_fused (res1, res2 [M,N] with the ADD2 kinds, NULL otherwise; y fp32 with ADD2_CAST_F32), but in
- * fp32 with one rounding at the end, GELU by erfc.  Made for one row and the few of a tree: W is read again for every 32 rows.  A long K
- * is shared by workgroups that meet in the split-K workspace where the columns alone leave CUs idle. */
+ * fp32 with one rounding at the end, GELU by erfc.  Made for one row and the few of a tree: W is read again for every 32 rows. */
 int dtas_gemv_q4_f16(const void* x, const void* Wq, const void* scale, const void* bias, const void* res1, const void* res2, void* y,
                      int64_t M, int64_t N, int64_t K, int32_t group, int32_t epilogue, void* stream);
 
@@ -439,7 +439,8 @@ int dtas_gemv_q4_f16(const void* x, const void* Wq, const void* scale, const voi
  * Q and out [batch, rows, heads, d], K and V [batch, nodes, kv_heads, d] (the nodes' own), K_cache and V_cache
  * [batch, kv_heads, capacity, d], all fp16; lens[batch] (clipped to [0, capacity]), parents[batch, nodes].  heads is a multiple of
  * kv_heads; query head h reads key head h / (heads / kv_heads).  d up to 256; multiples of 8 on 16-byte boundaries run on the matrix
- * cores, others element by element.  fp32 scores and sums.  Keys are shared over workgroups that meet in the split-K workspace. */
+ * cores, others element by element.  fp32 scores, statistics and sums; on the matrix cores a weight is rounded to fp16 for its product with the
+ * values.  scale is a finite number up to 2e38 either way. */
 int dtas_attn_tree_f16(const void* Q, const void* K, const void* V, const void* K_cache, const void* V_cache, const void* lens,
                        const void* parents, void* out, int64_t batch, int64_t nodes, int64_t rows, int64_t heads, int64_t kv_heads,
                        int64_t d, int64_t capacity, float scale, void* stream);

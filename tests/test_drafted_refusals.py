@@ -44,7 +44,7 @@ def test_gemv_q4_refuses(bad, why):
     (dict(batch=-1), "negative extent"), (dict(capacity=-1), "negative extent"), (dict(nodes=65, rows=65), "up to 64 nodes"),
     (dict(rows=10), "10 query rows of a tree of 9"), (dict(heads=7), "share 2 key heads"), (dict(kv_heads=0), "share 0 key heads"),
     (dict(d=257), "up to 256"), (dict(capacity=1 << 31), "overflow"), (dict(heads=65536), "overflow"),
-    (dict(batch=1 << 31, capacity=1 << 30, kv_heads=8), "overflow"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
+    (dict(batch=1 << 31, capacity=1 << 30, kv_heads=8), "overflow"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(scale=-3e38), "finite"),
     *((dict([(name, None)]), "NULL") for name in ("Q", "K", "V", "Kc", "Vc", "lens", "parents", "out")),
     *((dict(out=at), "overlaps") for at in (A, B, C, D + 64, E, F, G))])
 def test_attn_tree_refuses(bad, why):
