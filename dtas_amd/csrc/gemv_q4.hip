@@ -61,7 +61,9 @@ constexpr int kChunk = 128;
 
 // weights 0 4 1 5 2 6 3 7 of a word
 __device__ __forceinline__ f16x8 halves_of(unsigned word) {
-  constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u, k1024 = 0x64006400u;
+  constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+  unsigned k1024 = 0x64006400u;
+  asm("" : "+v"(k1024));  // (a register: two constants of one instruction would make it two)
   const f16x2 less = {-1031.f16, -1031.f16}, sixteenth = {0.0625f16, 0.0625f16}, less_high = {-71.f16, -71.f16};
   const unsigned next = word >> 8;
   const f16x2 a = __builtin_bit_cast(f16x2, (word & kLow) | k1024) + less;
@@ -92,27 +94,36 @@ struct Q4Args {
   unsigned* arrivals;
 };
 
-// One chunk of a row of W.  In the last chunk, of 32, 64 or 96, the lanes behind its end read the last 32 again: they meet zeros of x.
-__device__ __forceinline__ u32x4 load_w(const unsigned char* row, int64_t chunk, int64_t K, int quarter) {
-  const int64_t k = chunk * kChunk;
-  const int blocks = K - k >= kChunk ? 4 : static_cast<int>((K - k) / 32);
-  return *reinterpret_cast<const u32x4*>(row + k / 2 + (quarter < blocks ? quarter : blocks - 1) * 16);
+// What a workgroup has of K, counted from its first chunk (the LDS holds all its scales: few)
+struct Q4Part {
+  int64_t lo;       // its first chunk
+  int chunks, len;  // its chunks and k
+};
+__device__ __forceinline__ Q4Part part_of(const Q4Args& a) {
+  const int64_t chunks = (a.K + kChunk - 1) / kChunk, lo = chunks * blockIdx.y / a.splits, hi = chunks * (blockIdx.y + 1) / a.splits;
+  const int64_t end = hi * kChunk < a.K ? hi * kChunk : a.K;
+  return {lo, static_cast<int>(hi - lo), static_cast<int>(end - lo * kChunk)};
 }
-// Scales of `cols` rows from n0 on, chunks [lo, hi), into the LDS: a row is an odd number of 8-byte pieces (sixteen rows fall on different banks).
+// One chunk of a row of W (from the part's first on).  In the last chunk, of 32, 64 or 96, the lanes behind its end read the last 32 again: they meet zeros of x.
+__device__ __forceinline__ u32x4 load_w(const unsigned char* row, int chunk, int len, int quarter) {
+  const int left = (len - chunk * kChunk) / 32;
+  return *reinterpret_cast<const u32x4*>(row + (chunk * (kChunk / 2) + (quarter < left ? quarter : left - 1) * 16));
+}
+// Scales of `cols` rows from n0 on, of one part of K, into the LDS: a row is an odd number of 8-byte pieces (sixteen rows fall on different banks).
 // What lies behind the row's last scale is that one again (it meets sums of zero).
 template <int GS>
 __host__ __device__ constexpr int scale_pitch(int64_t chunks) {
   return static_cast<int>((chunks * (4 / GS) + 3) / 4) | 1;
 }
 template <int GS, int THREADS>
-__device__ __forceinline__ void stage_scales(char* lds, const Q4Args& a, int64_t n0, int cols, int64_t lo, int64_t hi) {
+__device__ __forceinline__ void stage_scales(char* lds, const Q4Args& a, int64_t n0, int cols, const Q4Part& part) {
   constexpr int kScales = 4 / GS;
-  const int64_t groups = a.K / (32 * GS), first = lo * kScales;
-  const int pieces = static_cast<int>(((hi - lo) * kScales + 3) / 4), pitch = scale_pitch<GS>(hi - lo);
+  const int64_t row = a.K / (32 * GS), first = part.lo * kScales;
+  const int pieces = (part.chunks * kScales + 3) / 4, pitch = scale_pitch<GS>(part.chunks);
+  const int groups = static_cast<int>(row - first < 4 * pieces ? row - first : 4 * pieces);  // those there are
   for (int t = threadIdx.x; t < cols * pieces; t += THREADS) {
-    const int r = t / pieces, c = t % pieces;
-    const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1, g = first + 4 * c;
-    const half_t* from = a.S + n * groups;
+    const int r = t / pieces, c = t % pieces, g = 4 * c;
+    const half_t* from = a.S + (n0 + r < a.N ? n0 + r : a.N - 1) * row + first;
     f16x4 v;
     if (g + 4 <= groups) {
       __builtin_memcpy(&v, from + g, 8);
@@ -171,37 +182,37 @@ __global__ void __launch_bounds__(64 * W) gemv_q4_kernel(Q4Args a, Q4Epilogue ep
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15, M = static_cast<int>(a.M);
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const int64_t chunks = (a.K + kChunk - 1) / kChunk, lo = chunks * blockIdx.y / a.splits, hi = chunks * (blockIdx.y + 1) / a.splits;
-  const unsigned char* w_at = a.Wq + (n0 + i16 < a.N ? n0 + i16 : a.N - 1) * (a.K / 2);  // columns past N repeat the last; never stored
+  const Q4Part part = part_of(a);
+  const unsigned char* w_at = a.Wq + (n0 + i16 < a.N ? n0 + i16 : a.N - 1) * (a.K / 2) + part.lo * (kChunk / 2);  // columns past N repeat the last; never stored
   u32x4 some[D];
-  auto chunk_of = [&](int64_t base, int d) { return base + (d / 2 * W + wave) * 2 + d % 2; };
-  auto load_all = [&](int64_t base) {
+  auto chunk_of = [&](int base, int d) { return base + (d / 2 * W + wave) * 2 + d % 2; };
+  auto load_all = [&](int base) {
 #pragma unroll
     for (int d = 0; d < D; ++d)
-      if (chunk_of(base, d) < hi) some[d] = load_w(w_at, chunk_of(base, d), a.K, quarter);
+      if (chunk_of(base, d) < part.chunks) some[d] = load_w(w_at, chunk_of(base, d), part.len, quarter);
   };
-  load_all(lo);
-  const int row_bytes = static_cast<int>(hi - lo) * (kChunk * 2), pieces = row_bytes / 16;
+  load_all(0);
+  const int row_bytes = part.chunks * (kChunk * 2), pieces = row_bytes / 16;
+  const half_t* x_from = a.x + part.lo * kChunk;
   for (int t = tid; t < pieces * M; t += 64 * W) {
     const int r = t / pieces, c = t % pieces;
-    const int64_t k = lo * kChunk + c * 8;
-    reinterpret_cast<u32x4*>(lds)[t] = k < a.K ? in_order(*reinterpret_cast<const u32x4*>(a.x + r * a.K + k)) : u32x4{0u, 0u, 0u, 0u};
+    reinterpret_cast<u32x4*>(lds)[t] = c * 8 < part.len ? in_order(*reinterpret_cast<const u32x4*>(x_from + r * a.K + c * 8)) : u32x4{0u, 0u, 0u, 0u};
   }
   char* lds_s = lds + row_bytes * M;
-  stage_scales<GS, 64 * W>(lds_s, a, n0, 16, lo, hi);
+  stage_scales<GS, 64 * W>(lds_s, a, n0, 16, part);
   __syncthreads();
   // row r of x is row 4 r of the operand; the others, never stored, repeat the last
   const char* x_at = lds + ((i16 >> 2) < M ? i16 >> 2 : M - 1) * row_bytes + quarter * 16;
-  const char* s_at = lds_s + i16 * scale_pitch<GS>(hi - lo) * 8;
+  const char* s_at = lds_s + i16 * scale_pitch<GS>(part.chunks) * 8;
   f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-  for (int64_t base = lo; base < hi; base += W * D) {
+  for (int base = 0; base < part.chunks; base += W * D) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      const int at = static_cast<int>(chunk_of(base, d) - lo);
-      if (chunk_of(base, d) >= hi) break;
+      const int at = chunk_of(base, d);
+      if (at >= part.chunks) break;
       multiply<1, 1, GS>(some[d], [&](int, int i) { return *reinterpret_cast<const f16x8*>(x_at + at * (kChunk * 2) + i * 64); }, s_at + at * (8 / GS), acc);
     }
-    if (base + W * D < hi) load_all(base + W * D);
+    if (base + W * D < part.chunks) load_all(base + W * D);
   }
   sums[wave][lane] = acc[0][0];
   __syncthreads();
@@ -241,21 +252,26 @@ __global__ void __launch_bounds__(64 * CT * KG) gemv_q4_rows_kernel(Q4Args a, Q4
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
   const int ct = wave % CT, kg = wave / CT;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kCols, m0 = static_cast<int64_t>(blockIdx.z) * kRows;
-  const int64_t chunks = (a.K + kChunk - 1) / kChunk, lo = chunks * blockIdx.y / a.splits, hi = chunks * (blockIdx.y + 1) / a.splits;
+  const Q4Part part = part_of(a);
   const int64_t col = n0 + ct * 16 + i16;
-  const unsigned char* w_at = a.Wq + (col < a.N ? col : a.N - 1) * (a.K / 2);  // columns past N repeat the last; never stored
+  const unsigned char* w_at = a.Wq + (col < a.N ? col : a.N - 1) * (a.K / 2) + part.lo * (kChunk / 2);  // columns past N repeat the last; never stored
   u32x4 w[SL], xr[kPieces];
-  auto load_all = [&](int64_t base) {
+  const half_t* x_from[kPieces];
+  int x_k[kPieces];
+#pragma unroll
+  for (int n = 0; n < kPieces; ++n) {
+    // piece: row, then chunk, then 16 bytes; rows past M repeat the last, never stored
+    const int id = n * 64 * W + tid, r = id / (kChunk / 8 * kAll);
+    x_k[n] = id % (kChunk / 8 * kAll) * 8;
+    x_from[n] = a.x + (m0 + r < a.M ? m0 + r : a.M - 1) * a.K + part.lo * kChunk + x_k[n];
+  }
+  auto load_all = [&](int base) {
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl)
-      if (base + kg * SL + sl < hi) w[sl] = load_w(w_at, base + kg * SL + sl, a.K, quarter);
+      if (base + kg * SL + sl < part.chunks) w[sl] = load_w(w_at, base + kg * SL + sl, part.len, quarter);
 #pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
-      // piece: row, then chunk, then 16 bytes; rows past M repeat the last, never stored
-      const int id = n * 64 * W + tid, c = id % (kChunk / 8), sl = id / (kChunk / 8) % kAll, r = id / (kChunk / 8 * kAll);
-      const int64_t k = (base + sl) * kChunk + c * 8, m = m0 + r < a.M ? m0 + r : a.M - 1;
-      xr[n] = base + sl < hi && k < a.K ? *reinterpret_cast<const u32x4*>(a.x + m * a.K + k) : u32x4{0u, 0u, 0u, 0u};
-    }
+    for (int n = 0; n < kPieces; ++n)
+      xr[n] = base * kChunk + x_k[n] < part.len ? *reinterpret_cast<const u32x4*>(x_from[n] + base * kChunk) : u32x4{0u, 0u, 0u, 0u};
   };
   auto keep_x = [&](int stage) {
 #pragma unroll
@@ -264,28 +280,28 @@ __global__ void __launch_bounds__(64 * CT * KG) gemv_q4_rows_kernel(Q4Args a, Q4
       *reinterpret_cast<u32x4*>(lds + stage * kStage + (sl * kRows + r) * kPitch + c * 16) = in_order(xr[n]);
     }
   };
-  load_all(lo);
-  stage_scales<GS, 64 * W>(lds_s, a, n0, kCols, lo, hi);
+  load_all(0);
+  stage_scales<GS, 64 * W>(lds_s, a, n0, kCols, part);
   keep_x(0);
   __syncthreads();
-  const char* s_at = lds_s + (ct * 16 + i16) * scale_pitch<GS>(hi - lo) * 8;
+  const char* s_at = lds_s + (ct * 16 + i16) * scale_pitch<GS>(part.chunks) * 8;
   const char* x_at = lds + (kg * SL * kRows + (i16 >> 2) + 4 * (i16 & 3)) * kPitch + quarter * 16;
   f32x4 acc[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
   int stage = 0;
-  for (int64_t base = lo; base < hi; base += kAll, stage ^= 1) {
+  for (int base = 0; base < part.chunks; base += kAll, stage ^= 1) {
     u32x4 now[SL];
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) now[sl] = w[sl];
-    const bool more = base + kAll < hi;
+    const bool more = base + kAll < part.chunks;
     if (more) load_all(base + kAll);
 #pragma unroll
     for (int sl = 0; sl < SL; ++sl) {
-      const int64_t at = base + kg * SL + sl;
-      if (at >= hi) break;
+      const int at = base + kg * SL + sl;
+      if (at >= part.chunks) break;
       multiply<MT, 4, GS>(now[sl], [&](int mt, int i) { return *reinterpret_cast<const f16x8*>(x_at + stage * kStage + (sl * kRows + mt * 16) * kPitch + i * 64); },
-                          s_at + static_cast<int>(at - lo) * (8 / GS), acc);
+                          s_at + at * (8 / GS), acc);
     }
     if (more) {
       keep_x(stage ^ 1);
