@@ -637,8 +637,9 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid 
 // of V): K and V are read once for up to 16 RT W rows, and no sum crosses wavefronts.  A tile is two steps: V(t) turns its scores into weights
 // (vector instructions), M(t) multiplies them with its values and the next tile's keys with Q (the matrix cores).  With eight wavefronts the second four
 // run one step behind the first, so that each SIMD has one wavefront in either step; left to themselves the two do the same at the same
-// time (256 rows of 128 against 65533 keys, 8 key heads: 118 us, with the turns 101 .. 110).  Stages that the loads write themselves, four of each, were level
-// (103 us; 84 without any loads, 69 with nothing but them).
+// time (256 rows of 128 against 65533 keys, 8 key heads: 118 us, with the turns 101 .. 110).  Without any loads it takes 84 us, with
+// nothing but them 69.  Stages that the loads write themselves, four of each, are up to 5 % shorter; but the compiler has every transposing read wait for
+// such loads, so they would have to be outstanding behind its back.
 //   tile t's keys are read in M(t - 1), its values in M(t): steps 2 t - 1 and 2 t + 1 of the first four, one later of the others.  What a wavefront
 //   loaded of K it stores in V(t) for tile t + 1 (the others: t + 2), of V for tile t (t + 1): behind the last reads of the tile that had the
 //   stage before, and a barrier ahead of the first of its own.
