@@ -419,17 +419,25 @@ int launch_q4_few(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
   return launch_q4(gemv_q4_kernel<GS, W, D>, a, ep, 16, 4, 64 * W, 64, kNumCU, 2 * W, a.M * kChunk * 2 + 16 * (8 / GS), 16 * 16, 60 * 1024, s);
 }
 template <int MT, int GS, int CT, int KG, int SL>
-int launch_q4_many(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
+int launch_q4_many(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s, int least = KG * SL) {
   constexpr int kRows = 16 * MT, kCols = 16 * CT;
-  return launch_q4(gemv_q4_rows_kernel<MT, GS, CT, KG, SL>, a, ep, kCols, kRows, 64 * CT * KG, kRows * kCols, kNumCU, KG * SL, kCols * (8 / GS), kCols * 16, 20 * 1024, s);
+  return launch_q4(gemv_q4_rows_kernel<MT, GS, CT, KG, SL>, a, ep, kCols, kRows, 64 * CT * KG, kRows * kCols, kNumCU, least, kCols * (8 / GS), kCols * 16, 20 * 1024, s);
 }
 template <int GS>
 int launch_q4_rows(const Q4Args& a, const Q4Epilogue& ep, hipStream_t s) {
   // few columns: more wavefronts to each sixteen.  2560 x 10240 (160 workgroups) on 4 / 8 / 16 wavefronts 14.9 / 10.4 / 7.9 us, 7680 x 2560 (480) 7.2 / 6.2 / 6.3,
   // 50280 x 4096 (3143) 27.0 (28.8 when the others were measured) / 31.5 / 40.5; four chunks requested at once instead of two are level to 10 % longer
   if (a.M <= 4) return a.N <= 16 * 256 ? launch_q4_few<GS, 16, 2>(a, ep, s) : a.N <= 16 * 1024 ? launch_q4_few<GS, 8, 2>(a, ep, s) : launch_q4_few<GS, 4, 2>(a, ep, s);
+  // Where blocks of 32 columns fill one round of the CUs at most, and K is not long: those, with all of K, instead of 64 columns and parts of K that are handed
+  // over.  16 x 2560 x 2560 9.0 -> 6.4 us, 16 x 7680 x 2560 9.9 -> 7.1, 64 x 4096 x 4096 12.4 -> 10.5, 64 x 4096 x 6144 14.9 -> 13.6; 16 x 2560 x 10240 would
+  // take 12.6 instead of 10.9, 64 x 10240 x 2560 (two rounds) 21.6 instead of 16.6.
+  const int rows = a.M <= 16 ? 16 : 32;
+  if (ceil_div(a.N, 32) * ceil_div(a.M, rows) <= kNumCU && a.K <= 6144) {
+    constexpr int kWhole = 64;  // chunks: more than there are
+    return a.M <= 16 ? launch_q4_many<1, GS, 2, 8, 1>(a, ep, s, kWhole) : launch_q4_many<2, GS, 2, 8, 1>(a, ep, s, kWhole);
+  }
   if (a.M <= 16) return launch_q4_many<1, GS, 4, 4, 2>(a, ep, s);
-  // by 32 rows, W again for the next 32: 64 rows at once are behind but for the widest W (64 x 2560 x 10240 25.4 us against 18.3, 64 x 4096 x 4096 17.3 / 12.8,
+  // by 32 rows, W again for the next 32: 64 rows at once are behind but for the widest W (64 x 2560 x 10240 25.4 us against 18.3,
   // 64 x 10240 x 2560 23.0 / 17.8, 48 x 11008 x 4096 20.9 / 22.9).  Sixteen wavefronts where the columns are few, eight beyond (10240 x 2560 20.5 / 17.8, 2560 x 10240 18.3 / 20.3)
   return a.N <= 8192 ? launch_q4_many<2, GS, 4, 4, 1>(a, ep, s) : launch_q4_many<2, GS, 4, 2, 2>(a, ep, s);
 }

@@ -80,6 +80,12 @@ def test_sizes(M, N, K, group):
     check(M, N, K, group, 0)
 
 
+@pytest.mark.parametrize("epilogue", [0, 2, 3])
+@pytest.mark.parametrize("M,N,K,group", [(7, 8230, 320, 32), (16, 8193, 128, 128), (33, 4200, 192, 64), (64, 4130, 96, 32), (5, 8300, 1280, 128)])
+def test_more_columns_than_one_round_of_narrow_blocks(M, N, K, group, epilogue):
+    check(M, N, K, group, epilogue)
+
+
 def test_many_rows_of_a_long_k():
     # the parts of all rows together are more than the workspace is asked for at once: several launches
     M, N, K, group = 4100, 8192, 5120, 32
