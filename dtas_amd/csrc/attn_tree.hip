@@ -161,8 +161,15 @@ __device__ __forceinline__ void see(uint64_t (&sees)[RT], int up, int lane, int 
 }
 
 // ---- Which part of which sequence a workgroup has.  A sequence's units of keys (the blocks of its cache, those of the nodes behind) are cut into runs of
-// `per` units at most, the smallest `per` (and `least` at least) with which all sequences together make no more than `budget` parts, and a
-// sequence no more than `most`; its parts take consecutive slots.
+// `per` units at most, the smallest `per` with which all sequences together make no more than `budget` parts, and a sequence no more than
+// `most`; its parts take consecutive slots.  A part costs what its sums take to be written and read again, all workgroups together the more the more there are:
+// with a unit's time t, K parts of U units in all and w for the sums of a part of every problem it is t U / K + w K, least at
+// per = U / K = `spread` sqrt(U), spread = sqrt(w / t).  Where the longest sequence in one piece, t longest, takes no more than that and the hand-over (`whole` units
+// of time), nothing is cut.
+struct Cut {
+  int least, most, whole;
+  float spread;
+};
 struct Part {
   int b, z, parts, first;  // sequence, which of its parts, of how many, the sequence's first slot; b < 0: nothing to do
 };
@@ -200,7 +207,12 @@ struct Sequences {
       : lens(a.lens), batch(batch_), unit(unit_), T(a.T), capacity(a.capacity), units0(lane < batch_ ? units_of(a.lens[lane], a.capacity, unit_, a.T) : 0) {}
   __device__ __forceinline__ int units(int c, int lane) const { return c == 0 ? units0 : c + lane < batch ? units_of(lens[c + lane], capacity, unit, T) : 0; }
 };
-__device__ __forceinline__ int deal(const Sequences& s, int budget, int least, int most, int lane) {
+__device__ __forceinline__ int least_of(const Cut& cut, int total, int longest) {
+  const float run = cut.spread * __builtin_amdgcn_sqrtf(static_cast<float>(total));
+  if (static_cast<float>(longest) <= static_cast<float>(cut.whole) + 2.f * run) return longest;
+  return run > static_cast<float>(cut.least) ? static_cast<int>(run + 0.5f) : cut.least;
+}
+__device__ __forceinline__ int deal(const Sequences& s, int budget, const Cut& cut, int lane) {
   int total = 0, longest = 0;
   for (int c = 0; c < s.batch; c += 64) {
     const int units = s.units(c, lane);
@@ -209,8 +221,9 @@ __device__ __forceinline__ int deal(const Sequences& s, int budget, int least, i
     longest = longest > top ? longest : top;
   }
   int per = (total + budget - 1) / budget;
+  const int least = least_of(cut, total, longest);
   per = per > least ? per : least;
-  per = per > (longest + most - 1) / most ? per : (longest + most - 1) / most;
+  per = per > (longest + cut.most - 1) / cut.most ? per : (longest + cut.most - 1) / cut.most;
   for (;;) {  // (per grows until the parts fit; with per = longest every sequence is one part, and budget >= batch)
     int parts = 0;
     for (int c = 0; c < s.batch; c += 64) parts += wave_total((s.units(c, lane) + per - 1) / per);
@@ -219,17 +232,18 @@ __device__ __forceinline__ int deal(const Sequences& s, int budget, int least, i
     per = more > per ? more : per + 1;
   }
 }
-__device__ __forceinline__ Part find_part(const TreeArgs& a, int batch, int unit, int slot, int budget, int least, int most, int lane) {
+__device__ __forceinline__ Part find_part(const TreeArgs& a, int batch, int unit, int slot, int budget, const Cut& cut, int lane) {
   if (budget == 0) return Part{slot, 0, 1, slot};
   if (batch == 1) {
     const int units = units_of(a.lens[0], a.capacity, unit, a.T);
+    const int least = least_of(cut, units, units);
     int per = (units + budget - 1) / budget;
     per = per > least ? per : least;
     const int parts = (units + per - 1) / per;
     return Part{slot < parts ? 0 : -1, slot, parts, 0};
   }
   const Sequences s(a, batch, unit, lane);
-  const int per = deal(s, budget, least, most, lane);
+  const int per = deal(s, budget, cut, lane);
   int base = 0;
   for (int c = 0; c < batch; c += 64) {
     const int parts = (s.units(c, lane) + per - 1) / per;
@@ -429,6 +443,7 @@ __device__ __forceinline__ void join_parts(const TreeArgs& a, int b, int hk, int
 // What a launch is made of: workgroup u has slot u % slots of key head (u / slots) % kv_heads and rows from (u / slots / kv_heads) on.
 struct TreeGrid {
   int batch, slots, budget, row_groups;
+  Cut cut;
   float* ws;
   unsigned* arrivals;
   int* dealt;  // [batch][2], for the launch that joins many rows: a sequence's parts and its first slot
@@ -453,7 +468,7 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
   const int g = a.heads / a.kv_heads, R = a.Tq * g;
   const int slot = static_cast<int>(blockIdx.x % grid.slots), hk = static_cast<int>(blockIdx.x / grid.slots % a.kv_heads), rg = static_cast<int>(blockIdx.x / grid.slots / a.kv_heads);
-  const Part part = find_part(a, grid.batch, kBlock, slot, grid.budget, W, 64 / RT, lane);
+  const Part part = find_part(a, grid.batch, kBlock, slot, grid.budget, grid.cut, lane);
   if (part.b < 0) return;
   const int b = part.b;
   const int64_t len = clamp_len(a.lens[b], a.capacity);
@@ -654,7 +669,7 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
   const int g = a.heads / a.kv_heads, R = a.Tq * g;
   const int slot = static_cast<int>(blockIdx.x % grid.slots), hk = static_cast<int>(blockIdx.x / grid.slots % a.kv_heads), rg = static_cast<int>(blockIdx.x / grid.slots / a.kv_heads);
-  const Part part = find_part(a, grid.batch, kTile, slot, grid.budget, 2, 64, lane);
+  const Part part = find_part(a, grid.batch, kTile, slot, grid.budget, grid.cut, lane);
   if (part.b < 0) return;
   const int b = part.b;
   if (grid.budget > 0 && part.z == 0 && hk == 0 && rg == 0 && tid == 0) {
@@ -936,22 +951,27 @@ __global__ void __launch_bounds__(256) attn_tree_join_kernel(TreeArgs a, TreeGri
   if (lane < kLanes && c < a.d) store_row4(out_row(a, b, hk, g, r) + c, v, 1.f / total);
 }
 
-// The launch of a kernel for `rows` rows and `threads` threads per workgroup and parts of at least `least` units of `unit` keys, at most `most` of
-// a sequence: `fill` workgroups for the whole chip
+// The launch of a kernel for `rows` rows and `threads` threads per workgroup and units of `unit` keys, parts of them as `cut` says: one workgroup
+// per CU.  `handed`: what a part's sums cost, in units of time (0: those of few rows are little)
 struct TreeShape {
-  int rows, threads, unit, least, most, fill;
+  int rows, threads, unit;
+  Cut cut;
+  float handed;
 };
 template <typename Kernel>
 int launch_tree(Kernel kernel, const TreeArgs& a, int64_t batch, int DP, const TreeShape& shape, bool counts, hipStream_t s, TreeGrid* grid, std::unique_lock<std::recursive_mutex>* lock) {
   const int64_t groups = ceil_div(static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads), shape.rows), problems = a.kv_heads * groups;
-  int64_t budget = shape.fill / problems;
-  const int64_t useful = batch * ceil_div(ceil_div(a.capacity, shape.unit) + ceil_div(a.T, shape.unit), shape.least), limit = batch * shape.most;
+  int64_t budget = kNumCU / problems;
+  Cut cut = shape.cut;
+  cut.spread = sqrtf(shape.handed * static_cast<float>(problems));
+  if (shape.handed == 0.f && problems * batch < 16) cut.whole = 0;  // (few workgroups, each slower than its hand-over)
+  const int64_t units = ceil_div(a.capacity, shape.unit) + ceil_div(a.T, shape.unit), useful = static_cast<float>(units) <= static_cast<float>(cut.whole) + 2.f * cut.spread * sqrtf(static_cast<float>(units + batch - 1)) ? 0 : batch * ceil_div(units, cut.least), limit = batch * cut.most;
   budget = budget > useful ? useful : budget;
   budget = budget > limit ? limit : budget;
-  if (budget <= batch) budget = 0;  // every sequence in one piece
+  if (budget <= batch) budget = 0;  // every sequence in one piece (as it would be by least_of, whatever the lengths: a sequence has one unit at least)
   const int64_t slots = budget == 0 ? batch : budget;
   if (batch > INT32_MAX || problems * slots > INT32_MAX) return fail("attn_tree: the launch has too many workgroups");
-  *grid = TreeGrid{static_cast<int>(batch), static_cast<int>(slots), static_cast<int>(budget), static_cast<int>(groups), nullptr, nullptr, nullptr};
+  *grid = TreeGrid{static_cast<int>(batch), static_cast<int>(slots), static_cast<int>(budget), static_cast<int>(groups), cut, nullptr, nullptr, nullptr};
   const size_t sums = static_cast<size_t>(problems * slots) * shape.rows * (DP + 2);
   if (budget > 0 && split_scratch(s, (sums + 2 * static_cast<size_t>(batch)) * sizeof(float), counts ? static_cast<size_t>(problems * batch) : 1, static_cast<int>(budget), &grid->ws,
                                   &grid->arrivals, lock) != 0)
@@ -962,19 +982,24 @@ int launch_tree(Kernel kernel, const TreeArgs& a, int64_t batch, int DP, const T
 }
 template <int DP, int RT, int W>
 int launch_few(const TreeArgs& a, int64_t batch, hipStream_t s) {
+  // Parts of W / 2 blocks at least, W of 32 rows (1 node, 32 heads on 8, after 500 keys 9.1 -> 8.3 us; 26 rows after 1000 would take 13.7 instead of 12.9), and none
+  // where a wavefront has two or three blocks of the whole (16 nodes, 32 heads of 80, after 500 9.1 -> 7.5; 2 x 8 nodes, 32 heads on 8, after 600 15.6 -> 14.0).
   TreeGrid grid;
   std::unique_lock<std::recursive_mutex> lock;
-  return launch_tree(attn_tree_kernel<DP, RT, W>, a, batch, DP, TreeShape{16 * RT, 64 * W, 32, W, 64 / RT, kNumCU}, true, s, &grid, &lock);
+  return launch_tree(attn_tree_kernel<DP, RT, W>, a, batch, DP, TreeShape{16 * RT, 64 * W, 32, Cut{RT == 1 ? W / 2 : W, 64 / RT, 5 * W / 2, 0.f}, 0.f}, true, s, &grid, &lock);
 }
 template <int DP, int RT, int W>
 int launch_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   TreeGrid grid;
   std::unique_lock<std::recursive_mutex> lock;  // (held until the kernel that joins the parts is enqueued as well)
-  const TreeShape shape{16 * RT * W, 64 * W, 64, 2, 64, kNumCU};
+  // Times in us: a tile of 64 keys; the second launch and what it waits for, 4; a part's sums, written and read at 4 TB/s.  8 sequences of 128 rows, 8 key heads,
+  // after 250 keys 20.0 -> 17.5.
+  const int64_t all = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
+  const float tile = 0.6f + 16 * RT * W * DP / 16384.f, sums = static_cast<float>(all < 16 * RT * W ? all : 16 * RT * W) * (DP + 2) * 4;
+  const TreeShape shape{16 * RT * W, 64 * W, 64, Cut{2, 64, static_cast<int>(4.f / tile), 0.f}, 2.f * sums / (4e6f * tile)};
   if (launch_tree(attn_tree_rows_kernel<DP, RT, W>, a, batch, DP, shape, false, s, &grid, &lock) != 0) return -1;
   if (grid.budget == 0) return 0;
-  const int64_t rows = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
-  hipLaunchKernelGGL(attn_tree_join_kernel<DP>, dim3(static_cast<unsigned>(ceil_div(rows, 4)), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
+  hipLaunchKernelGGL(attn_tree_join_kernel<DP>, dim3(static_cast<unsigned>(ceil_div(all, 4)), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
                      dim3(256), 0, s, a, grid, shape.rows);
   return check_launch("attn_tree");
 }

@@ -124,6 +124,12 @@ def test_many_sequences(B, Hkv, group, T):
     check(make(B, T, T, Hkv, group, 64, [(37 * b * b) % 700 for b in range(B)], 700))
 
 
+@pytest.mark.parametrize("B,Hkv,group,T,lens", [(8, 8, 8, 16, [250, 3, 0, 249, 251, 17, 250, 192]), (6, 2, 7, 12, [0, 1, 63, 64, 65, 400]), (3, 4, 4, 64, [300, 90, 0]),
+                                                 (2, 8, 4, 8, [600, 20]), (2, 16, 1, 30, [607, 609]), (1, 16, 1, 5, [575]), (1, 16, 1, 5, [577])])
+def test_caches_around_what_is_worth_cutting(B, Hkv, group, T, lens):
+    check(make(B, T, T, Hkv, group, 64, lens, 640))
+
+
 def test_one_long_sequence_among_short_ones():
     for group, T in ((2, 1), (8, 7)):
         check(make(6, T, T, 1, group, 64, [3, 9001, 0, 40, 1, 700], 9001))
