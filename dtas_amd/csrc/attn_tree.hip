@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(64) attn_tree_scalar_kernel(TreeArgs a, int64_
 //                 the keys inside an MFMA is free, so P never moves.  A = V^T in the same order: 4 keys of one channel per
 //                 transposing LDS read, from V's rows (32 bytes longer than a row: eight rows fall on different banks).
 // P is rounded to fp16 for its product (half a step, 2^-11 of each weight); scores, maxima, sums and O stay in fp32.
-// Two kernels: up to 16 (32) rows the wavefronts of a workgroup share the keys and load K's operands straight from memory; with more rows
+// Two kernels: of few rows (`launch_tree_rows` says which) the wavefronts of a workgroup share the keys and load K's operands straight from memory; with more rows
 // they share the rows and every key passes through the LDS once.
 constexpr int v_row_bytes(int DP) { return 2 * DP + 32; }
 // A kernel for DP channels serves head dimensions above `below(DP)`: a lane whose channels lie behind the head's last reads that head's last
@@ -1007,8 +1007,12 @@ int launch_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
 template <int DP>
 int launch_tree_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
-  if (rows <= 16) return launch_few<DP, 1, (DP <= 128 ? 8 : 4)>(a, batch, s);
-  if (rows <= 32) return launch_few<DP, 2, (DP <= 128 ? 8 : 4)>(a, batch, s);
+  // Beyond 16 rows, or 8 of heads of more than 128, sharing the keys pays only where they are few: 32 rows of 64 heads on 8 after 300 keys 8.1 us, sharing the rows 10.3,
+  // 20 rows of 32 on 8 after 500 12.8 / 11.6, 32 rows after 1000 16.7 / 13.2, after 16000 29.5 / 20.2; 16 rows of 256 after 1569 19.2 / 15.5.  16 rows of 80
+  // after 3001 12.6 / 15.6, one row of 256 on 8 heads after 4000 16.5 / 21.6.
+  const bool few = a.capacity <= 384;
+  if (rows <= (DP <= 128 ? 16 : 8) || (rows <= 16 && few)) return launch_few<DP, 1, (DP <= 128 ? 8 : 4)>(a, batch, s);
+  if (rows <= 32 && few) return launch_few<DP, 2, (DP <= 128 ? 8 : 4)>(a, batch, s);
   if (rows <= 64) return launch_rows<DP, 1, 4>(a, batch, s);
   if (rows <= 128 || DP > 128) return launch_rows<DP, 1, 8>(a, batch, s);
   if constexpr (DP <= 128) return launch_rows<DP, 2, 8>(a, batch, s);

@@ -130,6 +130,14 @@ def test_caches_around_what_is_worth_cutting(B, Hkv, group, T, lens):
     check(make(B, T, T, Hkv, group, 64, lens, 640))
 
 
+@pytest.mark.parametrize("capacity", [380, 384, 385, 900])
+@pytest.mark.parametrize("d", [64, 80, 128, 192, 256])
+@pytest.mark.parametrize("Hkv,group,T", [(1, 2, 10), (2, 8, 4), (1, 3, 5), (1, 8, 1), (1, 9, 1)])
+def test_capacities_around_the_choice_of_kernel(Hkv, group, T, d, capacity):
+    check(make(2, T, T, Hkv, group, d, [capacity, capacity - 70], capacity))
+    check(make(1, T, T, Hkv, group, d, [capacity - 1], capacity))
+
+
 def test_one_long_sequence_among_short_ones():
     for group, T in ((2, 1), (8, 7)):
         check(make(6, T, T, 1, group, 64, [3, 9001, 0, 40, 1, 700], 9001))
