@@ -988,6 +988,18 @@ int launch_few(const TreeArgs& a, int64_t batch, hipStream_t s) {
   std::unique_lock<std::recursive_mutex> lock;
   return launch_tree(attn_tree_kernel<DP, RT, W>, a, batch, DP, TreeShape{16 * RT, 64 * W, 32, Cut{RT == 1 ? W / 2 : W, 64 / RT, 5 * W / 2, 0.f}, 0.f}, true, s, &grid, &lock);
 }
+// us that a workgroup of `rows` rows takes for a tile of 64 keys
+inline float tile_us(int rows, int DP) { return 0.6f + static_cast<float>(rows * DP) / 16384.f; }
+// us of all tiles with `rows` rows per workgroup and full caches: one piece per sequence, or one workgroup per CU, whose sums are handed over (see launch_rows)
+inline float blocks_us(const TreeArgs& a, int64_t batch, int rows, int DP) {
+  const int64_t all = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads), problems = a.kv_heads * ceil_div(all, rows);
+  const float units = static_cast<float>(ceil_div(a.capacity, 64) + 1), tile = tile_us(rows, DP), whole = static_cast<float>(batch * problems) / kNumCU;
+  const float uncut = (whole > 1.f ? whole : 1.f) * units * tile;
+  if (kNumCU / problems <= batch) return uncut;
+  const float share = units * whole > 2.f ? units * whole : 2.f, parts = static_cast<float>(batch * problems) * units / share;
+  const float cut = share * tile + 4.f + parts * static_cast<float>(all < rows ? all : rows) * (DP + 2) * 8 / 4e6f;
+  return cut < uncut ? cut : uncut;
+}
 template <int DP, int RT, int W>
 int launch_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   TreeGrid grid;
@@ -995,7 +1007,7 @@ int launch_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   // Times in us: a tile of 64 keys; the second launch and what it waits for, 4; a part's sums, written and read at 4 TB/s.  8 sequences of 128 rows, 8 key heads,
   // after 250 keys 20.0 -> 17.5.
   const int64_t all = static_cast<int64_t>(a.Tq) * (a.heads / a.kv_heads);
-  const float tile = 0.6f + 16 * RT * W * DP / 16384.f, sums = static_cast<float>(all < 16 * RT * W ? all : 16 * RT * W) * (DP + 2) * 4;
+  const float tile = tile_us(16 * RT * W, DP), sums = static_cast<float>(all < 16 * RT * W ? all : 16 * RT * W) * (DP + 2) * 4;
   const TreeShape shape{16 * RT * W, 64 * W, 64, Cut{2, 64, static_cast<int>(4.f / tile), 0.f}, 2.f * sums / (4e6f * tile)};
   if (launch_tree(attn_tree_rows_kernel<DP, RT, W>, a, batch, DP, shape, false, s, &grid, &lock) != 0) return -1;
   if (grid.budget == 0) return 0;
@@ -1013,9 +1025,15 @@ int launch_tree_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   const bool few = a.capacity <= 384;
   if (rows <= (DP <= 128 ? 16 : 8) || (rows <= 16 && few)) return launch_few<DP, 1, (DP <= 128 ? 8 : 4)>(a, batch, s);
   if (rows <= 32 && few) return launch_few<DP, 2, (DP <= 128 ? 8 : 4)>(a, batch, s);
+  // Blocks of 64, 128 or 256 rows: larger ones read K and V less often, smaller ones hand fewer sums over.  256 rows on 8 heads of 128 after 1000 / 4000 / 16000 / 65533
+  // keys: 15.0, 21.7, 48.3, 163 us in blocks of 64, 19.1, 23.2, 37.8, 118 of 128, 23.7, 27.8, 39.2, 102 of 256.
   if (rows <= 64) return launch_rows<DP, 1, 4>(a, batch, s);
-  if (rows <= 128 || DP > 128) return launch_rows<DP, 1, 8>(a, batch, s);
-  if constexpr (DP <= 128) return launch_rows<DP, 2, 8>(a, batch, s);
+  const float by64 = blocks_us(a, batch, 64, DP), by128 = blocks_us(a, batch, 128, DP);
+  if constexpr (DP <= 128) {
+    const float by256 = rows > 128 ? blocks_us(a, batch, 256, DP) : INFINITY;
+    if (by256 < by64 && by256 < by128) return launch_rows<DP, 2, 8>(a, batch, s);
+  }
+  return by64 < by128 ? launch_rows<DP, 1, 4>(a, batch, s) : launch_rows<DP, 1, 8>(a, batch, s);
 }
 
 }  // namespace

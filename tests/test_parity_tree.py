@@ -138,6 +138,33 @@ def test_capacities_around_the_choice_of_kernel(Hkv, group, T, d, capacity):
     check(make(1, T, T, Hkv, group, d, [capacity - 1], capacity))
 
 
+@pytest.mark.parametrize("Hkv,d,capacity,lens", [(32, 64, 4200, [4097]), (32, 64, 4200, [1]), (32, 72, 6600, [6533]), (32, 128, 9100, [9001]), (16, 64, 4200, [4200, 63]),
+                                                 (32, 64, 2000, [1999]), (8, 128, 4000, [3907]), (4, 256, 8000, [7001]), (4, 192, 4000, [4000]), (2, 80, 1000, [999, 0])])
+def test_blocks_of_all_sizes(Hkv, d, capacity, lens):
+    # 256 rows of each key head: in blocks of 64, 128 or 256
+    check(make(len(lens), 64, 64, Hkv, 4, d, lens, capacity))
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("Hkv,d,capacity", [(32, 64, 4200), (32, 64, 2000), (32, 128, 9100), (4, 256, 8000), (1, 64, 100)])
+def test_a_value_that_is_no_number_in_blocks_of_all_sizes(Hkv, d, capacity, value):
+    host = make(1, 64, 64, Hkv, 4, d, [97], capacity)
+    host["parents"][:] = -1  # every node sees the cache and itself
+    host["V"][0, 7] = 0
+    want, tolerance = expected(host)
+    host["V"][0, 7, :, 3] = value
+    got = launch(host).double()
+    others = [t for t in range(64) if t != 7]
+    assert bool(((got - want).abs() <= tolerance)[:, others].all())
+    assert not bool(torch.isfinite(got[0, 7, :, 3]).any()) and bool(torch.isfinite(got[0, 7, :, :3]).all()) and bool(torch.isfinite(got[0, 7, :, 4:]).all())
+
+
+@pytest.mark.parametrize("Hkv,d,capacity", [(32, 64, 4200), (16, 128, 3000), (2, 256, 6000), (1, 80, 500)])
+def test_blocks_that_are_not_full(Hkv, d, capacity):
+    check(make(1, 43, 43, Hkv, 5, d, [capacity - 3], capacity))
+    check(make(1, 64, 21, Hkv, 5, d, [capacity - 3], capacity))
+
+
 def test_one_long_sequence_among_short_ones():
     for group, T in ((2, 1), (8, 7)):
         check(make(6, T, T, 1, group, 64, [3, 9001, 0, 40, 1, 700], 9001))
