@@ -290,3 +290,56 @@ def test_two_streams_and_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_two_recorded_graphs_share_a_workspace():
+    # recorded on one stream, the second needing a larger workspace than the first; lengths change between the replays
+    g = torch.Generator(device="cuda").manual_seed(9)
+    half = lambda *s: torch.randn(*s, device="cuda", generator=g).half()
+    words = lambda N, K: torch.randint(-2 ** 31, 2 ** 31, (N, K // 8), device="cuda", generator=g, dtype=torch.int64).to(torch.int32)
+
+    def attention(B, T, heads, kv, d, capacity):
+        parents = torch.arange(-1, T - 1, device="cuda", dtype=torch.int32).expand(B, T).contiguous()
+        return [half(B, T, heads, d), half(B, T, kv, d), half(B, T, kv, d), half(B, kv, capacity, d), half(B, kv, capacity, d),
+                torch.zeros(B, device="cuda", dtype=torch.int32), parents]
+
+    small = [attention(2, 3, 4, 2, 64, 3000), attention(1, 48, 4, 1, 128, 2000)]
+    large = [attention(3, 64, 32, 8, 128, 6000), attention(2, 1, 16, 8, 256, 3000)]
+    x, Wq, scale = half(20, 10240), words(300, 10240), half(300, 320).abs() * 0.01
+    target = torch.softmax(half(3, 5, 9000).float(), -1)
+    verify = [target, torch.softmax(half(3, 5, 9000).float(), -1), torch.randint(0, 9000, (3, 5), device="cuda", generator=g, dtype=torch.int64).to(torch.int32),
+              torch.tensor([-1, 0, 0, 1, 1], device="cuda", dtype=torch.int32).expand(3, 5).contiguous(), torch.rand(3, 5, device="cuda", generator=g),
+              torch.rand(3, device="cuda", generator=g)]
+
+    def outputs(sets):
+        return [torch.zeros_like(s[0]) for s in sets] + [torch.zeros(20, 300, device="cuda", dtype=torch.float16)] + \
+               [torch.zeros(3, 5, device="cuda", dtype=torch.int32), torch.zeros(3, device="cuda", dtype=torch.int32), torch.zeros(3, device="cuda", dtype=torch.int32)]
+
+    def run(sets, out):
+        for s, o in zip(sets, out):
+            ops.attn_tree(*s, o)
+        ops.gemv_q4(x, Wq, scale, None, out[2])
+        ops.verify_tree(*verify, *out[3:])
+
+    stream, graphs = torch.cuda.Stream(), []
+    for sets in (small, large):
+        played = outputs(sets)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run(sets, played)
+        graphs.append((graph, sets, played))
+    for replay in range(8):
+        graph, sets, played = graphs[replay % 2]
+        for s in sets:
+            s[5].copy_(torch.tensor([(replay * 977 + b * 1403) % (s[3].shape[2] + 1) for b in range(s[0].shape[0])]))
+        for t in played:
+            t.zero_()
+        eager = outputs(sets)
+        run(sets, eager)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        torch.cuda.synchronize()
+        for one, other in zip(played, eager):
+            assert torch.equal(one, other), replay
