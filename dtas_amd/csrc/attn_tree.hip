@@ -259,7 +259,8 @@ __device__ __forceinline__ Part find_part(const TreeArgs& a, int batch, int unit
   return Part{-1, 0, 0, 0};
 }
 
-// Where a unit of keys lies: in the cache, or among the nodes' own.  Rows behind the last valid key repeat that one.
+// Where a unit of keys lies: in the cache, or among the nodes' own.  Rows behind the last valid key are read as that one again: hidden, and their values
+// cleared where the weight zero is multiplied with them (a node's own: where one is no number, see no_number).
 struct Keys {
   const char *k, *v;
   unsigned stride;  // bytes between keys (a unit's rows lie within 4 GiB)
@@ -549,6 +550,11 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid 
       for (int n = 0; n < VL; ++n) odd = odd || no_number(vf[n]);
       odd = __builtin_amdgcn_ballot_w64(odd) != 0;
     }
+    if (!TREE && valid < kBlock) {  // (the weight of what lies behind the last key is zero, its value has to be as well: that key's own may be no number)
+#pragma unroll
+      for (int n = 0; n < VL; ++n)
+        if ((n * 64 + lane) / kChunks >= valid) vf[n] = u32x4{0u, 0u, 0u, 0u};
+    }
     if (!odd) {
 #pragma unroll
       for (int n = 0; n < VL; ++n) {
@@ -717,6 +723,13 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
   };
   auto keep_k = [&](int at) { keep(lds_k + (at & 1) * kK, k_row_bytes(DP), kf); };
   auto keep_v = [&](int at) {
+    if (at < cached && static_cast<int64_t>(at + 1) * kTile > len) {  // (the weight of what lies behind the last key is zero, its value has to be as well)
+      int valid = static_cast<int>(len - static_cast<int64_t>(at) * kTile);
+      asm("" : "+s"(valid));  // (compared here, not once ahead of the loop)
+#pragma unroll
+      for (int n = 0; n < kPieces; ++n)
+        if ((n * 64 * W + tid) / kChunks >= valid) vf[n] = u32x4{0u, 0u, 0u, 0u};
+    }
     keep(lds_v + (at & 1) * kV, v_row_bytes(DP), vf);
     if (at >= cached) {
       bool odd = false;

@@ -1,0 +1,38 @@
+"""Attention of a tree: keys and values that are no numbers, weights and scales at the ends of their range, in every kernel."""
+import math
+
+import pytest
+import torch
+
+from test_parity_tree import expected, launch, make
+
+pytestmark = pytest.mark.gpu
+
+# (nodes, key heads, query heads to each, d, capacity, elements off an aligned address): a wavefront's rows share the keys (16 rows, 32 rows, heads of 256), the
+# rows share the keys by 64, 128 and 256 (heads of 256 among them), element by element (an odd address, an odd head)
+FORMS = [(1, 2, 1, 64, 2300, 0), (4, 2, 2, 80, 2300, 0), (16, 3, 1, 128, 300, 0), (16, 1, 2, 64, 300, 0), (8, 2, 4, 128, 300, 0), (4, 1, 2, 256, 2300, 0), (9, 1, 3, 256, 300, 0),
+         (13, 2, 4, 96, 2300, 0), (64, 32, 4, 64, 2000, 0), (64, 32, 4, 64, 4200, 0), (64, 32, 4, 128, 9100, 0), (64, 4, 4, 256, 8000, 0), (40, 1, 1, 192, 2300, 0),
+         (4, 2, 2, 64, 300, 1), (3, 2, 2, 20, 300, 0)]
+
+
+def first_head(host, group):
+    """The inputs of the first key head and its rows alone."""
+    cut = {"Q": lambda t: t[:, :, :group], "K": lambda t: t[:, :, :1], "V": lambda t: t[:, :, :1], "Kc": lambda t: t[:, :1], "Vc": lambda t: t[:, :1]}
+    return {name: cut.get(name, lambda t: t)(t) for name, t in host.items()}
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("T,Hkv,group,d,capacity,offset,length",
+                         [(*form, length) for form in FORMS for length in ((1, 31, 32, 33, 63, 64, 65, 97, 259) if form[1] < 32 else (31, 64, 97))])
+def test_the_last_value_of_the_cache_is_no_number(T, Hkv, group, d, capacity, offset, length, value):
+    # it reaches the channel it stands in, of the rows of its key head, wherever the cache's last block ends
+    host = make(1, T, T, Hkv, group, d, [length], capacity)
+    host["Vc"][0, 0, length - 1, 3] = 0
+    want, tolerance = expected(first_head(host, group))
+    host["Vc"][0, 0, length - 1, 3] = value
+    got = launch(host, offset=offset).double()
+    assert bool(torch.isfinite(got[:, :, group:]).all())
+    mine = got[:, :, :group]
+    assert bool((torch.isnan(mine[..., 3]) if math.isnan(value) else mine[..., 3] == value).all())
+    others = [c for c in range(d) if c != 3]
+    assert bool(((mine - want).abs() <= tolerance)[..., others].all())
