@@ -44,9 +44,9 @@ __global__ void __launch_bounds__(64) attn_tree_scalar_kernel(TreeArgs a, int64_
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (lane + 64 * i < a.d) s = fmaf(qv[i], static_cast<float>(k[lane + 64 * i]), s);
-      s = wave_sum(s) * static_cast<float>(a.sign) * a.scale_log2;
+      s = wave_sum(s) * static_cast<float>(a.sign);  // (the maximum is that of the products: their differences are scaled, no product overflows by the scale)
       const float next = fmaxf(top, s);
-      const float keep = next == -INFINITY ? 1.f : exp2f(top - next), p = next == -INFINITY ? 0.f : exp2f(s - next);
+      const float keep = next == -INFINITY ? 1.f : exp2f((top - next) * a.scale_log2), p = next == -INFINITY ? 0.f : exp2f((s - next) * a.scale_log2);
       top = next;
       sum = fmaf(sum, keep, p);
 #pragma unroll
@@ -321,7 +321,17 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[NK], bool all, uint64_t shown, 
       for (int j = 0; j < 4; ++j) o[dt][j] *= keep;
     top = best;
   }
-  const float from = top == -INFINITY ? 0.f : -top * scale_log2;
+  // (s - top) scale as one multiply-add, s scale - top scale, which is off by the rounding of top scale, up to 2^-17 (weights that much of themselves) while that
+  // is 256 at most.  Where a row is beyond, that would be more than the products' own rounding, and overflow in the end: the difference is taken first.
+  const float base = top == -INFINITY ? 0.f : top;
+  float from = -base * scale_log2;
+  if (__builtin_amdgcn_ballot_w64(!(fabsf(from) <= 256.f)) != 0) {
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[kt][j] -= base;
+    from = 0.f;
+  }
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll

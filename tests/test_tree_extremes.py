@@ -36,3 +36,20 @@ def test_the_last_value_of_the_cache_is_no_number(T, Hkv, group, d, capacity, of
     assert bool((torch.isnan(mine[..., 3]) if math.isnan(value) else mine[..., 3] == value).all())
     others = [c for c in range(d) if c != 3]
     assert bool(((mine - want).abs() <= tolerance)[..., others].all())
+
+
+@pytest.mark.parametrize("scale", [2e26, 2.5e26, 1e38, -1e38, 2e38])
+@pytest.mark.parametrize("T,Hkv,group,d,capacity,offset", FORMS)
+def test_scales_up_to_the_largest(T, Hkv, group, d, capacity, offset, scale):
+    # products that are whole numbers: the keys with the row's largest (smallest, by a negative scale) share it, whatever the largest is
+    host = make(1, T, T, Hkv, group, d, [259], capacity, "chain")
+    g = torch.Generator().manual_seed(d)
+    for name in ("Q", "K", "Kc"):
+        host[name] = torch.randint(-3, 4, host[name].shape, generator=g).half()
+    host["Q"][..., 0], host["Kc"][..., 0], host["K"][..., 0] = 64, 64, 64  # (no product is near nought)
+    one = first_head(host, group)
+    want, _ = expected(one, scale)
+    got = launch(host, scale, offset).double()
+    # n equal weights of one key each: fp32 sums of up to 259 + 64 values (2^-24 each), a quotient and half a step
+    tolerance = 2.0 ** -10 * one["V"].double().abs().amax().clamp(min=float(one["Vc"].abs().max()))
+    assert bool(((got[:, :, :group] - want).abs() <= tolerance).all()), (got[0, 0, 0, :4], want[0, 0, 0, :4])
