@@ -75,7 +75,9 @@ __global__ void __launch_bounds__(64) attn_tree_scalar_kernel(TreeArgs a, int64_
 //   O^T = V^T P^T B = P^T as the scores' lanes hold it, its 8 keys per lane being 4 (l >> 4) .. + 3 of two key tiles: the order of
 //                 the keys inside an MFMA is free, so P never moves.  A = V^T in the same order: 4 keys of one channel per
 //                 transposing LDS read, from V's rows (32 bytes longer than a row: eight rows fall on different banks).
-// P is rounded to fp16 for its product (half a step, 2^-11 of each weight); scores, maxima, sums and O stay in fp32.
+// P is rounded to fp16 for its product, the type that the matrix cores take at this rate (in two halves, its products would take twice the MFMAs): 2^-11 of a weight down to
+// 2^-25 of the largest, 2^-36 of that below (see kRoom).  On random inputs results are 2.5 .. 2.9e-4 off the exact ones (root mean square, relative) where rounding to fp16 at the end
+// alone makes 2.1e-4.  Scores, maxima, sums and O stay in fp32.
 // Two kernels: of few rows (`launch_tree_rows` says which) the wavefronts of a workgroup share the keys and load K's operands straight from memory; with more rows
 // they share the rows and every key passes through the LDS once.
 constexpr int v_row_bytes(int DP) { return 2 * DP + 32; }
@@ -292,6 +294,13 @@ __device__ __forceinline__ f16x8 load_query(const half_t* row, int ks, int quart
   return load_channels<DP>(reinterpret_cast<const char*>(row), ks, quarter, d) * sign;
 }
 
+// P in fp16: a weight is 2^kRoom at the running maximum and 2^(kRoom + kAhead) = 2^15 at most.  The type's whole steps reach down to 2^-14, which is 2^-25 of the
+// maximum's weight (17.3 below it in the score): down to there a weight is off by half a step, 2^-11 of itself, below by 2^-36 of the maximum's, and what is less than
+// that is lost to the product with the values (not to the sum of the weights, in fp32): 2^-20 of the largest value at most after 65536 keys.  The maximum itself moves only when a
+// row's largest score leaves it behind by more than 2^kAhead: O is rescaled in few tiles instead of in most.  64 nodes after 65533 keys: 2^8 and 2^7 104 .. 107 us, 2^4 and
+// 2^11 level, 2^2 and 2^13 111.
+constexpr float kAhead = 4.f, kRoom = 11.f;
+
 // A weight per key from the products of one row tile, NK key tiles: mask, running maximum and sum, O rescaled where the maximum moved.
 // `shown` says which of the keys 16 kt + 4 (lane >> 4) + j the row sees (bit 16 kt + ..), all: none is hidden.
 template <int NK, int DT>
@@ -308,9 +317,6 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[NK], bool all, uint64_t shown, 
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) best = fmaxf(best, s[kt][j]);
-  // The sums are kept relative to a maximum that moves only when a row's largest score leaves it behind by more than 2^8: weights of up to 256 fit fp16 as
-  // well as those up to 1 (and the sums fp32), and O is rescaled in few tiles instead of in most.
-  constexpr float kAhead = 8.f;
   best = fmaxf(max_of_row(best), top);
   if (__builtin_amdgcn_ballot_w64((best - top) * scale_log2 > kAhead) != 0) {
     const float keep = best == -INFINITY ? 1.f : exp2_fast((top - best) * scale_log2);
@@ -324,13 +330,13 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[NK], bool all, uint64_t shown, 
   // (s - top) scale as one multiply-add, s scale - top scale, which is off by the rounding of top scale, up to 2^-17 (weights that much of themselves) while that
   // is 256 at most.  Where a row is beyond, that would be more than the products' own rounding, and overflow in the end: the difference is taken first.
   const float base = top == -INFINITY ? 0.f : top;
-  float from = -base * scale_log2;
+  float from = fmaf(-base, scale_log2, kRoom);
   if (__builtin_amdgcn_ballot_w64(!(fabsf(from) <= 256.f)) != 0) {
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[kt][j] -= base;
-    from = 0.f;
+    from = kRoom;
   }
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)

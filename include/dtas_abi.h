@@ -440,7 +440,7 @@ int dtas_gemv_q4_f16(const void* x, const void* Wq, const void* scale, const voi
  * [batch, kv_heads, capacity, d], all fp16; lens[batch] (clipped to [0, capacity]), parents[batch, nodes].  heads is a multiple of
  * kv_heads; query head h reads key head h / (heads / kv_heads).  d up to 256; multiples of 8 on 16-byte boundaries run on the matrix
  * cores, others element by element.  fp32 scores, statistics and sums; on the matrix cores a weight is rounded to fp16 for its product with the
- * values.  scale is a finite number up to 2e38 either way. */
+ * values (2^-11 of itself, and 2^-36 of the row's largest weight where that is more).  scale is a finite number up to 2e38 either way. */
 int dtas_attn_tree_f16(const void* Q, const void* K, const void* V, const void* K_cache, const void* V_cache, const void* lens,
                        const void* parents, void* out, int64_t batch, int64_t nodes, int64_t rows, int64_t heads, int64_t kv_heads,
                        int64_t d, int64_t capacity, float scale, void* stream);

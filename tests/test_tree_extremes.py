@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from dtas_amd import ops
 from test_parity_tree import expected, launch, make
 
 pytestmark = pytest.mark.gpu
@@ -36,6 +37,34 @@ def test_the_last_value_of_the_cache_is_no_number(T, Hkv, group, d, capacity, of
     assert bool((torch.isnan(mine[..., 3]) if math.isnan(value) else mine[..., 3] == value).all())
     others = [c for c in range(d) if c != 3]
     assert bool(((mine - want).abs() <= tolerance)[..., others].all())
+
+
+@pytest.mark.parametrize("gap", [9.0, 13.875, 15.0, 16.5])
+@pytest.mark.parametrize("T,Hkv,group,d", [(1, 32, 4, 64), (4, 32, 4, 128), (2, 32, 4, 256), (7, 32, 8, 64), (32, 32, 4, 64), (64, 32, 4, 64), (64, 32, 4, 128), (20, 32, 4, 256), (8, 32, 4, 80)])
+def test_a_long_flat_tail_behind_few_large_weights(T, Hkv, group, d, gap):
+    """Eight keys of no value whose scores lead those of all others by `gap`: what is left are the others' values, weighted by exp(-gap) each.
+
+    The others' weights are one number, off by half a step of fp16 (2^-11) and a rounding of its exponent (gap log2(e) 2^-23, exp2 of which is within 2^-22 besides),
+    and the products with values that are powers of two and their sums are exact (11 bits, less than 2^13 of them).  The sum of the weights has n additions in
+    fp32 at most, 2^-24 each, and as many again over wavefronts and parts.  Storing: 2^-11 of values above 2^-14."""
+    B, n = 10, 3999  # (more sequences than parts: each in one piece)
+    Q = torch.zeros(B, T, Hkv * group, d, device="cuda", dtype=torch.float16)
+    K, V = (torch.zeros(B, T, Hkv, d, device="cuda", dtype=torch.float16) for _ in range(2))
+    Kc, Vc = (torch.zeros(B, Hkv, n, d, device="cuda", dtype=torch.float16) for _ in range(2))
+    Q[..., 0] = 1
+    Kc[:, :, 0:256:32, 0] = gap
+    power = torch.exp2(torch.arange(d, device="cuda") % 3 + 6).half()
+    Vc[:], V[:] = power, power
+    Vc[:, :, 0:256:32] = 0
+    parents = torch.arange(-1, T - 1, device="cuda", dtype=torch.int32).expand(B, T).contiguous()
+    lens = torch.full((B,), n, device="cuda", dtype=torch.int32)
+    out = torch.empty_like(Q)
+    ops.attn_tree(Q, K, V, Kc, Vc, lens, parents, out, 1.0)
+    tail = (n - 8 + 1 + torch.arange(T, device="cuda").double()) * math.exp(-gap)  # (a node sees the nodes before it and itself)
+    want = (tail / (tail + 8))[None, :, None, None] * power.double()
+    assert float(want.min()) > 2.0 ** -14
+    tolerance = 2.0 ** -11 + gap * 1.45 * 2.0 ** -23 + 2.0 ** -22 + 2 * (n + T) * 2.0 ** -24 + 2.0 ** -11
+    assert float(((out.double() - want).abs() / want).max()) <= tolerance
 
 
 @pytest.mark.parametrize("scale", [2e26, 2.5e26, 1e38, -1e38, 2e38])
