@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(64) attn_tree_scalar_kernel(TreeArgs a, int64_
         if (lane + 64 * i < a.d) s = fmaf(qv[i], static_cast<float>(k[lane + 64 * i]), s);
       s = wave_sum(s) * static_cast<float>(a.sign);  // (the maximum is that of the products: their differences are scaled, no product overflows by the scale)
       const float next = fmaxf(top, s);
-      const float keep = next == -INFINITY ? 1.f : exp2f((top - next) * a.scale_log2), p = next == -INFINITY ? 0.f : exp2f((s - next) * a.scale_log2);
+      const float keep = next == -INFINITY ? 1.f : exp2f((top - next) * a.scale_log2), p = s == -INFINITY ? 0.f : exp2f((s - next) * a.scale_log2);  // (a score that is no number has no weight that is one)
       top = next;
       sum = fmaf(sum, keep, p);
 #pragma unroll

@@ -67,6 +67,35 @@ def test_a_long_flat_tail_behind_few_large_weights(T, Hkv, group, d, gap):
     assert float(((out.double() - want).abs() / want).max()) <= tolerance
 
 
+@pytest.mark.parametrize("at", [0, 5, 255, 258, "node"])
+@pytest.mark.parametrize("T,Hkv,group,d,capacity,offset", FORMS)
+def test_a_key_that_is_no_number_wherever_it_stands(T, Hkv, group, d, capacity, offset, at):
+    # also where everything in front of it has the score -inf, or nothing is in front of it: the rows that see it have no answer
+    length = 0 if at == "node" else 259
+    host = make(1, T, T, Hkv, group, d, [length], capacity, "chain")
+    host["Q"][..., 0] = 1
+    if at == "node":
+        host["K"][0, 0, 0, 0] = float("nan")
+    else:
+        host["Kc"][0, 0, :at, 0] = float("-inf")
+        host["Kc"][0, 0, at, 0] = float("nan")
+    got = launch(host, offset=offset)
+    assert bool(torch.isnan(got[:, :, :group]).all())
+    assert bool(torch.isfinite(got[:, :, group:]).all())
+
+
+@pytest.mark.parametrize("T,Hkv,group,d,capacity,offset", FORMS)
+def test_scores_of_minus_infinity_have_no_weight(T, Hkv, group, d, capacity, offset):
+    host = make(1, T, T, Hkv, group, d, [259], capacity, "chain")
+    host["Q"][..., 0] = 1
+    host["Kc"][0, 0, :, 0] = float("-inf")  # (the cache of the first key head: its rows see the nodes alone)
+    one = first_head(host, group)
+    want, tolerance = expected(dict(one, lens=torch.zeros(1, dtype=torch.int32)))
+    got = launch(host, offset=offset).double()
+    assert bool(((got[:, :, :group] - want).abs() <= tolerance).all())
+    assert bool(torch.isfinite(got[:, :, group:]).all())
+
+
 @pytest.mark.parametrize("scale", [2e26, 2.5e26, 1e38, -1e38, 2e38])
 @pytest.mark.parametrize("T,Hkv,group,d,capacity,offset", FORMS)
 def test_scales_up_to_the_largest(T, Hkv, group, d, capacity, offset, scale):
