@@ -385,6 +385,73 @@ __device__ __forceinline__ void add_key_by_key(const TreeArgs& a, int b, int hk,
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
+// A value may be infinite where its weight is too small for fp16 (below 2^-36 of the largest): zero times infinity, though the weight is a number in fp32 and the channel
+// infinite.  Such a channel shows in O, as NaN where the sum of the weights is a number (rare).  What it is instead depends on the keys alone whose values are no
+// numbers: they are looked for in the units first, first + step .. that the wavefront had, and summed with their weights in fp32.  The four lanes of a row hold a quarter of
+// its channels each.  (16 rows of 32 heads of 80 with such a key of 3001: 12 -> 16 us, 64 nodes after 65533 104 -> 370.)
+template <int DP, int UNIT, int DT>
+__device__ __forceinline__ void sum_again(const TreeArgs& a, int b, int hk, int64_t len, int cached, int first, int end, int step, int r, uint64_t sees, float top, float sum,
+                                          int lane, f32x4 (&o)[DT]) {
+  constexpr int KS = DP / 32;
+  f32x4 all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (dt * 16 + 16 <= below(DP) || dt * 16 + 4 * (lane >> 4) < a.d) all[j] += o[dt][j];
+  const float any = (all[0] + all[1]) + (all[2] + all[3]);
+  const bool mine = any != any && sum == sum;
+  if (__builtin_amdgcn_ballot_w64(mine) == 0) return;
+  asm volatile("" : "+v"(lane), "+v"(r));  // (nothing of what follows is computed ahead)
+  const int quarter = lane >> 4, g = a.heads / a.kv_heads, R = a.Tq * g, have = r < R ? r : R - 1;
+  const half_t* row = a.Q + ((static_cast<int64_t>(b) * a.Tq + have / g) * a.heads + hk * g + have % g) * a.d;
+  f16x8 q[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) q[ks] = load_query<DP>(row, ks, quarter, a.d, a.sign);
+  f32x4 fresh[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) fresh[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bool open = mine;  // (a lane whose channels have all become NaN has its answer)
+  for (int at = first; at < end && __builtin_amdgcn_ballot_w64(open) != 0; at += step) {
+    const Keys s = keys_of<UNIT>(a, b, hk, len, cached, at);
+    bool odd = false;
+    if (lane < UNIT && lane < s.valid)
+      for (int c = 0; c < a.d; c += 8) odd = odd || no_number(*reinterpret_cast<const u32x4*>(s.v + static_cast<unsigned>(lane) * s.stride + 2 * c));
+    for (uint64_t keys = __builtin_amdgcn_ballot_w64(odd); keys != 0 && __builtin_amdgcn_ballot_w64(open) != 0; keys &= keys - 1) {
+      const int key = __builtin_ctzll(keys);
+      float t = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const f16x8 k = load_channels<DP>(s.k + static_cast<unsigned>(key) * s.stride, ks, quarter, a.d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = fmaf(static_cast<float>(k[e]), static_cast<float>(q[ks][e]), t);
+      }
+      t = sum_of_row(t);
+      const float weight = t == -INFINITY ? 0.f : exp2_fast(fmaf(t - top, a.scale_log2, kRoom));
+      const bool shown = at < cached || ((sees >> ((at - cached) * UNIT + key)) & 1);
+      const half_t* v = reinterpret_cast<const half_t*>(s.v + static_cast<unsigned>(key) * s.stride);
+      float most = __builtin_nanf("");
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        if (dt * 16 + 16 <= below(DP) || dt * 16 + 4 * quarter < a.d) {
+          const f16x4 some = *reinterpret_cast<const f16x4*>(v + dt * 16 + 4 * quarter);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            fresh[dt][j] = shown ? fmaf(weight, static_cast<float>(some[j]), fresh[dt][j]) : fresh[dt][j];
+            most = fmaxf(most, fresh[dt][j]);
+          }
+        }
+      open = mine && most == most;
+    }
+  }
+  if (mine) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[dt][j] = o[dt][j] != o[dt][j] ? fresh[dt][j] : o[dt][j];
+  }
+}
+
 __device__ __forceinline__ half_t* out_row(const TreeArgs& a, int b, int hk, int g, int r) {
   return a.out + ((static_cast<int64_t>(b) * a.Tq + r / g) * a.heads + hk * g + r % g) * a.d;
 }
@@ -615,6 +682,7 @@ __global__ void __launch_bounds__(64 * W) attn_tree_kernel(TreeArgs a, TreeGrid 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     sum[rt] = sum_of_row(sum[rt]);
+    sum_again<DP, kBlock>(a, b, hk, len, cached, first + wave, end, W, rg * kRows + rt * 16 + i16, sees[rt], top[rt], sum[rt], lane, o[rt]);
     if (quarter == 0) {
       stat_m[wave][rt * 16 + i16] = top[rt];
       stat_l[wave][rt * 16 + i16] = sum[rt];
@@ -915,6 +983,7 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : W / 4) attn_tree_rows_
   for (int rt = 0; rt < RT; ++rt) {
     const int r = wave * 16 * RT + rt * 16 + i16;
     sum[rt] = sum_of_row(sum[rt]);
+    sum_again<DP, kTile>(a, b, hk, len, cached, first, end, 1, rg * kRows + r, sees[rt], top[rt], sum[rt], lane, o[rt]);
     if (r >= my_rows) continue;
     const float inv = 1.f / sum[rt];
     half_t* row = out_row(a, b, hk, g, rg * kRows + r);

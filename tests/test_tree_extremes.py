@@ -111,3 +111,24 @@ def test_scales_up_to_the_largest(T, Hkv, group, d, capacity, offset, scale):
     # n equal weights of one key each: fp32 sums of up to 259 + 64 values (2^-24 each), a quotient and half a step
     tolerance = 2.0 ** -10 * one["V"].double().abs().amax().clamp(min=float(one["Vc"].abs().max()))
     assert bool(((got[:, :, :group] - want).abs() <= tolerance).all()), (got[0, 0, 0, :4], want[0, 0, 0, :4])
+
+
+@pytest.mark.parametrize("gap", [10.0, 20.0, 30.0, 60.0])
+@pytest.mark.parametrize("at", [0, 40, 255, 258])
+@pytest.mark.parametrize("T,Hkv,group,d,capacity,offset", FORMS)
+def test_an_infinite_value_of_little_weight(T, Hkv, group, d, capacity, offset, at, gap):
+    # exp(-60) is a number in fp32 still: the channel is infinite, every other one as it would be
+    length = 259
+    host = make(1, T, T, Hkv, group, d, [length], capacity)
+    for name in ("Q", "K", "Kc"):
+        host[name][:] = 0
+    host["Q"][..., 0], host["Kc"][0, :, at, 0] = 1, -gap
+    host["Vc"][0, 0, at, 3] = 0
+    one = first_head(host, group)
+    want, tolerance = expected(one, 1.0)
+    host["Vc"][0, 0, at, 3] = float("inf")
+    got = launch(host, 1.0, offset).double()
+    mine, others = got[:, :, :group], [c for c in range(d) if c != 3]
+    assert bool((mine[..., 3] == float("inf")).all())
+    assert bool(((mine - want).abs() <= tolerance)[..., others].all())
+    assert bool(torch.isfinite(got[:, :, group:]).all())
