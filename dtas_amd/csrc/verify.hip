@@ -296,7 +296,8 @@ extern "C" int dtas_verify_tree_f32(const void* target, const void* draft, const
   if (nodes > DTAS_MAX_TREE_NODES) return fail("verify_tree: a tree holds up to %d nodes, got %lld", DTAS_MAX_TREE_NODES, (long long)nodes);
   if (batch == 0) return 0;
   if (nodes == 0 || V == 0) return fail("verify_tree: no node, or no token, to choose from");
-  if (V > INT32_MAX || batch > INT32_MAX) return fail("verify_tree: the extents overflow");
+  constexpr int64_t kMost = int64_t{1} << 60;
+  if (V > INT32_MAX || batch > INT32_MAX || V > kMost / nodes / batch) return fail("verify_tree: the extents overflow");
   if (!target || !draft || !tokens || !parents || !accept || !sample || !path || !count || !next) return fail("verify_tree: NULL buffer");
   const int64_t all = batch * nodes;
   struct Span { const void* at; int64_t bytes; };

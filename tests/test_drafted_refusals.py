@@ -100,3 +100,10 @@ def test_the_limit_is_the_headers():
     import re
     header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "dtas_abi.h")).read()
     assert int(re.search(r"#define DTAS_MAX_TREE_NODES (\d+)", header).group(1)) == _lib.MAX_TREE_NODES
+
+
+@pytest.mark.parametrize("extents", [dict(batch=(1 << 31) - 1, nodes=64, V=(1 << 31) - 1), dict(batch=1 << 25, nodes=64, V=1 << 30), dict(batch=(1 << 31) - 1, nodes=1, V=(1 << 31) - 1)])
+def test_verify_tree_refuses_rows_beyond_64_bits(extents):
+    # each extent is within its own range, the distributions' bytes are not
+    rc, message = verify(**extents)
+    assert rc == -1 and "verify_tree: the extents overflow" in message
