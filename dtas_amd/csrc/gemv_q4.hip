@@ -110,7 +110,7 @@ __device__ __forceinline__ u32x4 load_w(const unsigned char* row, int chunk, int
   return *reinterpret_cast<const u32x4*>(row + (chunk * (kChunk / 2) + (quarter < left ? quarter : left - 1) * 16));
 }
 // Scales of `cols` rows from n0 on, of one part of K, into the LDS: a row is an odd number of 8-byte pieces (sixteen rows fall on different banks).
-// What lies behind the row's last scale is that one again (it meets sums of zero).
+// What lies behind the row's last scale is zero (it meets sums of zero, and the last scale itself may be no number).
 template <int GS>
 __host__ __device__ constexpr int scale_pitch(int64_t chunks) {
   return static_cast<int>((chunks * (4 / GS) + 3) / 4) | 1;
@@ -129,7 +129,7 @@ __device__ __forceinline__ void stage_scales(char* lds, const Q4Args& a, int64_t
       __builtin_memcpy(&v, from + g, 8);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = from[g + i < groups ? g + i : groups - 1];
+      for (int i = 0; i < 4; ++i) v[i] = g + i < groups ? from[g + i] : half_t{0};
     }
     *reinterpret_cast<f16x4*>(lds + (r * pitch + c) * 8) = v;
   }
