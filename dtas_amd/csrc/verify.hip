@@ -344,9 +344,9 @@ extern "C" int dtas_cache_append_f16(const void* K, const void* V, const void* p
   if (layers < 0 || batch < 0 || nodes < 0 || slots < 0 || kv_heads < 0 || d < 0 || capacity < 0)
     return fail("cache_append: negative extent layers=%lld batch=%lld nodes=%lld slots=%lld kv_heads=%lld d=%lld capacity=%lld", (long long)layers,
                 (long long)batch, (long long)nodes, (long long)slots, (long long)kv_heads, (long long)d, (long long)capacity);
+  if (layers == 0 || batch == 0 || nodes == 0 || slots == 0 || kv_heads == 0 || d == 0 || capacity == 0) return 0;
   if ((path == nullptr) != (count == nullptr)) return fail("cache_append: path and count go together");
   if (!path && slots != nodes) return fail("cache_append: without a path every row has its slot (%lld rows, %lld slots)", (long long)nodes, (long long)slots);
-  if (layers == 0 || batch == 0 || nodes == 0 || slots == 0 || kv_heads == 0 || d == 0 || capacity == 0) return 0;
   constexpr int64_t kMost = int64_t{1} << 60;
   if (batch > INT32_MAX || nodes > INT32_MAX || slots > INT32_MAX || kv_heads > INT32_MAX || d > INT32_MAX || capacity > INT32_MAX ||
       batch > kMost / layers / kv_heads / d / capacity || batch > kMost / layers / kv_heads / d / nodes || batch > kMost / layers / kv_heads / d / slots)

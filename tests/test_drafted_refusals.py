@@ -107,3 +107,10 @@ def test_verify_tree_refuses_rows_beyond_64_bits(extents):
     # each extent is within its own range, the distributions' bytes are not
     rc, message = verify(**extents)
     assert rc == -1 and "verify_tree: the extents overflow" in message
+
+
+def test_empty_paths_and_batches_do_nothing():
+    # (an empty tensor has no address)
+    assert append(path=None, slots=0) == append(path=None, count=None, slots=0) == (0, "")
+    assert append(batch=0, path=None, count=None, slots=4) == append(layers=0, K=None, V=None, Kc=None, Vc=None) == (0, "")
+    assert append(path=None)[0] == append(count=None)[0] == append(path=None, count=None, slots=8)[0] == -1
