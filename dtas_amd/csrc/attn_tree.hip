@@ -1050,7 +1050,7 @@ __global__ void __launch_bounds__(256) attn_tree_join_kernel(TreeArgs a, TreeGri
 }
 
 // The launch of a kernel for `rows` rows and `threads` threads per workgroup and units of `unit` keys, parts of them as `cut` says: one workgroup
-// per CU.  `handed`: what a part's sums cost, in units of time (0: those of few rows are little)
+// per CU.  The lengths lie on the device: what is chosen here, and below, is chosen by the capacity (what the kernels cut, by the lengths).  `handed`: what a part's sums cost, in units of time (0: those of few rows are little)
 struct TreeShape {
   int rows, threads, unit;
   Cut cut;
@@ -1066,7 +1066,9 @@ int launch_tree(Kernel kernel, const TreeArgs& a, int64_t batch, int DP, const T
   const int64_t units = ceil_div(a.capacity, shape.unit) + ceil_div(a.T, shape.unit), useful = static_cast<float>(units) <= static_cast<float>(cut.whole) + 2.f * cut.spread * sqrtf(static_cast<float>(units + batch - 1)) ? 0 : batch * ceil_div(units, cut.least), limit = batch * cut.most;
   budget = budget > useful ? useful : budget;
   budget = budget > limit ? limit : budget;
-  if (budget <= batch) budget = 0;  // every sequence in one piece (as it would be by least_of, whatever the lengths: a sequence has one unit at least)
+  // Every sequence in one piece: no workgroup is left for a second one.  (Also where one is far longer than the others: 8 sequences on 32 key heads of 128, one after 32000 keys
+  // and seven after 100, take 398 us, the long one alone 91.)
+  if (budget <= batch) budget = 0;
   const int64_t slots = budget == 0 ? batch : budget;
   if (batch > INT32_MAX || problems * slots > INT32_MAX) return fail("attn_tree: the launch has too many workgroups");
   *grid = TreeGrid{static_cast<int>(batch), static_cast<int>(slots), static_cast<int>(budget), static_cast<int>(groups), cut, nullptr, nullptr, nullptr};
@@ -1120,11 +1122,13 @@ int launch_tree_rows(const TreeArgs& a, int64_t batch, hipStream_t s) {
   // Beyond 16 rows, or 8 of heads of more than 128, sharing the keys pays only where they are few: 32 rows of 64 heads on 8 after 300 keys 8.1 us, sharing the rows 10.3,
   // 20 rows of 32 on 8 after 500 12.8 / 11.6, 32 rows after 1000 16.7 / 13.2, after 16000 29.5 / 20.2; 16 rows of 256 after 1569 19.2 / 15.5.  16 rows of 80
   // after 3001 12.6 / 15.6, one row of 256 on 8 heads after 4000 16.5 / 21.6.
+  // (heads of 64, two sequences; 32 rows of 128 on 8 heads after 300 keys of one sequence take 14.7 sharing the keys and 11.3 sharing the rows)
   const bool few = a.capacity <= 384;
   if (rows <= (DP <= 128 ? 16 : 8) || (rows <= 16 && few)) return launch_few<DP, 1, (DP <= 128 ? 8 : 4)>(a, batch, s);
   if (rows <= 32 && few) return launch_few<DP, 2, (DP <= 128 ? 8 : 4)>(a, batch, s);
   // Blocks of 64, 128 or 256 rows: larger ones read K and V less often, smaller ones hand fewer sums over.  256 rows on 8 heads of 128 after 1000 / 4000 / 16000 / 65533
-  // keys: 15.0, 21.7, 48.3, 163 us in blocks of 64, 19.1, 23.2, 37.8, 118 of 128, 23.7, 27.8, 39.2, 102 of 256.
+  // keys: 15.0, 21.7, 48.3, 163 us in blocks of 64, 19.1, 23.2, 37.8, 118 of 128, 23.7, 27.8, 39.2, 102 of 256.  (The caches full: after 1000 keys in a cache of 32768 rows blocks of
+  // 256 are taken, and 24.1 us.)
   if (rows <= 64) return launch_rows<DP, 1, 4>(a, batch, s);
   const float by64 = blocks_us(a, batch, 64, DP), by128 = blocks_us(a, batch, 128, DP);
   if constexpr (DP <= 128) {

@@ -62,7 +62,8 @@ __device__ __forceinline__ f32x4 load4(const float* p) {
 }
 
 // The sum of max(p - c q, 0) over [from, to), by one wavefront; q is not read where c is 0.  `from` is a multiple of 4 of the row, and so is `to` unless it
-// is the row's end.  A pass over both rows of 50280 tokens takes a workgroup 3 us: what a CU draws from its L2 (in fp32 the sums take as long).
+// is the row's end.  A refusal, a pass of a workgroup over both rows of 50280 tokens, takes 4.4 us: a CU draws them from its
+// L2 in 3.7 (with a maximum in the place of the sums), the 64-bit arithmetic alone takes 3.1, and with sums in fp32 it is 3.9.
 __device__ __forceinline__ double sum_rest(const float* p, const float* q, double c, int64_t from, int64_t to, int lane) {
   double s[4] = {0.0, 0.0, 0.0, 0.0};
   constexpr int kAtOnce = 3;
