@@ -119,12 +119,19 @@ SIGNATURES = {
     "dtas_attn_tree_f16": [_vp] * 8 + [_i64] * 7 + [ctypes.c_float, _vp],
     "dtas_verify_tree_f32": [_vp] * 9 + [_i64] * 3 + [_vp],
     "dtas_cache_append_f16": [_vp] * 7 + [_i64] * 7 + [_vp],
+    "dtas_page_assign_i32": [_vp] * 9 + [_i64] * 5 + [_vp],
+    "dtas_page_append_f16": [_vp] * 5 + [_i64] * 6 + [_vp],
+    "dtas_attn_paged_f16": [_vp] * 6 + [_i64] * 8 + [ctypes.c_float, _vp],
+    "dtas_beam_select_f32": [_vp] * 7 + [_i64] * 4 + [_vp],
+    "dtas_page_reorder_f16": [_vp] * 10 + [_i64] * 8 + [_vp],
 }
 
 # entry points that builds of this ABI version from before them lack: such a build (DTAS_LIBRARY) serves everything else
-LATER = {"dtas_builtin_gemm", "dtas_gemv_q4_f16", "dtas_attn_tree_f16", "dtas_verify_tree_f32", "dtas_cache_append_f16"}
+LATER = {"dtas_builtin_gemm", "dtas_gemv_q4_f16", "dtas_attn_tree_f16", "dtas_verify_tree_f32", "dtas_cache_append_f16",
+         "dtas_page_assign_i32", "dtas_page_append_f16", "dtas_attn_paged_f16", "dtas_beam_select_f32", "dtas_page_reorder_f16"}
 
 MAX_TREE_NODES = 64
+MAX_BEAMS = 32
 
 _lib = None
 

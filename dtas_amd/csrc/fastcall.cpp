@@ -31,7 +31,9 @@ namespace {
   X(dtas_softmax_temperature_f32) X(dtas_split3_f16) X(dtas_swap_axes_f16) X(dtas_rotary_f16) X(dtas_take_f16)           \
   X(dtas_take_q8_f16) X(dtas_gemv_q8_f32) X(dtas_gemv_q8_f16) X(dtas_gemm_q8_f16_fused) X(dtas_last_error)
 // entry points that older builds of the library lack: null there, and the function leaves its calls to the Python body
-#define DTAS_LATER_ENTRIES(X) X(dtas_gemv_q4_f16) X(dtas_attn_tree_f16) X(dtas_verify_tree_f32) X(dtas_cache_append_f16)
+#define DTAS_LATER_ENTRIES(X)                                                                                            \
+  X(dtas_gemv_q4_f16) X(dtas_attn_tree_f16) X(dtas_verify_tree_f32) X(dtas_cache_append_f16) X(dtas_page_assign_i32)     \
+  X(dtas_page_append_f16) X(dtas_attn_paged_f16) X(dtas_beam_select_f32) X(dtas_page_reorder_f16)
 #define DTAS_DECLARE(name) decltype(&::name) p_##name = nullptr;
 DTAS_ENTRIES(DTAS_DECLARE)
 DTAS_LATER_ENTRIES(DTAS_DECLARE)
@@ -408,6 +410,78 @@ DTAS_FUNCTION(_cache_append, 7, {
   }
 })
 
+// ---- requests served from one pool of pages
+// lens, count, table, free, free_count, page, slots, new_lens, left, starts
+DTAS_FUNCTION(_page_assign, 10, {
+  auto *lens = a.tensor(0, at::kInt), *count = a.tensor(1, at::kInt), *table = a.tensor(2, at::kInt), *free = a.tensor(3, at::kInt), *height = a.tensor(4, at::kInt);
+  const int64_t page = a.integer(5);
+  auto *slots = a.tensor(6, at::kInt), *new_lens = a.tensor(7, at::kInt), *left = a.tensor(8, at::kInt);
+  if (a.ok && p_dtas_page_assign_i32 && table->dim() == 2 && free->dim() == 1 && height->numel() == 1 && left->numel() == 1) {
+    const int64_t B = table->size(0);
+    auto* starts = a.optional(9, at::kInt, B + 1);
+    for (auto* t : {lens, count, new_lens}) a.require(shaped(t, {B}));
+    a.require(starts ? starts->dim() == 1 && slots->dim() == 1 : slots->dim() == 2 && slots->size(0) == B);
+    if (a.ok && here({lens, count, table, free, height, slots, new_lens, left, starts}))
+      return DTAS_CALL(dtas_page_assign_i32, ptr(lens), ptr(count), ptr(table), ptr(free), ptr(height), ptr(starts), ptr(slots), ptr(new_lens), ptr(left), B,
+                       slots->size(-1), table->size(1), page, free->size(0));
+  }
+})
+
+// K, V, slots, K_pages, V_pages
+DTAS_FUNCTION(_page_append, 5, {
+  auto *K = a.tensor(0, F16), *V = a.tensor(1, F16), *slots = a.tensor(2, at::kInt), *Kp = a.tensor(3, F16), *Vp = a.tensor(4, F16);
+  if (a.ok && p_dtas_page_append_f16 && K->dim() >= 3 && Kp->dim() == K->dim() + 1 && V->sizes() == K->sizes() && Vp->sizes() == Kp->sizes()) {
+    const int64_t rows = K->size(-3), kv_heads = K->size(-2), d = K->size(-1);
+    a.require(Kp->size(-3) == kv_heads && Kp->size(-1) == d && slots->numel() == rows);
+    for (int64_t i = 0; i + 3 < K->dim(); ++i) a.require(K->size(i) == Kp->size(i));
+    if (a.ok && here({K, V, slots, Kp, Vp}))
+      return DTAS_CALL(dtas_page_append_f16, ptr(K), ptr(V), ptr(slots), ptr(Kp), ptr(Vp), K->numel() / (rows * kv_heads * d), rows, kv_heads, d, Kp->size(-2),
+                       Kp->size(-4));
+  }
+})
+
+// Q, K_pages, V_pages, table, lens, out, scale (None: 1 / sqrt(d)), beams
+DTAS_FUNCTION(_attn_paged, 8, {
+  auto *Q = a.tensor(0, F16), *Kp = a.tensor(1, F16), *Vp = a.tensor(2, F16), *table = a.tensor(3, at::kInt), *lens = a.tensor(4, at::kInt), *out = a.tensor(5, F16);
+  const int64_t beams = a.integer(7);
+  if (a.ok && p_dtas_attn_paged_f16 && Q->dim() == 3 && Kp->dim() == 4 && table->dim() == 2) {
+    const int64_t B = Q->size(0), heads = Q->size(1), d = Q->size(2);
+    const float scale = argv[6] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(d))) : a.number(6);
+    if (a.require(Kp->size(3) == d && Vp->sizes() == Kp->sizes() && out->sizes() == Q->sizes() && table->size(0) == B && shaped(lens, {B}) &&
+                  here({Q, Kp, Vp, table, lens, out})))
+      return DTAS_CALL(dtas_attn_paged_f16, ptr(Q), ptr(Kp), ptr(Vp), ptr(table), ptr(lens), ptr(out), B, heads, Kp->size(1), d, Kp->size(2), Kp->size(0),
+                       table->size(1), beams, scale);
+  }
+})
+
+// logits, scores, done, tokens, parents, new_scores, new_done, eos
+DTAS_FUNCTION(_beam_select, 8, {
+  auto *logits = a.tensor(0, F32), *scores = a.tensor(1, F32), *tokens = a.tensor(3, at::kInt), *parents = a.tensor(4, at::kInt), *new_scores = a.tensor(5, F32);
+  const int64_t eos = a.integer(7);
+  if (a.ok && p_dtas_beam_select_f32 && logits->dim() == 3) {
+    const int64_t groups = logits->size(0), beams = logits->size(1);
+    auto *done = a.optional(2, at::kInt, groups * beams), *new_done = a.optional(6, at::kInt, groups * beams);
+    for (auto* t : {scores, done, tokens, parents, new_scores, new_done}) a.require(!t || shaped(t, {groups, beams}));
+    if (a.ok && here({logits, scores, done, tokens, parents, new_scores, new_done}))
+      return DTAS_CALL(dtas_beam_select_f32, ptr(logits), ptr(scores), ptr(done), ptr(tokens), ptr(parents), ptr(new_scores), ptr(new_done), groups, beams,
+                       logits->size(2), eos);
+  }
+})
+
+// parents, table, lens, free, free_count, new_table, new_lens, left, K_pages, V_pages
+DTAS_FUNCTION(_page_reorder, 10, {
+  auto *parents = a.tensor(0, at::kInt), *table = a.tensor(1, at::kInt), *lens = a.tensor(2, at::kInt), *free = a.tensor(3, at::kInt), *height = a.tensor(4, at::kInt);
+  auto *new_table = a.tensor(5, at::kInt), *new_lens = a.tensor(6, at::kInt), *left = a.tensor(7, at::kInt), *Kp = a.tensor(8, F16), *Vp = a.tensor(9, F16);
+  if (a.ok && p_dtas_page_reorder_f16 && table->dim() == 3 && free->dim() == 1 && Kp->dim() >= 4) {
+    const int64_t groups = table->size(0), beams = table->size(1), pages = Kp->size(-4), kv_heads = Kp->size(-3), page = Kp->size(-2), d = Kp->size(-1);
+    for (auto* t : {parents, lens, new_lens}) a.require(shaped(t, {groups, beams}));
+    if (a.require(new_table->sizes() == table->sizes() && Vp->sizes() == Kp->sizes() && free->size(0) == pages && height->numel() == 1 && left->numel() == 1 &&
+                  here({parents, table, lens, free, height, new_table, new_lens, left, Kp, Vp})))
+      return DTAS_CALL(dtas_page_reorder_f16, ptr(parents), ptr(table), ptr(lens), ptr(free), ptr(height), ptr(new_table), ptr(new_lens), ptr(left), ptr(Kp), ptr(Vp),
+                       Kp->numel() / (pages * kv_heads * page * d), groups, beams, table->size(2), kv_heads, d, page, pages);
+  }
+})
+
 // bind({entry point: address}, DtasError)
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *addresses, *error;
@@ -443,6 +517,7 @@ PyMethodDef methods[] = {DTAS_METHOD(add), DTAS_METHOD(copy), DTAS_METHOD(cast),
                          DTAS_METHOD(softmax_temperature), DTAS_METHOD(split3), DTAS_METHOD(swap_axes), DTAS_METHOD(rotary),
                          DTAS_METHOD(take), DTAS_METHOD(take_q8), DTAS_METHOD(gemv_q8_f32), DTAS_METHOD(gemv_q8), DTAS_METHOD(gemm_q8),
                          DTAS_METHOD(_gemv_q4), DTAS_METHOD(_attn_tree), DTAS_METHOD(_verify_tree), DTAS_METHOD(_cache_append),
+                         DTAS_METHOD(_page_assign), DTAS_METHOD(_page_append), DTAS_METHOD(_attn_paged), DTAS_METHOD(_beam_select), DTAS_METHOD(_page_reorder),
                          {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

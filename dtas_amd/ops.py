@@ -629,3 +629,126 @@ def cache_append(K: torch.Tensor, V: torch.Tensor, path: Optional[torch.Tensor],
             layers *= extent
         check(lib().dtas_cache_append_f16(_p(K), _p(V), _p(path), _p(count), _p(K_cache), _p(V_cache), _p(lens), layers, B, nodes,
                                           nodes if path is None else path.shape[1], kv_heads, d, capacity, _stream()), "dtas_cache_append_f16")
+
+
+def page_assign(lens: torch.Tensor, count: torch.Tensor, table: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, page: int,
+                slots: torch.Tensor, new_lens: torch.Tensor, left: torch.Tensor, starts: Optional[torch.Tensor] = None) -> None:
+    """Pages for the rows that join, and their slots: count[b] rows join sequence b behind its lens[b], row t at position j = lens[b] + t
+    with slot table[b, j // page] * page + j % page.  What the table (B, columns) lacks for that is taken from the top of the stack
+    free (pages), free_count (1) high, in the order of the sequences; left (1) gets its new height, new_lens (B) the lengths with what
+    joined; they may be free_count and lens themselves.  slots is (B, rows), -1 behind a sequence's count, or with ``starts`` (B + 1, written
+    as well) one row of all sequences' rows one behind the other, -1 behind the last.  All int32.  A sequence that cannot be served keeps its
+    length and gets no page and no slot: no room in its table or in slots, a negative length or count, or more pages needed by it and those
+    in front than there are.  ``page_append`` takes the slots, ``attn_paged`` the table and new_lens."""
+    if _fastcall._page_assign(lens, count, table, free, free_count, page, slots, new_lens, left, starts):
+        return
+    with _one_device("page_assign", lens, count, table, free, free_count, slots, new_lens, left, starts):
+        _ints("page_assign", lens, count, table, free, free_count, slots, new_lens, left, starts)
+        if table.dim() != 2 or free.dim() != 1 or slots.dim() != (2 if starts is None else 1):
+            raise ValueError("page_assign: expects table (B, columns), free (pages) and slots (B, rows), or (rows) with starts (B + 1)")
+        B, columns = table.shape
+        if any(tuple(t.shape) != (B,) for t in (lens, count, new_lens)) or free_count.numel() != 1 or left.numel() != 1 \
+                or (starts is None and slots.shape[0] != B) or (starts is not None and tuple(starts.shape) != (B + 1,)):
+            raise ValueError("page_assign: shape mismatch")
+        check(lib().dtas_page_assign_i32(_p(lens), _p(count), _p(table), _p(free), _p(free_count), _p(starts), _p(slots), _p(new_lens), _p(left),
+                                         B, slots.shape[-1], columns, int(page), free.shape[0], _stream()), "dtas_page_assign_i32")
+
+
+def page_append(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor) -> None:
+    """Rows into their slots: K_pages[..., s // page, h, s % page, :] = K[..., n, h, :] with s = slots[n], and V alike.  K and V (..., rows,
+    kv_heads, d), the pools (..., pages, kv_heads, page, d), fp16, with the same leading extents (the layers, or none); slots int32, as many as
+    rows, of any shape (``page_assign`` writes them).  Slots outside [0, pages * page) are left out; they are distinct otherwise."""
+    if _fastcall._page_append(K, V, slots, K_pages, V_pages):
+        return
+    with _one_device("page_append", K, V, slots, K_pages, V_pages):
+        if any(t.dtype != torch.float16 for t in (K, V, K_pages, V_pages)):
+            raise ValueError("page_append: expects fp16 keys, values and pages")
+        _ints("page_append", slots)
+        if K.dim() < 3 or K_pages.dim() != K.dim() + 1:
+            raise ValueError("page_append: expects K (..., rows, kv_heads, d) and pages (..., pages, kv_heads, page, d)")
+        rows, kv_heads, d = K.shape[-3:]
+        pages, page = K_pages.shape[-4], K_pages.shape[-2]
+        if V.shape != K.shape or V_pages.shape != K_pages.shape or tuple(K_pages.shape) != (*K.shape[:-3], pages, kv_heads, page, d) or slots.numel() != rows:
+            raise ValueError("page_append: shape mismatch")
+        layers = 1
+        for extent in K.shape[:-3]:
+            layers *= extent
+        check(lib().dtas_page_append_f16(_p(K), _p(V), _p(slots), _p(K_pages), _p(V_pages), layers, rows, kv_heads, d, page, pages, _stream()),
+              "dtas_page_append_f16")
+
+
+def attn_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, out: torch.Tensor,
+               scale: Optional[float] = None, beams: int = 1) -> None:
+    """Attention of one new token per sequence over its pages: out [b, h] = softmax(scale * Q[b, h] . keys) . values over the positions
+    j < lens[b] (the token's own among them: ``page_append`` goes first), position j in page table[b, j // page], row j % page.  Q and out (B,
+    heads, d), one layer's K_pages and V_pages (pages, kv_heads, page, d), fp16; table int32 (B, columns), lens int32 (B).  heads is a
+    multiple of kv_heads; scale 1 / sqrt(d) if None.  Positions in pages outside the pool are not seen; a row that sees nothing is zeros.
+    With ``beams`` > 1 every so many sequences in a row form a group, whose pages of the same column are read once for all that name
+    them; the result is that of beams = 1.  Pages of a multiple of 16 positions, d a multiple of 8 and data on 16-byte boundaries run on the
+    matrix cores, others element by element."""
+    if _fastcall._attn_paged(Q, K_pages, V_pages, table, lens, out, scale, beams):
+        return
+    with _one_device("attn_paged", Q, K_pages, V_pages, table, lens, out):
+        if any(t.dtype != torch.float16 for t in (Q, K_pages, V_pages, out)):
+            raise ValueError("attn_paged: expects fp16 queries, pages and output")
+        _ints("attn_paged", table, lens)
+        if Q.dim() != 3 or K_pages.dim() != 4 or table.dim() != 2:
+            raise ValueError("attn_paged: expects Q (B, heads, d), pages (pages, kv_heads, page, d) and table (B, columns)")
+        B, heads, d = Q.shape
+        pages, kv_heads, page = K_pages.shape[:3]
+        if K_pages.shape[3] != d or V_pages.shape != K_pages.shape or out.shape != Q.shape or table.shape[0] != B or tuple(lens.shape) != (B,):
+            raise ValueError("attn_paged: shape mismatch")
+        check(lib().dtas_attn_paged_f16(_p(Q), _p(K_pages), _p(V_pages), _p(table), _p(lens), _p(out), B, heads, kv_heads, d, page, pages, table.shape[1],
+                                        int(beams), d ** -0.5 if scale is None and d else float(scale or 0.0), _stream()), "dtas_attn_paged_f16")
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: Optional[torch.Tensor], tokens: torch.Tensor, parents: torch.Tensor,
+                new_scores: torch.Tensor, new_done: Optional[torch.Tensor], eos: int = -1) -> None:
+    """The best continuations of each request's beams: candidate (w, v) has scores[w] + log_softmax(logits[w])[v]; a beam that is done goes on
+    with token ``eos`` alone, at scores[w].  The best, as many as there are beams, in their order (ties: the lower w, then the lower v): parents
+    w and tokens v int32, new_scores; new_done where the parent was done or the token is eos.  logits (requests, beams, V) and scores
+    (requests, beams) fp32, done int32 (requests, beams) or None with new_done None: no beam is done.  new_scores and new_done may be scores
+    and done themselves.  What is no finite number counts as -inf (a request begins with scores (0, -inf, ...)).  Up to 32 beams.
+    ``page_reorder`` takes the parents."""
+    if _fastcall._beam_select(logits, scores, done, tokens, parents, new_scores, new_done, eos):
+        return
+    with _one_device("beam_select", logits, scores, done, tokens, parents, new_scores, new_done):
+        if any(t.dtype != torch.float32 for t in (logits, scores, new_scores)):
+            raise ValueError("beam_select: expects fp32 logits and scores")
+        _ints("beam_select", done, tokens, parents, new_done)
+        if logits.dim() != 3:
+            raise ValueError("beam_select: expects logits (requests, beams, V)")
+        groups, beams, V = logits.shape
+        if any(t is not None and tuple(t.shape) != (groups, beams) for t in (scores, done, tokens, parents, new_scores, new_done)):
+            raise ValueError("beam_select: shape mismatch")
+        check(lib().dtas_beam_select_f32(_p(logits), _p(scores), _p(done), _p(tokens), _p(parents), _p(new_scores), _p(new_done), groups, beams, V, int(eos),
+                                         _stream()), "dtas_beam_select_f32")
+
+
+def page_reorder(parents: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, new_table: torch.Tensor,
+                 new_lens: torch.Tensor, left: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor) -> None:
+    """Tables and lengths follow the beams that were chosen: row w of a request takes the pages and the length of its row parents[w] (outside
+    [0, beams): none any more).  A page that is filled in part stays with the first row of a parent, the others take a copy of its rows in all layers;
+    pages that no row of the request names any more go back onto the stack free (pages), free_count (1) high.  A prompt is handed to all beams with
+    parents 0, a request that has ended lets go with parents -1.  parents, lens, new_lens (requests, beams), table and new_table (requests, beams,
+    columns), int32; K_pages and V_pages (..., pages, kv_heads, page, d) fp16 with all layers in front.  new_table, new_lens and left (1) may
+    be table, lens and free_count themselves.  A row for whose copy no page is left is lost, with length -1: not while the stack
+    holds a page for each row.  Up to 32 beams."""
+    if _fastcall._page_reorder(parents, table, lens, free, free_count, new_table, new_lens, left, K_pages, V_pages):
+        return
+    with _one_device("page_reorder", parents, table, lens, free, free_count, new_table, new_lens, left, K_pages, V_pages):
+        _ints("page_reorder", parents, table, lens, free, free_count, new_table, new_lens, left)
+        if any(t.dtype != torch.float16 for t in (K_pages, V_pages)):
+            raise ValueError("page_reorder: expects fp16 pages")
+        if table.dim() != 3 or free.dim() != 1 or K_pages.dim() < 4:
+            raise ValueError("page_reorder: expects table (requests, beams, columns), free (pages) and pages (..., pages, kv_heads, page, d)")
+        groups, beams, columns = table.shape
+        pages, kv_heads, page, d = K_pages.shape[-4:]
+        if any(tuple(t.shape) != (groups, beams) for t in (parents, lens, new_lens)) or new_table.shape != table.shape or V_pages.shape != K_pages.shape \
+                or free.shape[0] != pages or free_count.numel() != 1 or left.numel() != 1:
+            raise ValueError("page_reorder: shape mismatch")
+        layers = 1
+        for extent in K_pages.shape[:-4]:
+            layers *= extent
+        check(lib().dtas_page_reorder_f16(_p(parents), _p(table), _p(lens), _p(free), _p(free_count), _p(new_table), _p(new_lens), _p(left), _p(K_pages), _p(V_pages),
+                                          layers, groups, beams, columns, kv_heads, d, page, pages, _stream()), "dtas_page_reorder_f16")

@@ -466,6 +466,67 @@ int dtas_cache_append_f16(const void* K, const void* V, const void* path, const 
                           int64_t layers, int64_t batch, int64_t nodes, int64_t slots, int64_t kv_heads, int64_t d, int64_t capacity,
                           void* stream);
 
+/* ==== requests served together from one pool of pages ==========================================================
+ * No PrimFunc of the reference: its runtime keeps a cache per sequence.  The entry points below serve many requests, the beams of a
+ * beam search among them, whose keys and values lie in pages of one pool: K_pages and V_pages [layers, pages, kv_heads, page, d] (or
+ * one layer of them), fp16, `page` positions to a page.  table[batch, columns] names a sequence's pages in order: position j of
+ * sequence b lies in page table[b, j / page], row j % page; lens[batch] says how many positions it holds, so that only the first
+ * ceil(lens[b] / page) entries of its row mean anything.  free[pages] is the stack of the pages that no table names, free_count[1] its
+ * height.  All of these are int32 on the device, and nothing here comes back to the host: values outside their range are treated as
+ * stated, never followed.  Pages are shared only between the rows of one group (the beams of one request), in the same column; the page that a row
+ * is still filling belongs to it alone, as dtas_page_reorder leaves it. */
+#define DTAS_MAX_BEAMS 32
+
+/* ---- pages for the rows that join, and their slots ----
+ * count[b] rows join sequence b behind its lens[b].  Its row t gets slot table[b, j / page] * page + j % page, j = lens[b] + t; columns from
+ * ceil(lens[b] / page) on are taken from the top of the free stack, in the order of the sequences.  A sequence that cannot be served keeps its
+ * length and gets no page and no slot (-1): lens[b] or count[b] negative; more than columns * page positions; more rows than the slot map has for it;
+ * or the pages that it and the sequences before it need (those not served for another reason need none) exceed free_count.  A sequence that needs no page is
+ * never short of one.  slots without starts: [batch, rows], count[b] of `rows` used, -1 behind them.  With starts [batch + 1]: slots[rows], the rows of all
+ * sequences one behind the other, sequence b's from starts[b] = sum of max(count[i], 0), i < b, on (at most 2^31 - 1), -1 behind the last; one whose
+ * rows end behind `rows` is not served.  A page of the table or the stack outside [0, pages) leaves its rows without a slot.  new_lens[batch]: the lengths
+ * with what joined (new_lens == lens: in place); left[1]: the stack's new height (left == free_count: in place).  `free` is only read; pages * page < 2^31. */
+int dtas_page_assign_i32(const void* lens, const void* count, void* table, const void* free, const void* free_count, void* starts, void* slots,
+                         void* new_lens, void* left, int64_t batch, int64_t rows, int64_t columns, int64_t page, int64_t pages, void* stream);
+
+/* ---- rows into their slots, in all layers ----
+ * K_pages[l, s / page, h, s % page, :] = K[l, n, h, :] with s = slots[n], and V alike: K and V [layers, rows, kv_heads, d].  Slots outside [0, pages * page)
+ * are left out; slots that occur twice are the caller's mistake (either row's pieces may win).  pages * page < 2^31. */
+int dtas_page_append_f16(const void* K, const void* V, const void* slots, void* K_pages, void* V_pages, int64_t layers, int64_t rows,
+                         int64_t kv_heads, int64_t d, int64_t page, int64_t pages, void* stream);
+
+/* ---- attention of one new token per sequence over its pages ----
+ * out[b,h,:] = sum_j softmax_j(scale * Q[b,h,:] . k_j) v_j over the positions j < lens[b] (clipped to [0, columns * page]; the token's own is among
+ * them); positions in pages outside [0, pages) are not seen, a row that sees nothing is zeros.  Q and out [batch, heads, d], one layer's K_pages and V_pages
+ * [pages, kv_heads, page, d]; heads is a multiple of kv_heads, query head h reads key head h / (heads / kv_heads).  Sequences in a row, `beams` of them, form a group: a
+ * page that several of them name in the same column is read once for all (the result is the same with beams = 1).  batch is a multiple of beams.
+ * d up to 256; d a multiple of 8, data on 16-byte boundaries and pages of a multiple of 16 positions run on the matrix cores, others element by element.  fp32 scores,
+ * statistics and sums; weights in fp16 on the matrix cores, as in dtas_attn_tree_f16.  scale is a finite number up to 2e38 either way.  Uses the
+ * split-K workspace, under the rules stated at the top of this file. */
+int dtas_attn_paged_f16(const void* Q, const void* K_pages, const void* V_pages, const void* table, const void* lens, void* out, int64_t batch,
+                        int64_t heads, int64_t kv_heads, int64_t d, int64_t page, int64_t pages, int64_t columns, int64_t beams, float scale, void* stream);
+
+/* ---- the best continuations of each request's beams ----
+ * logits [groups, beams, V], scores [groups, beams], fp32.  Candidate (w, v) of a group has scores[w] + log_softmax(logits[w])[v]; a beam that is done (done[w] != 0)
+ * goes on with token eos alone, at scores[w].  What is no finite number counts as -inf.  The `beams` best candidates in their order, ties to the lower w, then the lower
+ * v: parents, tokens [groups, beams] int32, new_scores [groups, beams] fp32; new_done = done of the parent, or token == eos.  done and new_done [groups, beams] int32,
+ * or both NULL: no beam is done.  eos outside [0, V): none is (a beam that is done then has no candidate).  new_scores == scores and new_done == done are allowed.  beams up to DTAS_MAX_BEAMS.
+ * Candidates are compared in 64 bits, sums of exponentials are in 64 bits over terms in 32.  Uses the split-K workspace. */
+int dtas_beam_select_f32(const void* logits, const void* scores, const void* done, void* tokens, void* parents, void* new_scores, void* new_done,
+                         int64_t groups, int64_t beams, int64_t V, int64_t eos, void* stream);
+
+/* ---- tables, lengths and part-filled pages follow the beams that were chosen ----
+ * Row w of a group takes the pages and the length of its row parents[g, w]; with a parent outside [0, beams) it holds nothing any more.  A page that is filled only in part
+ * stays with the first row (of those with the same parent), the others take a copy of its rows, in all layers, in a page from the stack.  Pages that no row of
+ * the group names any more go onto the stack first, in the order of group, column and row; the copies take theirs from its top, in the order of group and row.  A row for whose
+ * copy no page is left is lost: its length becomes -1 (it cannot happen with groups * (beams - 1) pages on the stack).
+ * parents, lens, new_lens [groups, beams], table and new_table [groups, beams, columns], free [pages], all layers' K_pages and V_pages.  new_table == table, new_lens == lens and
+ * left == free_count: in place.  new_table is written in the columns that its rows hold.  Lengths are clipped to [0, columns * page], entries outside [0, pages) are handed on as they are.
+ * beams up to DTAS_MAX_BEAMS.  Uses the split-K workspace. */
+int dtas_page_reorder_f16(const void* parents, const void* table, const void* lens, void* free, const void* free_count, void* new_table, void* new_lens,
+                          void* left, void* K_pages, void* V_pages, int64_t layers, int64_t groups, int64_t beams, int64_t columns, int64_t kv_heads, int64_t d,
+                          int64_t page, int64_t pages, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
