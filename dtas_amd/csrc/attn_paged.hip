@@ -74,125 +74,113 @@ __global__ void __launch_bounds__(64) attn_paged_scalar_kernel(PagedArgs a, int6
 // all its addresses are a scalar and a lane's constant.  K comes as the matrix cores take it, straight from memory; V passes through a piece of the LDS that is the
 // wavefront's own and is read from there transposed.  The next visit's K and V are on their way in registers, and the table's entries a block further ahead.
 // In a group a block is visited once for every page that its sequences name there; rows that do not name it have their scores masked.
-// Sequences are cut into parts by their lengths, on the device: see find_part.
+// The blocks of all problems, one behind the other, are dealt out in equal shares, on the device, which knows the lengths: see Share.
+constexpr int kStreamed = 2;  // loads that nobody repeats (nt): 2.3 GB in pieces of 8 KiB 6.0 TB/s without, 6.8 with
+constexpr int kNear = 8;
+constexpr int most_shares(int RT) { return 256 / RT; }
+__device__ __forceinline__ uint64_t pair_of(float a, float b) { return static_cast<uint64_t>(__builtin_bit_cast(unsigned, a)) | static_cast<uint64_t>(__builtin_bit_cast(unsigned, b)) << 32; }
 struct PagedGrid {
-  int problems, slots, beams, sub, subs;  // a problem: `sub` sequences at most of a group of `beams`, `subs` of which make up the group
-  int row_groups, extra, least, most;     // extra: parts that all problems together may have beyond one each (0: nothing is cut)
-  float whole;
+  int problems, beams, sub, subs;  // a problem: `sub` sequences at most of a group of `beams`, `subs` of which make up the group
+  int shares, row_groups, least;   // workgroups per key head and row group; a share's blocks, if there are as many
   float* ws;
   unsigned* arrivals;
-};
-struct Part {
-  int p, z, parts, first;  // problem, which of its parts, of how many, where the first one's sums lie; p < 0: nothing to do
 };
 __device__ __forceinline__ int first_sequence(const PagedGrid& grid, int p, int* count) {
   const int group = p / grid.subs, s = p - group * grid.subs, left = grid.beams - s * grid.sub;
   *count = left < grid.sub ? left : grid.sub;
   return group * grid.beams + s * grid.sub;
 }
-// blocks of 32 keys of a problem: those of its longest sequence
+// blocks of 32 keys of a problem: those of its longest sequence (one, to write its noughts, where that is empty)
 __device__ __forceinline__ int blocks_of(const PagedArgs& a, const PagedGrid& grid, int p) {
   int count;
   const int b = first_sequence(grid, p, &count);
-  unsigned longest = 0;
+  unsigned longest = 1;
   for (int i = 0; i < count; ++i) {
     const unsigned len = length_of(a, b + i);
     longest = longest > len ? longest : len;
   }
   return static_cast<int>((longest + 31) / 32);
 }
-// Parts of at most `per` blocks: a workgroup's even share of all blocks, `least` at least, and no more than `most` parts of one problem; nothing is cut where the longest problem is
-// not much more than that.  Every problem has a part; all have problems + blocks / per <= problems + extra.
-__device__ __forceinline__ int blocks_per_part(const PagedGrid& grid, float total, int longest) {
-  const float even = total * 1.0001f / static_cast<float>(grid.extra);
-  if (static_cast<float>(longest) <= grid.whole * even + static_cast<float>(grid.least)) return longest > 0 ? longest : 1;
-  int per = static_cast<int>(even) + 1;
-  per = per > grid.least ? per : grid.least;
-  const int few = (longest + grid.most - 1) / grid.most;
-  return per > few ? per : few;
-}
-__device__ __forceinline__ int parts_of(int blocks, int per) { return blocks > per ? (blocks + per - 1) / per : 1; }
-__device__ __forceinline__ Part found_at(int slot, int p0, int parts, int upto, int cut_upto, int lane_base, int cut_base) {
-  const uint64_t here = __builtin_amdgcn_ballot_w64(slot >= lane_base + upto - parts && slot < lane_base + upto);
-  if (here == 0) return Part{-1, 0, 0, 0};
-  const int l = __builtin_ctzll(here), n = __builtin_amdgcn_readlane(parts, l);
-  return Part{p0 + l, slot - (lane_base + __builtin_amdgcn_readlane(upto, l) - n), n, cut_base + __builtin_amdgcn_readlane(cut_upto, l) - n};
-}
+// Workgroup s has the blocks from s * per up to (s + 1) * per, but for a boundary less than `near` from the end of a problem, which moves there: a problem is cut into pieces
+// only where that is worth handing its sums over.  Every workgroup finds out for itself which problem its share begins in (p, whose blocks begin at `at`), and what
+// pieces there are of a problem follows from where its blocks begin and end.
+struct Share {
+  int p, at, from, to, per, near;
+};
 template <int W>
-__device__ __forceinline__ Part find_part(const PagedArgs& a, const PagedGrid& grid, int slot, int lane, int wave) {
-  if (grid.extra == 0) return Part{slot, 0, 1, 0};
+__device__ __forceinline__ Share find_share(const PagedArgs& a, const PagedGrid& grid, int s, int lane, int wave) {
+  auto cut = [&](int total) {
+    int per = (total + grid.shares - 1) / grid.shares;
+    per = per > grid.least ? per : grid.least;
+    const int64_t from = static_cast<int64_t>(s) * per;
+    return Share{-1, 0, from < total ? static_cast<int>(from) : -1, total - from > per ? static_cast<int>(from + per) : total, per, per / kNear + 1};
+  };
+  if (grid.problems == 1) {
+    Share share = cut(blocks_of(a, grid, 0));
+    share.p = share.from < 0 ? -1 : 0;
+    return share;
+  }
   if (grid.problems <= 64) {
-    const int blocks = lane < grid.problems ? blocks_of(a, grid, lane) : 0;
-    const int per = blocks_per_part(grid, wave_sum(static_cast<float>(blocks)), wave_most(blocks));
-    const int parts = lane < grid.problems ? parts_of(blocks, per) : 0;
-    return found_at(slot, 0, parts, sum_upto(parts), sum_upto(parts > 1 ? parts : 0), 0, 0);
+    const int blocks = lane < grid.problems ? blocks_of(a, grid, lane) : 0, upto = sum_upto(blocks);
+    Share share = cut(__builtin_amdgcn_readlane(upto, 63));
+    if (share.from < 0) return share;
+    share.p = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > share.from));
+    share.at = __builtin_amdgcn_readlane(upto - blocks, share.p);
+    return share;
   }
   // the wavefronts have a range of the problems each
-  __shared__ float totals[W];
-  __shared__ int longest[W], counts[W], cuts[W];
-  __shared__ Part found;
-  const int range = (grid.problems + 64 * W - 1) / (64 * W) * 64, from = wave * range, to = from + range < grid.problems ? from + range : grid.problems;
-  float total = 0.f;
-  int most = 0;
-  for (int c = from; c < to; c += 64) {
-    const int blocks = c + lane < to ? blocks_of(a, grid, c + lane) : 0, top = wave_most(blocks);
-    total += wave_sum(static_cast<float>(blocks));
-    most = most > top ? most : top;
-  }
-  if (lane == 0) {
-    totals[wave] = total;
-    longest[wave] = most;
-  }
-  if (threadIdx.x == 0) found.p = -1;
+  __shared__ int totals[W], found[2];
+  const int range = (grid.problems + 64 * W - 1) / (64 * W) * 64, first = wave * range, last = first + range < grid.problems ? first + range : grid.problems;
+  int total = 0;
+  for (int c = first; c < last; c += 64) total += wave_total(c + lane < last ? blocks_of(a, grid, c + lane) : 0);
+  if (lane == 0) totals[wave] = total;
   __syncthreads();
-  total = 0.f;
-  most = 0;
+  int base = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    total += totals[w];
-    most = most > longest[w] ? most : longest[w];
+    if (w == wave) base = all;
+    all += totals[w];
   }
-  const int per = blocks_per_part(grid, total, most);
-  int count = 0, cut = 0;
-  for (int c = from; c < to; c += 64) {
-    const int parts = c + lane < to ? parts_of(blocks_of(a, grid, c + lane), per) : 0;
-    count += wave_total(parts);
-    cut += wave_total(parts > 1 ? parts : 0);
-  }
-  if (lane == 0) {
-    counts[wave] = count;
-    cuts[wave] = cut;
-  }
-  __syncthreads();
-  int base = 0, cut_base = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w)
-    if (w < wave) {
-      base += counts[w];
-      cut_base += cuts[w];
-    }
-  if (slot >= base && slot < base + count) {
-    for (int c = from; c < to; c += 64) {
-      const int parts = c + lane < to ? parts_of(blocks_of(a, grid, c + lane), per) : 0, upto = sum_upto(parts), cut_upto = sum_upto(parts > 1 ? parts : 0);
-      const Part part = found_at(slot, c, parts, upto, cut_upto, base, cut_base);
-      if (part.p >= 0) {
-        if (lane == 0) found = part;
+  Share share = cut(all);
+  if (share.from >= base && share.from < base + total) {
+    for (int c = first; c < last; c += 64) {
+      const int blocks = c + lane < last ? blocks_of(a, grid, c + lane) : 0, upto = base + sum_upto(blocks);
+      const uint64_t behind = __builtin_amdgcn_ballot_w64(upto > share.from);
+      if (behind != 0) {
+        const int l = __builtin_ctzll(behind), at = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(blocks, l);  // (outside the branch, where all lanes are)
+        if (lane == 0) {
+          found[0] = c + l;
+          found[1] = at;
+        }
         break;
       }
-      base += __builtin_amdgcn_readlane(upto, 63);
-      cut_base += __builtin_amdgcn_readlane(cut_upto, 63);
+      base = __builtin_amdgcn_readlane(upto, 63);
     }
   }
   __syncthreads();
-  const Part part = found;
-  return Part{__builtin_amdgcn_readfirstlane(part.p), __builtin_amdgcn_readfirstlane(part.z), __builtin_amdgcn_readfirstlane(part.parts),
-              __builtin_amdgcn_readfirstlane(part.first)};
+  if (share.from < 0) return share;
+  share.p = __builtin_amdgcn_readfirstlane(found[0]);
+  share.at = __builtin_amdgcn_readfirstlane(found[1]);
+  return share;
 }
 
-// two halves of 16 keys at positions pos and pos + 16, where their K and V lie, and which sequences of the problem (bits) see them
+// The 8 channels of k step ks that a lane of `quarter` holds.  Of two steps that make up a 128-byte line of a row a lane has 32 contiguous bytes; of a single last one 16.
+template <int DP>
+__device__ __forceinline__ int channels_at(int ks, int quarter) {
+  return ks / 2 * 2 + 1 < DP / 32 ? ks / 2 * 64 + quarter * 16 + (ks & 1) * 8 : ks * 32 + quarter * 8;
+}
+template <int DP>
+__device__ __forceinline__ f16x8 channels_of(const half_t* row, int ks, int quarter, int d) {
+  const int at = channels_at<DP>(ks, quarter);
+  const f16x8 v = *reinterpret_cast<const f16x8*>(row + (at < d ? at : d - 8));
+  return at < d ? v : f16x8{};
+}
+
+// two halves of 16 keys at positions pos and pos + 16: where their K and V lie (bytes from the head's first), how many bytes of them are read (what is behind comes as nought,
+// and costs nothing), and which sequences of the problem (bits) see them
 struct Visit {
-  const char *k[2], *v[2];
-  unsigned pos, seen[2];
+  int64_t at[2];
+  unsigned bytes[2], seen[2], pos;
 };
 __device__ __forceinline__ unsigned bits_below(int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; }
 // over the sixteen rows of the lanes
@@ -204,13 +192,36 @@ __device__ __forceinline__ unsigned any_row(unsigned v) {
   return static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), 0));
 }
 
+// About how many blocks the sequences of a group have in common: 64 columns are looked at (which of them does not matter to the result)
+__device__ __forceinline__ int common_blocks(const PagedArgs& a, const int* names, int nb, unsigned my_len, unsigned longest, int lane) {
+  const unsigned columns = (longest + a.page - 1) / a.page, column = static_cast<unsigned>(static_cast<uint64_t>(columns) * lane / 64);
+  const int theirs = column < columns ? names[column] : -1;
+  bool same = true;
+  for (int i = 1; i < nb; i += 4) {
+    int some[4];
+    unsigned len[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = i + u < nb ? i + u : nb - 1;
+      len[u] = __shfl(my_len, j);
+      some[u] = column * a.page < len[u] ? names[static_cast<int64_t>(j) * a.columns + column] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) same = same && some[u] == theirs;
+  }
+  const uint64_t apart = __builtin_amdgcn_ballot_w64(!same);
+  const int l = apart == 0 ? 64 : __builtin_ctzll(apart);
+  if (l == 64) return static_cast<int>((longest + 31) / 32);
+  return l == 0 ? 0 : static_cast<int>(static_cast<unsigned>(static_cast<uint64_t>(columns) * (l - 1) / 64) * a.page / 32);
+}
+
 // A value may be infinite where its weight is too small for fp16 (below 2^-36 of the largest): zero times infinity, though the weight is a number in fp32 and the channel
-// infinite.  Such a channel shows in O, as NaN where the sum of the weights is a number (rare).  What it is instead depends on the keys alone whose values are no
-// numbers: they are looked for in the wavefront's blocks first, first + step .., and summed with their weights in fp32.  The four lanes of a row hold a quarter of
+// infinite.  Such a channel shows in O, as NaN where the sum of the weights is a number (rare); what visits took out is known as well.  What it is instead depends on the keys alone
+// whose values are no numbers: they are looked for in what the wavefront had, the items first, first + step .., and summed with their weights in fp32.  The four lanes of a row hold a quarter of
 // its channels each, and follow their own row's table.
 template <int DP, int KS, int DT>
-__device__ __forceinline__ void sum_again(const PagedArgs& a, const int* names, int beam, int hk, unsigned len, unsigned longest, unsigned first, unsigned step,
-                                          const f16x8 (&q)[KS], float top, float sum, int lane, f32x4 (&o)[DT]) {
+__device__ __forceinline__ void sum_again(const PagedArgs& a, const int* names, int b0, int beam, int hk, unsigned len, int common, int nb, int first, int last, int step,
+                                          const f16x8 (&q)[KS], float top, float sum, int lane, bool taken_out, f32x4 (&o)[DT]) {
   f32x4 all = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -218,18 +229,23 @@ __device__ __forceinline__ void sum_again(const PagedArgs& a, const int* names, 
     for (int j = 0; j < 4; ++j)
       if (dt * 16 + 16 <= below(DP) || dt * 16 + 4 * (lane >> 4) < a.d) all[j] += o[dt][j];
   const float some = (all[0] + all[1]) + (all[2] + all[3]);
-  const bool mine = some != some && sum == sum;
-  if (__builtin_amdgcn_ballot_w64(mine) == 0) return;
+  if (__builtin_amdgcn_ballot_w64((some != some && sum == sum) || taken_out) == 0) return;
   asm volatile("" : "+v"(lane), "+v"(beam));  // (nothing of what follows is computed ahead)
   const int quarter = lane >> 4;
   f32x4 fresh[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) fresh[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (unsigned at = first; at < (longest + 31) / 32; at += step)
-    for (unsigned pos = at * 32; pos < at * 32 + 32 && pos < longest; ++pos) {
+  for (int item = first; item < last; item += step) {
+    // (a group's block that is taken once for each sequence: what the first of those that name a page visits counts for all of them)
+    const int q0 = item - common, at = q0 < 0 ? item : common + q0 / nb, one = q0 < 0 ? -1 : q0 - q0 / nb * nb;
+    for (unsigned pos = at * 32u; pos < at * 32u + 32; ++pos) {
       const unsigned column = pos / a.page;
       const int page = pos < len ? names[static_cast<int64_t>(beam) * a.columns + column] : -1;
-      const bool shown = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages);
+      bool shown = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages);
+      for (int i = 0; one >= 0 && i <= one; ++i) {
+        const int theirs = pos / 16 * 16 < length_of(a, b0 + i) ? names[static_cast<int64_t>(i) * a.columns + column] : -1;
+        shown = shown && (theirs == page) == (i == one);
+      }
       const int64_t from = ((static_cast<int64_t>(shown ? page : 0) * a.kv_heads + hk) * a.page + (pos - column * a.page)) * a.d;
       const half_t *k = a.K + from, *v = a.V + from;
       bool odd = false;
@@ -244,7 +260,7 @@ __device__ __forceinline__ void sum_again(const PagedArgs& a, const int* names, 
       float t = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const f16x8 some_k = load_channels<DP>(reinterpret_cast<const char*>(k), ks, quarter, a.d);
+        const f16x8 some_k = channels_of<DP>(k, ks, quarter, a.d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) t = fmaf(static_cast<float>(some_k[e]), static_cast<float>(q[ks][e]), t);
       }
@@ -261,12 +277,12 @@ __device__ __forceinline__ void sum_again(const PagedArgs& a, const int* names, 
           }
         }
     }
-  if (mine) {
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[dt][j] = o[dt][j] != o[dt][j] ? fresh[dt][j] : o[dt][j];
   }
+  // (without such a key in it fresh is nought)
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[dt][j] = fresh[dt][j] + (o[dt][j] == o[dt][j] || sum != sum ? o[dt][j] : 0.f);
 }
 
 template <int DP, int RT, int W, bool GROUP>
@@ -276,16 +292,40 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
   __shared__ __attribute__((aligned(16))) char lds[W * kWave];
   __shared__ float stat_m[W][kRows], stat_l[W][kRows];
   __shared__ int flag;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, i16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = a.heads / a.kv_heads;
-  const int slot = static_cast<int>(blockIdx.x % grid.slots), hk = static_cast<int>(blockIdx.x / grid.slots % a.kv_heads), rg = static_cast<int>(blockIdx.x / grid.slots / a.kv_heads);
-  const Part part = find_part<W>(a, grid, slot, lane, wave);
-  if (part.p < 0) return;
-  int nb = 1;
-  const int b0 = GROUP ? first_sequence(grid, part.p, &nb) : part.p, R = nb * g;
+  const int hk = static_cast<int>(blockIdx.x % a.kv_heads), s_mine = static_cast<int>(blockIdx.x / a.kv_heads % grid.shares), rg = static_cast<int>(blockIdx.x / a.kv_heads / grid.shares);
+  const Share share = find_share<W>(a, grid, s_mine, threadIdx.x & 63, wave);
+  if (share.from < 0) return;
   const unsigned row_bytes = 2u * a.d;
   const int64_t head_bytes = static_cast<int64_t>(a.page) * row_bytes, page_bytes = head_bytes * a.kv_heads;
   const char *Kh = reinterpret_cast<const char*>(a.K) + hk * head_bytes, *Vh = reinterpret_cast<const char*>(a.V) + hk * head_bytes;
+  const int64_t kind = static_cast<int64_t>(hk) * grid.row_groups + rg;
+  char* mine = lds + wave * kWave;
+
+  for (int p = share.p, begin = share.at, end; begin < share.to; ++p, begin = end) {
+  const int p_blocks = __builtin_amdgcn_readfirstlane(blocks_of(a, grid, p));
+  end = begin + p_blocks;
+  // this problem's cuts: boundaries s from first_cut to last_cut; the blocks that are this workgroup's, and which piece they are
+  const int first_cut = (begin + share.near + share.per - 1) / share.per, last_cut = (end - share.near) / share.per, cuts = last_cut >= first_cut ? last_cut - first_cut + 1 : 0;
+  int lo = 0, hi = p_blocks, z = 0;
+  if (begin < share.from) {
+    if (share.from - begin < share.near) lo = 0;
+    else if (end - share.from < share.near) continue;
+    else lo = share.from - begin, z = s_mine - first_cut + 1;
+  }
+  if (end > share.to) {
+    if (share.to - begin < share.near) break;
+    if (end - share.to >= share.near) hi = share.to - begin;
+  }
+  const int parts = cuts + 1;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // (what depends on it is computed for each problem anew: kept from one to the next it would take half the registers)
+  const int lane = tid & 63, quarter = lane >> 4, i16 = lane & 15;
+  const unsigned tr_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)mine)) +
+                         (4 * quarter + (i16 >> 2)) * v_row_bytes(DP) + (i16 & 3) * 8;
+  int nb = 1;
+  const int b0 = GROUP ? first_sequence(grid, p, &nb) : p, R = nb * g;
 
   // ---- the rows
   f16x8 q[RT][KS];
@@ -297,27 +337,48 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
     beam[rt] = GROUP ? have / g : 0;
     const half_t* row = a.Q + (static_cast<int64_t>(b0 + beam[rt]) * a.heads + hk * g + (have - beam[rt] * g)) * a.d;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) q[rt][ks] = load_query<DP>(row, ks, quarter, a.d, a.sign);
+    for (int ks = 0; ks < KS; ++ks) q[rt][ks] = channels_of<DP>(row, ks, quarter, a.d) * a.sign;
     row_len[rt] = length_of(a, b0 + beam[rt]);
   }
   // lengths of the sequences (GROUP: lane i & 31 holds sequence i's), the longest and the shortest
   const unsigned my_len = GROUP ? ((lane & 31) < nb ? length_of(a, b0 + (lane & 31)) : 0u) : length_of(a, b0);
   const unsigned longest = GROUP ? static_cast<unsigned>(wave_most(static_cast<int>(my_len))) : static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(my_len)));
   const unsigned shortest = GROUP ? 0x7fffffffu - static_cast<unsigned>(wave_most((lane & 31) < nb ? static_cast<int>(0x7fffffffu - my_len) : 0)) : longest;
-  const unsigned blocks = (longest + 31) / 32, stride = static_cast<unsigned>(part.parts) * W;
   const unsigned everyone = nb >= 32 ? ~0u : (1u << nb) - 1u;
 
   // ---- where the next visit is
   const int* names = a.table + static_cast<int64_t>(b0) * a.columns;
-  auto place = [&](int page, unsigned in_page, const char*& k, const char*& v) {
-    const int64_t at = page * page_bytes + static_cast<int64_t>(in_page) * row_bytes;
-    k = Kh + at;
-    v = Vh + at;
+  auto place = [&](Visit& to, int h, int page, unsigned in_page, bool there) {
+    const unsigned pos = to.pos + 16 * h, rows = pos < longest ? longest - pos : 0u;
+    to.at[h] = page * page_bytes + static_cast<int64_t>(in_page) * row_bytes;
+    to.bytes[h] = there ? (rows < 16 ? rows : 16u) * row_bytes : 0u;
   };
-  unsigned blk = static_cast<unsigned>(wave) * part.parts + part.z;  // the block whose entries come next
+  // What the wavefronts take in turn: blocks; in a group a block that all share, and of the others (from about `common` on) a block for each sequence, which visits what that
+  // one names first.  So pieces of a group that has grown apart are as long as others.
+  int common = p_blocks, first = lo, last = hi;
+  if constexpr (GROUP) {
+    common = common_blocks(a, names, nb, my_len, longest, lane);
+    const int items = common + (p_blocks - common) * nb;
+    const float ratio = static_cast<float>(items) / static_cast<float>(p_blocks);
+    auto item_of = [&](int at) {
+      const int it = static_cast<int>(static_cast<float>(at) * ratio);
+      return at >= p_blocks || it > items ? items : it;
+    };
+    first = item_of(lo);
+    last = item_of(hi);
+  }
+  auto block_of = [&](int it, int& one) {
+    one = -1;
+    if (!GROUP || it < common) return it;
+    const unsigned q = static_cast<unsigned>(it - common), b = q / static_cast<unsigned>(nb);
+    one = static_cast<int>(q - b * nb);
+    return common + static_cast<int>(b);
+  };
+  int item = first + wave;  // the one whose entries come next
   // GROUP: a block's entries, lane (half, sequence); else those of 32 of the wavefront's blocks, lane (block, half)
-  auto gather = [&](unsigned at, int& entry, unsigned& in_page) {
-    const unsigned pos = GROUP ? at * 32 + (lane >> 5) * 16 : (at + (lane >> 1) * stride) * 32 + (lane & 1) * 16;
+  auto gather = [&](int at, int& entry, unsigned& in_page) {
+    int one;
+    const unsigned pos = GROUP ? static_cast<unsigned>(block_of(at, one)) * 32 + (lane >> 5) * 16 : static_cast<unsigned>(at + (lane >> 1) * W) * 32 + (lane & 1) * 16;
     const unsigned column = pos / a.page;
     in_page = pos - column * a.page;
     entry = pos < my_len && (!GROUP || (lane & 31) < nb) ? names[(GROUP ? static_cast<int64_t>(lane & 31) * a.columns : 0) + column] : -1;
@@ -325,23 +386,35 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
   int entry, entry_next;
   unsigned in_page, in_page_next, left[2] = {0, 0}, pos_now = 0;
   int taken = 0;  // (of the 32 blocks)
-  gather(blk, entry, in_page);
-  gather(blk + (GROUP ? stride : 32 * stride), entry_next, in_page_next);
+  gather(item, entry, in_page);
+  gather(item + (GROUP ? W : 32 * W), entry_next, in_page_next);
   auto advance = [&](Visit& to) -> bool {
     if constexpr (GROUP) {
       while ((left[0] | left[1]) == 0) {
-        if (blk >= blocks) return false;
-        if (taken != 0) {  // (the first block's entries are there)
+        if (item >= last) {
+          to.bytes[0] = to.bytes[1] = 0;
+          return false;
+        }
+        if (taken != 0) {  // (the first one's entries are there)
           entry = entry_next;
           in_page = in_page_next;
-          gather(blk + stride, entry_next, in_page_next);
+          gather(item + W, entry_next, in_page_next);
         }
         taken = 1;
-        pos_now = blk * 32;
-        blk += stride;
+        int one;
+        pos_now = static_cast<unsigned>(block_of(item, one)) * 32;
+        item += W;
         const uint64_t some = __builtin_amdgcn_ballot_w64(static_cast<unsigned>(entry) < static_cast<unsigned>(a.pages));
         left[0] = static_cast<unsigned>(some);
         left[1] = static_cast<unsigned>(some >> 32);
+        if (one >= 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int page = __builtin_amdgcn_readlane(entry, one + 32 * h);
+            const unsigned same = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(entry == page) >> (32 * h)) & left[h];
+            left[h] = ((same >> one) & 1) != 0 && __builtin_ctz(same) == one ? same : 0u;
+          }
+        }
       }
       to.pos = pos_now;
       int page[2] = {0, 0};
@@ -354,61 +427,87 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
           left[h] &= ~to.seen[h];
         }
       }
-      // (a half that nobody sees here is read from the other's page)
-      if (to.seen[0] == 0) page[0] = page[1];
-      if (to.seen[1] == 0) page[1] = page[0];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) place(page[h], static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(in_page), 32 * h)), to.k[h], to.v[h]);
+      for (int h = 0; h < 2; ++h) place(to, h, page[h], static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(in_page), 32 * h)), to.seen[h] != 0);
     } else {
-      if (blk >= blocks) return false;
+      if (item >= last) {
+        to.bytes[0] = to.bytes[1] = 0;
+        return false;
+      }
       if (taken == 32) {
         entry = entry_next;
         in_page = in_page_next;
-        gather(blk + 32 * stride, entry_next, in_page_next);
+        gather(item + 32 * W, entry_next, in_page_next);
         taken = 0;
       }
-      to.pos = blk * 32;
+      to.pos = static_cast<unsigned>(item) * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int page = __builtin_amdgcn_readlane(entry, 2 * taken + h);
         const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages);
         to.seen[h] = there ? 1u : 0u;
-        place(there ? page : 0, static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(in_page), 2 * taken + h)), to.k[h], to.v[h]);
+        place(to, h, there ? page : 0, static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(in_page), 2 * taken + h)), there);
       }
       ++taken;
-      blk += stride;
+      item += W;
     }
     return true;
   };
 
-  // ---- a lane's pieces of K and V
+  // ---- a lane's pieces of K and V.  As the matrix cores take K, a load would touch 64 bytes of each of sixteen keys; two loads that make up a line fetch it whole for
+  // eight keys each instead, and a rotation within sixteen lanes puts the pieces where they belong
   f16x8 kf[2][KS];
   u32x4 vf[VL];
   unsigned k_at[KS], v_at[VH];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    const int at = ks * 32 + quarter * 8;
-    k_at[ks] = i16 * row_bytes + 2u * (at < a.d ? at : a.d - 8);
+    const bool pair = ks / 2 * 2 + 1 < KS;
+    const int row = pair ? (lane & 7) + 8 * (ks & 1) : i16, at = pair ? ks / 2 * 64 + (lane >> 3) * 8 : channels_at<DP>(ks, quarter);
+    k_at[ks] = at < a.d ? row * row_bytes + 2u * at : kOob;
   }
 #pragma unroll
   for (int n = 0; n < VH; ++n) {
     const int id = n * 64 + lane, c = id % kChunks;
-    v_at[n] = id / kChunks * row_bytes + 16u * (c * 8 < a.d ? c : a.d / 8 - 1);
+    v_at[n] = c * 8 < a.d ? id / kChunks * row_bytes + 16u * c : kOob;
   }
   auto load_k = [&](const Visit& from) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < 2; ++kt) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(Kh + from.at[kt], from.bytes[kt]);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = *reinterpret_cast<const f16x8*>(from.k[kt] + k_at[ks]);
+      for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(r, k_at[ks], 0, kStreamed));
+    }
+  };
+  auto settle_k = [&] {  // piece (load n, bit 3 of the lane = x) -> (step x, bit 3 = n)
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int ks = 0; ks + 1 < KS; ks += 2) {
+        u32x4 even = __builtin_bit_cast(u32x4, kf[kt][ks]), odd = __builtin_bit_cast(u32x4, kf[kt][ks + 1]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int x = static_cast<int>(even[w]), y = static_cast<int>(odd[w]);
+          even[w] = static_cast<unsigned>(__builtin_amdgcn_update_dpp(x, y, 0x128, 0xf, 0xc, false));  // row_ror:8 into lanes 8 .. 15 of a row
+          odd[w] = static_cast<unsigned>(__builtin_amdgcn_update_dpp(y, x, 0x128, 0xf, 0x3, false));   // ... 0 .. 7
+        }
+        kf[kt][ks] = __builtin_bit_cast(f16x8, even);
+        kf[kt][ks + 1] = __builtin_bit_cast(f16x8, odd);
+      }
+    }
   };
   auto load_v = [&](const Visit& from) {
 #pragma unroll
-    for (int n = 0; n < VL; ++n) vf[n] = *reinterpret_cast<const u32x4*>(from.v[n / VH] + v_at[n % VH]);
+    for (int h = 0; h < 2; ++h) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(Vh + from.at[h], from.bytes[h]);
+#pragma unroll
+      for (int n = 0; n < VH; ++n) vf[h * VH + n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v_at[n], 0, kStreamed));
+    }
   };
 
   f32x4 o[RT][DT];
   float top[RT], sum[RT];
   bool saw[RT];
+  unsigned taken_out = 0;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     top[rt] = -INFINITY;
@@ -417,17 +516,11 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  char* mine = lds + wave * kWave;
-  const unsigned tr_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)mine)) +
-                         (4 * quarter + (i16 >> 2)) * v_row_bytes(DP) + (i16 & 3) * 8;
 
-  auto visit = [&](const Visit& here, bool more, const Visit& next) {
+  // (the next one's loads are not behind a branch, behind which the compiler would wait for them whenever it waits for an earlier one: the last visit's next has no bytes)
+  auto visit = [&](const Visit& here, const Visit& next) {
     f32x4 s[RT][2];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        if (ks * 32 + 32 > below(DP) && ks * 32 + quarter * 8 >= a.d) kf[kt][ks] = f16x8{};
+    settle_k();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -436,10 +529,9 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][ks], q[rt][ks], s[rt][kt], 0, 0, 0);
       }
-    if (more) load_k(next);
+    load_k(next);
     const bool all = here.seen[0] == everyone && here.seen[1] == everyone && here.pos + 32 <= shortest;
     unsigned shown[RT];
-    bool odd = false;
     if (!all) {
       unsigned any = 0;
 #pragma unroll
@@ -449,15 +541,19 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
         saw[rt] = saw[rt] || shown[rt] != 0;
         any |= shown[rt];
       }
-      any = any_row(any);
-      // values that nobody sees would meet weights of zero, and may be no numbers
+      if constexpr (GROUP) {
+        // values that nobody sees, or only some rows, would meet weights of zero: the former go, and of the latter what is no number (rare), which is added at the end
+        any = any_row(any);
 #pragma unroll
-      for (int n = 0; n < VL; ++n)
-        if (!((any >> ((n * 64 + lane) / kChunks)) & 1)) vf[n] = u32x4{0u, 0u, 0u, 0u};
-      if constexpr (GROUP) {  // nor must those that only some rows see
+        for (int n = 0; n < VL; ++n) {
+          const bool there = ((any >> ((n * 64 + lane) / kChunks)) & 1) != 0;
 #pragma unroll
-        for (int n = 0; n < VL; ++n) odd = odd || no_number(vf[n]);
-        odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+          for (int w = 0; w < 4; ++w) {
+            const unsigned low = vf[n][w] & 0x7c00u, high = vf[n][w] & 0x7c000000u, gone = (low == 0x7c00u ? 0xffffu : 0u) | (high == 0x7c000000u ? 0xffff0000u : 0u);
+            taken_out |= there ? gone : 0u;
+            vf[n][w] = there ? vf[n][w] & ~gone : 0u;
+          }
+        }
       }
     } else {
 #pragma unroll
@@ -466,42 +562,18 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
         saw[rt] = true;
       }
     }
-    if (!GROUP || !odd) {
 #pragma unroll
-      for (int n = 0; n < VL; ++n) {
-        const int id = n * 64 + lane, row = id / kChunks, c = id % kChunks;
-        *reinterpret_cast<u32x4*>(mine + row * v_row_bytes(DP) + c * 16) = vf[n];
-      }
+    for (int n = 0; n < VL; ++n) {
+      const int id = n * 64 + lane, row = id / kChunks, c = id % kChunks;
+      *reinterpret_cast<u32x4*>(mine + row * v_row_bytes(DP) + c * 16) = vf[n];
     }
-    if (more) load_v(next);
+    load_v(next);
     f16x8 p[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       weigh<2, DT>(s[rt], all, shown[rt], quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
       p[rt] = weights_f16(s[rt][0], s[rt][1]);
-      if (GROUP && odd) {  // (rare) key by key, a row adding up what it sees
-        float* room = reinterpret_cast<float*>(mine);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          room[(4 * quarter + j) * 16 + i16] = s[rt][0][j];
-          room[(16 + 4 * quarter + j) * 16 + i16] = s[rt][1][j];
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        for (int key = 0; key < 32; ++key) {
-          const float weight = room[key * 16 + i16];
-          const half_t* v = reinterpret_cast<const half_t*>((key < 16 ? here.v[0] : here.v[1]) + (key & 15) * row_bytes);
-          if ((shown[rt] >> key) & 1) {
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (dt * 16 + 4 * quarter < a.d) o[rt][dt][j] = fmaf(weight, static_cast<float>(v[dt * 16 + 4 * quarter + j]), o[rt][dt][j]);
-          }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
     }
-    if (GROUP && odd) return;
     auto add = [&](int dt, const f16x4& lo, const f16x4& hi) {
       const f16x8 vt = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
@@ -529,7 +601,7 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
   }
   while (more) {
     more = advance(next);
-    visit(here, more, next);
+    visit(here, next);
     here = next;
   }
 
@@ -537,7 +609,7 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     sum[rt] = sum_of_row(sum[rt]);
-    sum_again<DP>(a, names, beam[rt], hk, row_len[rt], longest, static_cast<unsigned>(wave) * part.parts + part.z, stride, q[rt], top[rt], sum[rt], lane, o[rt]);
+    sum_again<DP>(a, names, b0, beam[rt], hk, row_len[rt], GROUP ? common : p_blocks, nb, first + wave, last, W, q[rt], top[rt], sum[rt], lane, taken_out != 0, o[rt]);
     if (quarter == 0) {
       stat_m[wave][rt * 16 + i16] = top[rt];
       stat_l[wave][rt * 16 + i16] = saw[rt] ? sum[rt] : -1.f;
@@ -551,9 +623,10 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
     return best;
   };
   const int my_rows = R - rg * kRows < kRows ? R - rg * kRows : kRows;
-  const int64_t problem = static_cast<int64_t>(hk) * grid.row_groups + rg;
-  float* shares = grid.ws + (problem * 2 * grid.extra + part.first) * kShare;
-  float* share = shares + static_cast<int64_t>(part.z) * kShare;
+  // a piece's sums: of the one that begins a problem among the last ones of the workgroups, of others among the first ones
+  float *firsts = grid.ws + kind * 2 * grid.shares * kShare, *lasts = firsts + static_cast<int64_t>(grid.shares) * kShare;
+  auto sums_of = [&](int y) { return y == 0 ? lasts + static_cast<int64_t>(first_cut - 1) * kShare : firsts + static_cast<int64_t>(first_cut - 1 + y) * kShare; };
+  float* handed = parts > 1 ? sums_of(z) : nullptr;
   auto out_row = [&](int r) {  // (of this workgroup's)
     const int at = rg * kRows + r, beam_of = GROUP ? at / g : 0;
     return a.out + (static_cast<int64_t>(b0 + beam_of) * a.heads + hk * g + (at - beam_of * g)) * a.d;
@@ -586,62 +659,111 @@ __global__ void __launch_bounds__(64 * W) attn_paged_kernel(PagedArgs a, PagedGr
         l += stat_l[w][r] * weight_of(stat_m[w][r], best, a.scale_log2);
         any = any || !(stat_l[w][r] < 0.f);
       }
-      if (part.parts > 1) {
-        store_out(v, reinterpret_cast<f32x4*>(share + r * DP + c), true);
-        if (c == 0) store_stat(share, kRows, DP, r, best, any ? l : -1.f);
+      if (parts > 1) {
+        store_out(v, reinterpret_cast<f32x4*>(handed + r * DP + c), true);
+        if (c == 0) store_stat(handed, kRows, DP, r, best, any ? l : -1.f);
       } else {
         store_row4(out_row(r) + c, v, any ? 1.f / l : 0.f);
       }
     }
     __syncthreads();
   }
-  if (part.parts == 1 || !last_to_arrive(grid.arrivals + problem * grid.problems + part.p, part.parts, &flag)) return;
+  if (parts == 1 || !last_to_arrive(grid.arrivals + kind * grid.problems + p, parts, &flag)) continue;
 
-  // ---- whoever is last joins the parts in their order
-  static_assert(128 / RT * kRows * 8 <= W * kWave, "the parts' statistics fit the LDS");
-  uint64_t* stats = reinterpret_cast<uint64_t*>(lds);
-  constexpr int kAtOnce = 8;  // parts requested before the first is used: a trip to memory per eight
-  uint64_t one[kAtOnce], other[kAtOnce];
+  // ---- whoever is last joins the parts in their order: a wavefront per row finds the parts' weights, then a thread has four channels of a row, of every S-th part
+  // where there are threads left
+  constexpr int kItems = DP / 4, kAtOnce = 8;  // parts requested before the first is used: a trip to memory per eight
+  const int items_all = my_rows * kItems;
+  int spread = 1;
+  while (spread * 2 * items_all <= 64 * W && spread < parts) spread *= 2;
+  const int lot = tid / items_all, mine_of = tid - lot * items_all;
+  f32x4 some[kAtOnce];
   auto request = [&](int at, int y0) {
-    const int i = at / (DP / 4), c = 4 * (at % (DP / 4));
+    const int offset = at / kItems * DP + 4 * (at % kItems);
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
-      const int y = y0 + u < part.parts ? y0 + u : part.parts - 1;
-      const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(y) * kShare + i * DP + c);
-      one[u] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      other[u] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int y = y0 + u * spread < parts ? y0 + u * spread : parts - 1;
+      const uint64_t* two = reinterpret_cast<const uint64_t*>(sums_of(y) + offset);
+      const uint64_t low = __hip_atomic_load(two, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), high = __hip_atomic_load(two + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      some[u] = f32x4{__builtin_bit_cast(float, static_cast<unsigned>(low)), __builtin_bit_cast(float, static_cast<unsigned>(low >> 32)),
+                      __builtin_bit_cast(float, static_cast<unsigned>(high)), __builtin_bit_cast(float, static_cast<unsigned>(high >> 32))};
     }
   };
-  const int last = my_rows * (DP / 4);
-  if (tid < last) request(tid, 0);  // (on their way while the statistics come)
-  for (int at = tid; at < part.parts * kRows; at += 64 * W)
-    if (at % kRows < my_rows)
-      stats[at] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(shares + static_cast<int64_t>(at / kRows) * kShare + kRows * DP) + at % kRows, __ATOMIC_RELAXED,
-                                    __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  for (int at = tid; at < last; at += 64 * W) {
-    const int i = at / (DP / 4), c = 4 * (at % (DP / 4));
-    if (at != tid) request(at, 0);
-    float best = -INFINITY, l = 0.f;
+  if (lot < spread) request(mine_of, lot);  // (on their way while the statistics come)
+  constexpr int kMost = most_shares(RT);
+  float* weights = reinterpret_cast<float*>(lds);  // [row][part]
+  static_assert(kRows * kMost * 4 + 64 * W * 16 <= W * kWave, "the parts' weights and the threads' sums fit the LDS");
+  for (int i = wave; i < my_rows; i += W) {
+    float tops[kMost / 64], sums[kMost / 64], best = -INFINITY, total = 0.f;
     bool any = false;
-    for (int y = 0; y < part.parts; ++y) best = fmaxf(best, __builtin_bit_cast(float, static_cast<unsigned>(stats[y * kRows + i])));
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int y0 = 0; y0 < part.parts; y0 += kAtOnce) {
-      if (y0 > 0) request(at, y0);
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        if (y0 + u >= part.parts) break;
-        const uint64_t two = stats[(y0 + u) * kRows + i];
-        const float w = weight_of(__builtin_bit_cast(float, static_cast<unsigned>(two)), best, a.scale_log2), theirs = __builtin_bit_cast(float, static_cast<unsigned>(two >> 32));
-        any = any || !(theirs < 0.f);
-        l = fmaf(w, theirs, l);
-        v[0] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u])), v[0]);
-        v[1] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(one[u] >> 32)), v[1]);
-        v[2] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u])), v[2]);
-        v[3] = fmaf(w, __builtin_bit_cast(float, static_cast<unsigned>(other[u] >> 32)), v[3]);
+    for (int c = 0; c < kMost / 64; ++c) {
+      const int y = c * 64 + lane;
+      uint64_t two = pair_of(-INFINITY, -1.f);
+      if (y < parts) two = __hip_atomic_load(reinterpret_cast<const uint64_t*>(sums_of(y) + kRows * DP) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      tops[c] = __builtin_bit_cast(float, static_cast<unsigned>(two));
+      sums[c] = __builtin_bit_cast(float, static_cast<unsigned>(two >> 32));
+      any = any || !(sums[c] < 0.f);
+      best = fmaxf(best, tops[c]);
+    }
+    best = wave_max(best);
+#pragma unroll
+    for (int c = 0; c < kMost / 64; ++c) {
+      tops[c] = weight_of(tops[c], best, a.scale_log2);
+      total = fmaf(tops[c], sums[c], total);
+    }
+    total = wave_sum(total);
+    const float inv = __builtin_amdgcn_ballot_w64(any) != 0 ? 1.f / total : 0.f;
+#pragma unroll
+    for (int c = 0; c < kMost / 64; ++c)
+      if (c * 64 + lane < parts) weights[i * kMost + c * 64 + lane] = tops[c] * inv;
+  }
+  __syncthreads();
+  if (spread > 1) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (lot < spread) {
+      const float* w = weights + mine_of / kItems * kMost;
+      for (int y0 = lot; y0 < parts; y0 += kAtOnce * spread) {
+        if (y0 != lot) request(mine_of, y0);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int y = y0 + u * spread;
+          if (y >= parts) break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = fmaf(w[y], some[u][j], v[j]);
+        }
       }
     }
-    if (c < a.d) store_row4(out_row(i) + c, v, any ? 1.f / l : 0.f);
+    f32x4* sums = reinterpret_cast<f32x4*>(lds + kRows * kMost * 4);
+    sums[tid] = v;
+    __syncthreads();
+    if (lot == 0) {
+      for (int s = 1; s < spread; ++s) {
+        const f32x4 one = sums[s * items_all + mine_of];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += one[j];
+      }
+      const int c = 4 * (mine_of % kItems);
+      if (c < a.d) store_row4(out_row(mine_of / kItems) + c, v, 1.f);
+    }
+  } else {
+    for (int at = tid; at < items_all; at += 64 * W) {
+      const float* w = weights + at / kItems * kMost;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int y0 = 0; y0 < parts; y0 += kAtOnce) {
+        if (y0 > 0 || at != tid) request(at, y0);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          if (y0 + u >= parts) break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = fmaf(w[y0 + u], some[u][j], v[j]);
+        }
+      }
+      const int c = 4 * (at % kItems);
+      if (c < a.d) store_row4(out_row(at / kItems) + c, v, 1.f);
+    }
+  }
+  __syncthreads();  // (the LDS is the next problem's)
   }
 }
 
@@ -654,38 +776,38 @@ int launch_paged(const PagedArgs& a, int64_t batch, int beams, int sub, hipStrea
   grid.subs = static_cast<int>(ceil_div(grid.beams, grid.sub));
   const int64_t problems = batch / grid.beams * grid.subs;
   grid.row_groups = GROUP ? 1 : static_cast<int>(ceil_div(g, 16 * RT));
-  const int64_t kinds = a.kv_heads * static_cast<int64_t>(grid.row_groups), blocks = ceil_div(a.room, 32);
-  grid.least = W;
-  grid.most = 128 / RT;
-  grid.whole = 1.f;
-  constexpr int64_t kParts = 512;
-  int64_t extra = ceil_div(kParts, kinds);
-  if (blocks <= grid.least) extra = 0;  // (nothing that could be cut)
-  grid.extra = static_cast<int>(extra);
-  const int64_t slots = problems + extra;
-  if (slots > INT32_MAX / kinds) return fail("attn_paged: the launch has too many workgroups");
+  const int64_t kinds = a.kv_heads * static_cast<int64_t>(grid.row_groups), blocks = a.room < 32 ? 1 : ceil_div(a.room, 32);
+  if (problems > INT32_MAX / blocks) return fail("attn_paged: the tables hold too many positions");
   grid.problems = static_cast<int>(problems);
-  grid.slots = static_cast<int>(slots);
+  grid.least = W;
+  constexpr int64_t kWorkgroups = 256;
+  int64_t shares = kinds < kWorkgroups ? kWorkgroups / kinds : 1;
+  shares = shares < most_shares(RT) ? shares : most_shares(RT);
+  grid.shares = static_cast<int>(shares);
   std::unique_lock<std::recursive_mutex> lock;
-  if (extra > 0 && split_scratch(s, static_cast<size_t>(kinds * 2 * extra) * 16 * RT * (DP + 2) * sizeof(float), static_cast<size_t>(kinds * problems), static_cast<int>(extra),
-                                 &grid.ws, &grid.arrivals, &lock) != 0)
+  if (shares > 1 && split_scratch(s, static_cast<size_t>(kinds * 2 * shares) * 16 * RT * (DP + 2) * sizeof(float), static_cast<size_t>(kinds * problems), static_cast<int>(shares),
+                                  &grid.ws, &grid.arrivals, &lock) != 0)
     return -1;
-  hipLaunchKernelGGL((attn_paged_kernel<DP, RT, W, GROUP>), dim3(static_cast<unsigned>(kinds * slots)), dim3(64 * W), 0, s, a, grid);
+  hipLaunchKernelGGL((attn_paged_kernel<DP, RT, W, GROUP>), dim3(static_cast<unsigned>(kinds * shares)), dim3(64 * W), 0, s, a, grid);
   return check_launch("attn_paged");
 }
 template <int DP>
 int launch_paged_rows(const PagedArgs& a, int64_t batch, int beams, hipStream_t s) {
-  constexpr int W = DP <= 128 ? 8 : 4;
   const int g = a.heads / a.kv_heads;
-  // a problem holds as many sequences of a group as 32 rows do
-  if (beams > 1 && g <= 16) {
-    int sub = 32 / g;
-    sub = sub > beams ? beams : sub;
-    if (sub * g <= 16) return launch_paged<DP, 1, W, true>(a, batch, beams, sub, s);
-    return launch_paged<DP, 2, W, true>(a, batch, beams, sub, s);
+  // 32 rows at a time where their sums and the queries leave room for the keys (heads of up to 128), 16 beyond.  A problem holds as many sequences of a group as that; with
+  // heads of more than 128 the sequences of a group are read one by one.
+  if constexpr (DP <= 128) {
+    if (beams > 1 && g <= 16) {
+      int sub = 32 / g;
+      sub = sub > beams ? beams : sub;
+      if (sub * g <= 16) return launch_paged<DP, 1, 8, true>(a, batch, beams, sub, s);
+      return launch_paged<DP, 2, 4, true>(a, batch, beams, sub, s);
+    }
+    if (g <= 16) return launch_paged<DP, 1, 8, false>(a, batch, beams, 1, s);
+    return launch_paged<DP, 2, 4, false>(a, batch, beams, 1, s);
+  } else {
+    return launch_paged<DP, 1, 4, false>(a, batch, beams, 1, s);
   }
-  if (g <= 16) return launch_paged<DP, 1, W, false>(a, batch, beams, 1, s);
-  return launch_paged<DP, 2, W, false>(a, batch, beams, 1, s);
 }
 
 }  // namespace
