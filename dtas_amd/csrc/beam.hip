@@ -3,11 +3,11 @@
 //   candidate (w, v) of a group: scores[w] + logits[w][v] - log sum_u exp(logits[w][u]); of a beam that is done: (w, eos) with scores[w]
 //   the `beams` best, by (score descending, w, v ascending); what is no finite number counts as -inf
 //
-// Within a beam the order is that of the logits, so one pass over them is enough: a workgroup has a piece of one beam's logits in registers, and leaves
-// its maximum, its sum of exponentials (terms in 32 bits, each product with log2 e kept to twice that; the sum in 64) and its best candidates in their order; whoever is
-// last among a group's workgroups has the sums of all and compares what is left, in 64 bits.
-// Both times the best W of many are found without sorting them: every lane has the best of its own, the W-th best of these in a wavefront is as good as W of all at least, so only
-// what is not below that (the best of the wavefronts') can be among the W; these few are counted out against each other.
+// Within a beam the order is that of the logits, so one pass over them is enough: a workgroup goes through a part of one beam's logits and keeps its maximum, its sum of
+// exponentials (terms in 32 bits, each product with log2 e kept to twice that; the sum in 64) and its W best so far; whoever is last among a group's workgroups has the
+// sums of all and compares what is left, in 64 bits.
+// The W best of many are found without sorting them: every lane has the best of its own, the W-th best of these in a wavefront is as good as W of all at least, so only what is not
+// below that can be among the W.  These few are counted out against each other; behind the first piece of a part only what beats the W-th best so far is left.
 #include "gemm_common.h"
 
 namespace dtas {
@@ -19,7 +19,7 @@ struct BeamArgs {
   int *tokens, *parents;
   float* new_scores;
   int* new_done;
-  int beams, parts;
+  int beams, parts, per;  // logits per part, a multiple of 4
   int64_t V, eos;
   uint64_t* room;      // [groups][beams][parts][2 + beams]: maximum and number of candidates, sum, candidates (logit, token)
   unsigned* arrivals;  // [groups]
@@ -32,15 +32,21 @@ __device__ __forceinline__ uint64_t pair_of(float x, unsigned y) { return static
 __device__ __forceinline__ float first_of(uint64_t v) { return __builtin_bit_cast(float, static_cast<unsigned>(v)); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
-constexpr int kBeamThreads = 256, kBeamWaves = kBeamThreads / 64;
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 
-// exp(x - m) for x <= m: the exponent as the rounded product with log2 e and what that rounding left
+constexpr int kBeamThreads = 512, kBeamWaves = kBeamThreads / 64;
+
+// exp(x - m) for x <= m, nought for -inf and for what is no number: the exponent as the rounded product with log2 e and what that rounding left
 __device__ __forceinline__ float exp_below(float x, float m) {
   constexpr float kHigh = 1.44269502f, kLow = 1.92596299e-8f, kLn2 = 0.693147182f;
-  const float d = x - m, t = d * kHigh;
-  if (!(t > -200.f)) return x == x ? 0.f : x;  // (that is nothing next to the maximum's 1; what is no number stays none)
-  const float e = __builtin_amdgcn_exp2f(t), r = fmaf(d, kHigh, -t) + d * kLow;
+  const float d = fmaxf(x - m, -150.f), t = d * kHigh;
+  const float e = __builtin_amdgcn_exp2f(t), r = fmaf(d, kLow, fmaf(d, kHigh, -t));
   return fmaf(e, r * kLn2, e);
+}
+// the next number below (-inf: itself)
+__device__ __forceinline__ float below_of(float v) {
+  const int bits = __builtin_bit_cast(int, v);
+  return v == -INFINITY ? v : v == 0.f ? -__builtin_bit_cast(float, 1) : __builtin_bit_cast(float, v > 0.f ? bits - 1 : bits + 1);
 }
 
 // sums over the lanes whose numbers agree but for the bits below `width` (a power of two up to 64)
@@ -52,32 +58,12 @@ __device__ __forceinline__ float max_over(float v, int width) {
   for (int k = 1; k < width; k *= 2) v = fmaxf(v, __shfl_xor(v, k));
   return v;
 }
-// The W-th largest of the lanes' values
-__device__ __forceinline__ float nth_in_wave(float v, int W, int lane) {
+// The W-th largest of the lanes' values: the least of those that fewer than W are above
+__device__ __forceinline__ float nth_in_wave(float v, int W) {
   int above = 0;
 #pragma unroll 16
-  for (int i = 0; i < 64; ++i) {
-    const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));
-    above += o > v || (o == v && i < lane) ? 1 : 0;
-  }
-  const uint64_t at = __builtin_amdgcn_ballot_w64(above == W - 1);
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at ? __builtin_ctzll(at) : 0));
-}
-__device__ __forceinline__ double nth_in_wave(double v, int W, int lane) {
-  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
-  const int low = static_cast<int>(bits), high = static_cast<int>(bits >> 32);
-  auto lane_of = [&](int i) {
-    const unsigned l = __builtin_amdgcn_readlane(low, i), h = __builtin_amdgcn_readlane(high, i);
-    return __builtin_bit_cast(double, static_cast<uint64_t>(h) << 32 | l);
-  };
-  int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < 64; ++i) {
-    const double o = lane_of(i);
-    above += o > v || (o == v && i < lane) ? 1 : 0;
-  }
-  const uint64_t at = __builtin_amdgcn_ballot_w64(above == W - 1);
-  return lane_of(at ? __builtin_ctzll(at) : 0);
+  for (int i = 0; i < 64; ++i) above += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)) > v ? 1 : 0;
+  return -wave_max(above < W ? -v : -INFINITY);
 }
 
 // A candidate's place in the order: score, then the beam, then the logit, then the token (of one beam's candidates the sum may be the same where the logits are not)
@@ -112,136 +98,232 @@ __device__ Key first_in_block(Key k, Key* slots) {
 }
 
 constexpr int kFew = 1024, kFewKeys = 512;  // candidates that are counted out; more (many equal ones, hardly any numbers) are taken one after the other
+constexpr int kPieces = 4, kPiece = kBeamThreads * 4 * kPieces;  // 16 logits per thread at a time
 
-template <int U>  // 16-byte pieces per thread
 __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   union Lds {
-    struct { float logit[kFew]; int at[kFew]; } piece;
-    struct { double score[kFewKeys]; float logit[kFewKeys]; int beam[kFewKeys], token[kFewKeys]; } all;
+    struct { __attribute__((aligned(16))) float logit[kFew]; int at[kFew]; } piece;
+    struct { __attribute__((aligned(32))) double score[kFewKeys]; float logit[kFewKeys]; int beam[kFewKeys], token[kFewKeys]; } all;
   };
   __shared__ Lds few;
   __shared__ Key slots[kBeamWaves];
-  __shared__ float tops[kBeamWaves], bounds[kBeamWaves];
-  __shared__ double sums[kBeamWaves], key_bounds[kBeamWaves];
-  __shared__ double log_sum[DTAS_MAX_BEAMS];
-  __shared__ float top_of[DTAS_MAX_BEAMS], chosen_score[DTAS_MAX_BEAMS];
+  __shared__ float tops[kBeamWaves], bounds[kBeamWaves], best_logit[2][DTAS_MAX_BEAMS];
+  __shared__ int best_at[2][DTAS_MAX_BEAMS];
+  __shared__ double sums[kBeamWaves], log_sum[DTAS_MAX_BEAMS], stat_s[kBeamThreads];
+  __shared__ float top_of[DTAS_MAX_BEAMS], chosen_score[DTAS_MAX_BEAMS], stat_m[kBeamThreads];
   __shared__ int chosen_beam[DTAS_MAX_BEAMS], chosen_token[DTAS_MAX_BEAMS];
-  __shared__ int flag, count;
-  constexpr int kPiece = kBeamThreads * 4 * U;
+  __shared__ int flag, counts[2];  // (of one piece and of the next: a wavefront may be that far ahead of another)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x, w = blockIdx.y, W = a.beams;
-  const int64_t g = blockIdx.z, from = static_cast<int64_t>(part) * kPiece;
-  const int here = static_cast<int>(a.V - from < kPiece ? a.V - from : kPiece), stride = 2 + W;
+  const int64_t g = blockIdx.z, from = static_cast<int64_t>(part) * a.per;
+  const int here = static_cast<int>(a.V - from < a.per ? a.V - from : a.per), stride = 2 + W;
   const bool plain = finite(a.scores[g * W + w]) && !(a.done && a.done[g * W + w] != 0);
+  auto most = [&](const float* of) {
+    float v = of[0];
+#pragma unroll
+    for (int i = 1; i < kBeamWaves; ++i) v = fmaxf(v, of[i]);
+    return v;
+  };
   if (plain) {
     const float* row = a.logits + (g * W + w) * a.V + from;
-    float x[U][4];
+    float x[kPieces][4], y[kPieces][4];
+    auto load = [&](float (&to)[kPieces][4], int base) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = u * kBeamThreads * 4 + tid * 4;
-      if (i + 4 <= here) {
-        f32x4 v;  // (rows of an odd vocabulary begin off 16 bytes)
-        __builtin_memcpy(&v, __builtin_assume_aligned(row + i, 4), 16);
+      for (int u = 0; u < kPieces; ++u) {
+        const int i = base + u * kBeamThreads * 4 + tid * 4;
+        if (i + 4 <= here) {
+          f32x4 v;  // (rows of an odd vocabulary begin off 16 bytes)
+          __builtin_memcpy(&v, __builtin_assume_aligned(row + i, 4), 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[u][j] = v[j];
-      } else {
+          for (int j = 0; j < 4; ++j) to[u][j] = v[j];
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[u][j] = i + j < here ? row[i + j] : -INFINITY;
+          for (int j = 0; j < 4; ++j) to[u][j] = i + j < here ? row[i + j] : -INFINITY;
+        }
       }
-    }
-    if (tid == 0) count = 0;
-    float own = -INFINITY;
+    };
+    load(x, 0);
+    if (tid < 2) counts[tid] = 0;
+    int have = 0, side = 0;  // (of the best so far, in best_logit[side])
+    float limit = -INFINITY, m = -INFINITY;
+    double s = 0.0;
+    bool strange = false;
+    for (int base = 0, turn = 0; base < here; base += kPiece, turn ^= 1) {
+      if (base + kPiece < here) load(y, base + kPiece);
+      float own = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) own = fmaxf(own, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
-    const float wave_top = wave_max(own), bound = nth_in_wave(own, W, lane);
-    if (lane == 0) {
-      tops[wave] = wave_top;
-      bounds[wave] = bound;
-    }
-    __syncthreads();
-    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), least = fmaxf(fmaxf(bounds[0], bounds[1]), fmaxf(bounds[2], bounds[3]));
-    double sum = 0.0;
+      for (int u = 0; u < kPieces; ++u) own = fmaxf(own, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
+      if (have < W) {
+        const float bound = nth_in_wave(own, W);
+        if (lane == 0) bounds[wave] = bound;
+        __syncthreads();
+        limit = most(bounds);
+      }
+      const float wave_top = wave_max(own);
+      if (wave_top > m) {
+        s = m == -INFINITY ? 0.0 : s * exp(static_cast<double>(m) - static_cast<double>(wave_top));
+        m = wave_top;
+      }
+      float terms[kPieces];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < kPieces; ++u) {
+        terms[u] = (exp_below(x[u][0], m) + exp_below(x[u][1], m)) + (exp_below(x[u][2], m) + exp_below(x[u][3], m));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (x[u][j] >= least && finite(x[u][j])) {
-          const int n = atomicAdd(&count, 1);
-          if (n < kFew) {
-            few.piece.logit[n] = x[u][j];
-            few.piece.at[n] = u * kBeamThreads * 4 + tid * 4 + j;
+        for (int j = 0; j < 4; ++j) strange = strange || x[u][j] != x[u][j];
+      }
+      s += (terms[0] + terms[1]) + (terms[2] + terms[3]);
+      // (an equal one behind the best so far is no better)
+      const float above = have == W ? limit : below_of(limit);
+      if (own > above) {
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (x[u][j] > above) {
+              const int n = atomicAdd(&counts[turn], 1);
+              if (n < kFew) {
+                few.piece.logit[n] = x[u][j];
+                few.piece.at[n] = base + u * kBeamThreads * 4 + tid * 4 + j;
+              }
+            }
+      }
+      __syncthreads();
+      const int n = counts[turn];
+      if (n > 0) {
+        const int old = have;
+        const float* old_logit = best_logit[side];
+        const int* old_at = best_at[side];
+        side ^= 1;
+        if (n <= kFew) {
+          have = old + n < W ? old + n : W;
+          for (int i = tid; i < n + old; i += kBeamThreads) {
+            const float mine = i < n ? few.piece.logit[i] : old_logit[i - n];
+            const int at = i < n ? few.piece.at[i] : old_at[i - n];
+            int rank = 0, level = 0;
+            for (int k = 0; k < n; k += 4) {
+              const f32x4 some = *reinterpret_cast<const f32x4*>(few.piece.logit + k);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const bool in = k + j < n;
+                rank += in && some[j] > mine ? 1 : 0;
+                level += in && some[j] == mine ? 1 : 0;
+              }
+            }
+            if (level > (i < n ? 1 : 0))  // (equal ones go by their places)
+              for (int k = 0; k < n; ++k) rank += few.piece.logit[k] == mine && few.piece.at[k] < at ? 1 : 0;
+            for (int k = 0; k < old; ++k) rank += old_logit[k] > mine || (old_logit[k] == mine && old_at[k] < at) ? 1 : 0;
+            if (rank < W) {
+              best_logit[side][rank] = mine;
+              best_at[side][rank] = at;
+            }
+          }
+        } else {
+          float last = INFINITY;
+          int last_at = -1;
+          for (have = 0; have < W; ++have) {
+            Key best = no_key();
+            auto offer = [&](float logit, int at) {
+              const Key k{0.0, logit, 0, at};
+              if (finite(logit) && (logit < last || (logit == last && at > last_at)) && before(k, best)) best = k;
+            };
+#pragma unroll
+            for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) offer(x[u][j], base + u * kBeamThreads * 4 + tid * 4 + j);
+            if (tid < old) offer(old_logit[tid], old_at[tid]);
+            best = first_in_block(best, slots);
+            if (best.token == INT32_MAX) break;
+            last = best.logit;
+            last_at = best.token;
+            if (tid == 0) {
+              best_logit[side][have] = last;
+              best_at[side][have] = last_at;
+            }
           }
         }
-        sum += x[u][j] == -INFINITY ? 0.f : exp_below(x[u][j], top);
+        __syncthreads();
+        if (tid == 0) counts[turn] = 0;
+        if (have == W) limit = best_logit[side][W - 1];
+        __syncthreads();
       }
-    sum = sum_over(sum, 64);
-    if (lane == 0) sums[wave] = sum;
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u][j] = y[u][j];
+    }
+    if (lane == 0) tops[wave] = m;
+    __syncthreads();
+    const float top = most(tops);
+    s = sum_over(s, 64);
+    if (m != -INFINITY) s *= exp(static_cast<double>(m) - static_cast<double>(top));
+    if (__builtin_amdgcn_ballot_w64(strange) != 0) s = __builtin_nan("");
+    if (lane == 0) sums[wave] = s;
     __syncthreads();
     uint64_t* room = a.room + ((g * W + w) * a.parts + part) * stride;
-    const int n = count;
-    int found = n < W ? n : W;
-    if (n <= kFew) {
-      for (int i = tid; i < n; i += kBeamThreads) {
-        const float mine = few.piece.logit[i];
-        const int at = few.piece.at[i];
-        int rank = 0;
-        for (int k = 0; k < n; ++k) rank += few.piece.logit[k] > mine || (few.piece.logit[k] == mine && few.piece.at[k] < at) ? 1 : 0;
-        if (rank < W) put(room + 2 + rank, pair_of(mine, static_cast<unsigned>(from + at)));
-      }
-    } else {
-      float last = INFINITY;
-      int last_at = -1;
-      for (found = 0; found < W; ++found) {
-        Key best = no_key();
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const Key k{0.0, x[u][j], 0, u * kBeamThreads * 4 + tid * 4 + j};
-            if (finite(k.logit) && (k.logit < last || (k.logit == last && k.token > last_at)) && before(k, best)) best = k;
-          }
-        best = first_in_block(best, slots);
-        if (best.token == INT32_MAX) break;
-        last = best.logit;
-        last_at = best.token;
-        if (tid == 0) put(room + 2 + found, pair_of(last, static_cast<unsigned>(from + last_at)));
-      }
-    }
+    if (tid < have) put(room + 2 + tid, pair_of(best_logit[side][tid], static_cast<unsigned>(from + best_at[side][tid])));
     if (tid == 0) {
-      put(room, pair_of(top, static_cast<unsigned>(found)));
-      put(room + 1, __builtin_bit_cast(uint64_t, ((sums[0] + sums[1]) + sums[2]) + sums[3]));
+      double all = sums[0];
+      for (int i = 1; i < kBeamWaves; ++i) all += sums[i];
+      put(room, pair_of(top, static_cast<unsigned>(have)));
+      put(room + 1, __builtin_bit_cast(uint64_t, all));
     }
   }
   // ---- whoever is last among the group's workgroups.  What they left passes the L2 (the XCDs' are not coherent); an arrival is counted once its own has drained
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) {
-    const unsigned arrived = __hip_atomic_fetch_add(a.arrivals + g, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    flag = arrived == static_cast<unsigned>(W) * a.parts - 1;
-    if (flag) put(a.arrivals + g, 0u);  // re-armed for the next launch
-    count = 0;
+  const int lists = W * a.parts;
+  if (lists > 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      const unsigned arrived = __hip_atomic_fetch_add(a.arrivals + g, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      flag = arrived == static_cast<unsigned>(lists) - 1;
+      if (flag) put(a.arrivals + g, 0u);  // re-armed for the next launch
+    }
+  } else if (tid == 0) {
+    flag = 1;
   }
+  if (tid == 0) counts[0] = 0;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (!flag) return;
   const uint64_t* room = a.room + g * W * a.parts * stride;
   const float* scores = a.scores + g * W;
   const int* done = a.done ? a.done + g * W : nullptr;
+  auto is_done = [&](int i) { return done && done[i] != 0; };
+  auto goes_on = [&](int i) { return finite(scores[i]) && is_done(i) && a.eos >= 0 && a.eos < a.V; };
+  // a thread per part of a beam; what they left, and the first of their candidates, in one trip to memory (further lists, if there are more, are read when they are needed)
+  constexpr int kAhead = 4;
+  struct List {
+    uint64_t head, sum, one[kAhead];
+  };
+  auto fetch = [&](int t) {
+    List l{};
+    const int i = t / a.parts;
+    if (t < lists && finite(scores[i]) && !is_done(i)) {
+      const uint64_t* at = room + static_cast<int64_t>(t) * stride;
+      l.head = get(at);
+      l.sum = get(at + 1);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) l.one[u] = get(at + 2 + (u < W ? u : W - 1));
+    }
+    return l;
+  };
+  const List mine = fetch(tid);
+  stat_m[tid] = first_of(mine.head);
+  stat_s[tid] = __builtin_bit_cast(double, mine.sum);
+  __syncthreads();
   // the beams' sums, several beams to a wavefront where there are few parts
   int width = 1;
   while (width < a.parts && width < 64) width *= 2;
   const int each = 64 / width, sub = lane / width, first = lane - sub * width;
   for (int i0 = wave * each; i0 < W; i0 += kBeamWaves * each) {
     const int i = i0 + sub;
-    const bool plain_row = i < W && finite(scores[i]) && !(done && done[i] != 0);
+    const bool plain_row = i < W && finite(scores[i]) && !is_done(i);
     float m = -INFINITY;
     double s = 0.0;
-    if (plain_row && first < a.parts) {
-      m = first_of(get(room + (i * a.parts + first) * stride));
-      s = __builtin_bit_cast(double, get(room + (i * a.parts + first) * stride + 1));
-    }
-    for (int p = first + 64; plain_row && p < a.parts; p += 64) {  // (parts of one lane's: one sum on the larger maximum)
-      const float o = first_of(get(room + (i * a.parts + p) * stride)), both = fmaxf(m, o);
-      const double t = __builtin_bit_cast(double, get(room + (i * a.parts + p) * stride + 1));
-      s = (m == -INFINITY ? s : s * exp(static_cast<double>(m) - static_cast<double>(both))) + (o == -INFINITY ? t : t * exp(static_cast<double>(o) - static_cast<double>(both)));
+    for (int p = first; plain_row && p < a.parts; p += 64) {  // (one lane's parts: one sum on the larger maximum)
+      const int t = i * a.parts + p;
+      const float o = t < kBeamThreads ? stat_m[t] : first_of(get(room + static_cast<int64_t>(t) * stride)), both = fmaxf(m, o);
+      const double more = t < kBeamThreads ? stat_s[t] : __builtin_bit_cast(double, get(room + static_cast<int64_t>(t) * stride + 1));
+      s = (m == -INFINITY ? s : s * exp(static_cast<double>(m) - static_cast<double>(both))) + (o == -INFINITY ? more : more * exp(static_cast<double>(o) - static_cast<double>(both)));
       m = both;
     }
     const float top = max_over(m, width);
@@ -252,32 +334,30 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     }
   }
   __syncthreads();
-  auto is_done = [&](int i) { return done && done[i] != 0; };
   auto normal = [&](int i) { return finite(scores[i]) && !is_done(i) && finite(top_of[i]) && fabs(log_sum[i]) < INFINITY; };
   auto key_of = [&](int i, uint64_t one) {
     const float x = first_of(one);
     return Key{static_cast<double>(scores[i]) + ((static_cast<double>(x) - static_cast<double>(top_of[i])) - log_sum[i]), x, i, static_cast<int>(one >> 32)};
   };
   auto ended_key = [&](int i) { return Key{static_cast<double>(scores[i]), 0.f, i, static_cast<int>(a.eos)}; };
-  auto goes_on = [&](int i) { return finite(scores[i]) && is_done(i) && a.eos >= 0 && a.eos < a.V; };
-  // the lists' first candidates (a beam that is done has one, in its first part's place), and the bound that they give
-  const int lists = W * a.parts;
-  double own = -INFINITY;
+  auto size_of = [](const List& l) { return static_cast<int>(l.head >> 32); };
+  // the bound that the lists' first candidates give, rounded to 32 bits like what is held against it (a beam that is done has one candidate, in its first part's place)
+  float own = -INFINITY;
   for (int t = tid; t < lists; t += kBeamThreads) {
     const int i = t / a.parts;
     if (normal(i)) {
-      const uint64_t head = get(room + static_cast<int64_t>(t) * stride), one = get(room + static_cast<int64_t>(t) * stride + 2);
-      if (static_cast<int>(head >> 32) > 0) own = fmax(own, key_of(i, one).score);
+      const List l = t == tid ? mine : fetch(t);
+      if (size_of(l) > 0) own = fmaxf(own, static_cast<float>(key_of(i, l.one[0]).score));
     } else if (t == i * a.parts && goes_on(i)) {
-      own = fmax(own, ended_key(i).score);
+      own = fmaxf(own, static_cast<float>(ended_key(i).score));
     }
   }
-  const double bound = nth_in_wave(own, W, lane);
-  if (lane == 0) key_bounds[wave] = bound;
+  const float bound = nth_in_wave(own, W);
+  if (lane == 0) bounds[wave] = bound;
   __syncthreads();
-  const double least = fmax(fmax(key_bounds[0], key_bounds[1]), fmax(key_bounds[2], key_bounds[3]));
+  const float least = most(bounds);
   auto keep = [&](const Key& k) {
-    const int n = atomicAdd(&count, 1);
+    const int n = atomicAdd(&counts[0], 1);
     if (n >= kFewKeys) return;
     few.all.score[n] = k.score;
     few.all.logit[n] = k.logit;
@@ -287,17 +367,19 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   for (int t = tid; t < lists; t += kBeamThreads) {
     const int i = t / a.parts;
     if (normal(i)) {
+      List l = t == tid ? mine : fetch(t);
       const uint64_t* at = room + static_cast<int64_t>(t) * stride;
-      const int n = static_cast<int>(get(at) >> 32);
+      const int n = size_of(l);
       bool more = n > 0;
-      for (int k0 = 0; more; k0 += 4) {
-        uint64_t some[4];
+      for (int k0 = 0; more; k0 += kAhead) {
+        if (k0 > 0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) some[u] = get(at + 2 + (k0 + u < n ? k0 + u : n - 1));
+          for (int u = 0; u < kAhead; ++u) l.one[u] = get(at + 2 + (k0 + u < n ? k0 + u : n - 1));
+        }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const Key k = key_of(i, some[u]);
-          more = more && k0 + u < n && k.score >= least;
+        for (int u = 0; u < kAhead; ++u) {
+          const Key k = key_of(i, l.one[u]);
+          more = more && k0 + u < n && static_cast<float>(k.score) >= least;
           if (more) keep(k);
         }
       }
@@ -306,17 +388,28 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     }
   }
   __syncthreads();
-  const int n = count;
+  const int n = counts[0];
   int found = n < W ? n : W;
   if (n <= kFewKeys) {
     for (int i = tid; i < n; i += kBeamThreads) {
-      const Key mine{few.all.score[i], few.all.logit[i], few.all.beam[i], few.all.token[i]};
-      int rank = 0;
-      for (int k = 0; k < n; ++k) rank += before(Key{few.all.score[k], few.all.logit[k], few.all.beam[k], few.all.token[k]}, mine) ? 1 : 0;
+      const Key key{few.all.score[i], few.all.logit[i], few.all.beam[i], few.all.token[i]};
+      int rank = 0, level = 0;
+      for (int k = 0; k < n; k += 4) {
+        const f64x4 some = *reinterpret_cast<const f64x4*>(few.all.score + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = k + j < n;
+          rank += in && some[j] > key.score ? 1 : 0;
+          level += in && some[j] == key.score ? 1 : 0;
+        }
+      }
+      if (level > 1)
+        for (int k = 0; k < n; ++k)
+          if (few.all.score[k] == key.score) rank += before(Key{key.score, few.all.logit[k], few.all.beam[k], few.all.token[k]}, key) ? 1 : 0;
       if (rank < W) {
-        chosen_beam[rank] = mine.beam;
-        chosen_token[rank] = mine.token;
-        chosen_score[rank] = static_cast<float>(mine.score);
+        chosen_beam[rank] = key.beam;
+        chosen_token[rank] = key.token;
+        chosen_score[rank] = static_cast<float>(key.score);
       }
     }
   } else {
@@ -356,22 +449,30 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     }
   }
   __syncthreads();
-  const bool mine = tid < W;
-  const int parent = mine ? chosen_beam[tid] : 0, token = mine ? chosen_token[tid] : 0;
+  const bool one_of = tid < W;
+  const int parent = one_of ? chosen_beam[tid] : 0, token = one_of ? chosen_token[tid] : 0;
   const bool ended = (done && done[parent] != 0) || token == a.eos;
   __syncthreads();  // (scores and done may be the outputs: they have been read)
-  if (!mine) return;
+  if (!one_of) return;
   a.parents[g * W + tid] = parent;
   a.tokens[g * W + tid] = token;
   a.new_scores[g * W + tid] = chosen_score[tid];
   if (a.new_done) a.new_done[g * W + tid] = ended ? 1 : 0;
 }
 
-constexpr int64_t kBeamWords = int64_t{1} << 25, kBeamPiece = kBeamThreads * 4 * 2;  // (64-bit words of a launch; the smallest piece)
-template <int U>
+constexpr int64_t kBeamWords = int64_t{1} << 25, kLeastPart = 2048;  // 64-bit words of a launch's lists; logits of a part
+// Parts of a row: two workgroups per CU, of 2048 logits at least (4096: 13.6 us instead of 14.1 for one group of 4 beams, 44.0 instead of 38.6 for one of 32, even for the others).
+inline int64_t beam_parts(int64_t rows, int64_t V) {
+  int64_t parts = rows < 512 ? 512 / rows : 1;
+  if (parts > ceil_div(V, kLeastPart)) parts = ceil_div(V, kLeastPart);
+  const int64_t per = ceil_div(ceil_div(V, parts), 4) * 4;
+  return ceil_div(V, per);
+}
+
 int launch_beam(BeamArgs a, int64_t groups, hipStream_t s) {
-  a.parts = static_cast<int>(ceil_div(a.V, kBeamThreads * 4 * U));
-  const int64_t per_group = static_cast<int64_t>(a.beams) * a.parts, words = per_group * (2 + a.beams);
+  a.parts = static_cast<int>(beam_parts(groups * a.beams, a.V));
+  a.per = static_cast<int>(ceil_div(ceil_div(a.V, a.parts), 4) * 4);
+  const int64_t words = static_cast<int64_t>(a.beams) * a.parts * (2 + a.beams);
   // as many groups at a time as 256 MiB of the workspace, and a grid, hold
   int64_t some = kBeamWords / words;
   if (some > 65535) some = 65535;
@@ -381,7 +482,7 @@ int launch_beam(BeamArgs a, int64_t groups, hipStream_t s) {
     std::unique_lock<std::recursive_mutex> lock;
     if (split_scratch(s, static_cast<size_t>(now * words) * 8, static_cast<size_t>(now), a.parts, &room, &a.arrivals, &lock) != 0) return -1;
     a.room = reinterpret_cast<uint64_t*>(room);
-    hipLaunchKernelGGL(beam_select_kernel<U>, dim3(static_cast<unsigned>(a.parts), static_cast<unsigned>(a.beams), static_cast<unsigned>(now)), dim3(kBeamThreads), 0, s, a);
+    hipLaunchKernelGGL(beam_select_kernel, dim3(static_cast<unsigned>(a.parts), static_cast<unsigned>(a.beams), static_cast<unsigned>(now)), dim3(kBeamThreads), 0, s, a);
     if (check_launch("beam_select") != 0) return -1;
     const int64_t rows = now * a.beams;
     a.logits += rows * a.V;
@@ -407,8 +508,7 @@ extern "C" int dtas_beam_select_f32(const void* logits, const void* scores, cons
   if ((done == nullptr) != (new_done == nullptr)) return fail("beam_select: done and new_done go together");
   if (groups == 0 || beams == 0) return 0;
   if (V == 0) return fail("beam_select: no token to choose from");
-  if (V > INT32_MAX || groups > INT32_MAX || V > (int64_t{1} << 60) / beams / groups) return fail("beam_select: the extents overflow");
-  if (beams * ceil_div(V, kBeamPiece) * (2 + beams) > kBeamWords) return fail("beam_select: a vocabulary of %lld is too large", (long long)V);
+  if (V > (int64_t{1} << 30) || groups > INT32_MAX || V > (int64_t{1} << 60) / beams / groups) return fail("beam_select: the extents overflow");
   if (!logits || !scores || !tokens || !parents || !new_scores) return fail("beam_select: NULL buffer");
   const int64_t rows = groups * beams;
   struct Span { const void* at; int64_t bytes; };
@@ -422,10 +522,6 @@ extern "C" int dtas_beam_select_f32(const void* logits, const void* scores, cons
       if (out[j].at && overlaps(out[i].at, out[i].bytes, out[j].at, out[j].bytes)) return fail("beam_select: the outputs overlap");
   }
   BeamArgs a{static_cast<const float*>(logits), static_cast<const float*>(scores), static_cast<const int*>(done), static_cast<int*>(tokens), static_cast<int*>(parents),
-             static_cast<float*>(new_scores), static_cast<int*>(new_done), static_cast<int>(beams), 0, V, eos, nullptr, nullptr};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  // pieces of 2048, 4096 or 8192 logits: as many workgroups as two per CU, or as fill the chip while the pieces are the smallest
-  if (rows * ceil_div(V, 8192) >= 512) return launch_beam<8>(a, groups, s);
-  if (rows * ceil_div(V, 4096) >= 512) return launch_beam<4>(a, groups, s);
-  return launch_beam<2>(a, groups, s);
+             static_cast<float*>(new_scores), static_cast<int*>(new_done), static_cast<int>(beams), 0, 0, V, eos, nullptr, nullptr};
+  return launch_beam(a, groups, static_cast<hipStream_t>(stream));
 }

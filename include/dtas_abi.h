@@ -510,7 +510,7 @@ int dtas_attn_paged_f16(const void* Q, const void* K_pages, const void* V_pages,
  * logits [groups, beams, V], scores [groups, beams], fp32.  Candidate (w, v) of a group has scores[w] + log_softmax(logits[w])[v]; a beam that is done (done[w] != 0)
  * goes on with token eos alone, at scores[w].  What is no finite number counts as -inf.  The `beams` best candidates in their order, ties to the lower w, then the lower
  * v: parents, tokens [groups, beams] int32, new_scores [groups, beams] fp32; new_done = done of the parent, or token == eos.  done and new_done [groups, beams] int32,
- * or both NULL: no beam is done.  eos outside [0, V): none is (a beam that is done then has no candidate).  new_scores == scores and new_done == done are allowed.  beams up to DTAS_MAX_BEAMS.
+ * or both NULL: no beam is done.  eos outside [0, V): none is (a beam that is done then has no candidate).  new_scores == scores and new_done == done are allowed.  beams up to DTAS_MAX_BEAMS, V up to 2^30.
  * Candidates are compared in 64 bits, sums of exponentials are in 64 bits over terms in 32.  Uses the split-K workspace. */
 int dtas_beam_select_f32(const void* logits, const void* scores, const void* done, void* tokens, void* parents, void* new_scores, void* new_done,
                          int64_t groups, int64_t beams, int64_t V, int64_t eos, void* stream);

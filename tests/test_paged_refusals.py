@@ -69,8 +69,8 @@ def test_attn_paged_refuses(bad, why):
 
 
 @pytest.mark.parametrize("bad,why", [
-    (dict(groups=-1), "negative extent"), (dict(beams=33), "up to 32 beams"), (dict(V=0), "no token"), (dict(V=1 << 31), "overflow"), (dict(groups=1 << 31), "overflow"),
-    (dict(done=None), "go together"), (dict(new_done=None), "go together"), (dict(V=1 << 30, beams=32), "too large"),
+    (dict(groups=-1), "negative extent"), (dict(beams=33), "up to 32 beams"), (dict(V=0), "no token"), (dict(V=(1 << 30) + 1), "overflow"), (dict(groups=1 << 31), "overflow"),
+    (dict(done=None), "go together"), (dict(new_done=None), "go together"),
     *((dict([(name, None)]), "NULL") for name in ("logits", "scores", "tokens", "parents", "new_scores")),
     (dict(tokens=A), "output overlaps"), (dict(new_scores=B + 4), "output overlaps"), (dict(new_done=C + 4), "output overlaps"), (dict(new_scores=C), "output overlaps"),
     (dict(new_done=B), "output overlaps"), (dict(parents=D + 4), "outputs overlap"), (dict(new_scores=E), "outputs overlap"), (dict(new_done=F), "outputs overlap")])
