@@ -42,7 +42,7 @@ __device__ __forceinline__ unsigned upto_in_block(unsigned v, unsigned* slots, u
 // A thread per sequence finds out what it needs and, from the sums over the sequences before it, whether the pool has it; then a thread per row looks up its sequence
 // (packed rows: by halving the starts, which lie in the LDS) and its slot.  The row that begins a page writes it into the table, so that no two threads write one entry,
 // and nobody reads an entry that this launch writes.  Every workgroup repeats the sums for itself: no hand-over between workgroups, whose
-// trip through memory costs more than the sums of a thousand sequences.
+// trip through memory costs more than the sums of a thousand sequences.  3.4 us, a launch's time, for 64 sequences of a row; 5.7 for 16384 packed rows.
 struct AssignArgs {
   const int *lens, *count;
   int* table;
@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(THREADS) page_assign_kernel(AssignArgs a, bool
 
 // ---- rows into their slots ----------------------------------------------------------------------------------------------
 // A workgroup has `run` rows of one layer, of K and of V, in 16-byte pieces (or elements): a row of all key heads at least, two pieces per thread and turn.
+// 2047 packed rows of 32 heads of 80 (42 MB read and written): 8.4 us, 5.0 TB/s, the rate of a large copy; 64 rows: 3.75 us, a launch's time.
 template <typename U>
 __global__ void __launch_bounds__(256) page_append_kernel(const U* __restrict__ K, const U* __restrict__ V, const int* __restrict__ slots, U* __restrict__ Kp,
                                                           U* __restrict__ Vp, int64_t rows, int kv_heads, int per_row, unsigned page, int64_t pages, int run, unsigned runs) {
@@ -172,6 +173,8 @@ __global__ void __launch_bounds__(256) page_append_kernel(const U* __restrict__ 
 // parent's from that lane, and compares its own with all that are taken: what nobody takes goes onto the stack, once.  Where on the stack is known when all groups have
 // counted: the pages wait in the workspace, and whoever is last among the workgroups puts them down in their order, and takes the pages for copies from the top
 // (in this order: a pool that has a page too few for the moment would lose a row otherwise).  The copies are a second launch.
+// What binds are trips to memory, one behind the other: lengths, entries, the arrival, what was given back, what is wanted: 6.2 us for one group of 4 beams, 9.8 for 24 of 8 (18.8 with a
+// wavefront per list of pages in settle_pool instead of a thread per page).
 struct ReorderArgs {
   const int *parents, *table, *lens;
   int* free;
@@ -196,7 +199,7 @@ __device__ __forceinline__ T get(const T* at) { return __hip_atomic_load(at, __A
 
 constexpr int kReorderThreads = 1024;
 __device__ void settle_pool(const ReorderArgs& a) {
-  __shared__ unsigned slots[kReorderThreads / 64], many[kReorderThreads], before[kReorderThreads];
+  __shared__ unsigned slots[kReorderThreads / 64], before[kReorderThreads];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nwaves = blockDim.x >> 6;
   const int64_t threads = blockDim.x;
   const int stack = *a.free_count;
@@ -219,14 +222,19 @@ __device__ void settle_pool(const ReorderArgs& a) {
     const unsigned n = c + tid < segments ? get(a.backs + c + tid) : 0u;
     unsigned total;
     const unsigned behind = upto(n, total);
-    many[tid] = n;
     before[tid] = behind - n;
     __syncthreads();
-    for (int i = wave; i < threads && c + i < segments; i += nwaves)
-      for (unsigned j = lane; j < many[i]; j += 64) {
-        const uint64_t at = height + before[i] + j;
-        if (at < static_cast<uint64_t>(a.pages)) put(a.free + at, get(a.back + (c + i) * a.share + j));
+    // a thread per page: the last list that begins at it or before (an empty one begins where the next does)
+    const unsigned lists = segments - c < threads ? static_cast<unsigned>(segments - c) : static_cast<unsigned>(threads);
+    for (unsigned j = tid; j < total; j += static_cast<unsigned>(threads)) {
+      unsigned low = 0, high = lists;
+      while (high - low > 1) {
+        const unsigned mid = (low + high) / 2;
+        if (before[mid] <= j) low = mid;
+        else high = mid;
       }
+      if (height + j < static_cast<uint64_t>(a.pages)) put(a.free + height + j, get(a.back + (c + low) * a.share + (j - before[low])));
+    }
     height += total;
     __syncthreads();
   }
@@ -277,6 +285,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
   const int from = first + (has ? parent : 0);
   const unsigned their_len = __shfl(len, from), their_named = __shfl(named, from), new_len = has ? their_len : 0u, new_named = has ? their_named : 0u;
   bool later = false;  // (a row of the same parent stands in front)
+#pragma unroll 4
   for (int i = 0; i < a.beams; ++i) {  // (every lane shuffles)
     const int one = __shfl(parent, first + i);
     later = later || (one == parent && i < w);
@@ -305,6 +314,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
     const bool mine = has && c < hi && c < new_named;
     const int take = mine ? theirs : -1;
     bool kept = false, again = false;
+#pragma unroll 4
     for (int i = 0; i < a.beams; ++i) {
       const int some = __shfl(take, first + i), one = __shfl(entry, first + i);
       kept = kept || some == entry;
@@ -320,7 +330,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
     }
     entry = next;
   }
-  if (lane == 0) put(a.backs + g * a.waves + wave, given);
+  if (lane == 0 && wave < a.waves) put(a.backs + g * a.waves + wave, given);
   __syncthreads();
   if (wave == 0 && row && sub == 0) {
     const uint64_t one = copy[w];
@@ -339,23 +349,37 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
   if (flag) settle_pool(a);
 }
 
-// The copies: a workgroup per copy and layer, the filled rows of all key heads, of K and of V
+// The copies: a wavefront per copy, layer, key head and K or V, four pieces per lane on their way at a time.  24 groups of 8 beams, 16 layers of 8 heads of 128, pages of 32 (95 MB
+// read and written): 24 us of the call's 33.7 (eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
 template <typename U>
 __global__ void __launch_bounds__(256) page_copy_kernel(U* __restrict__ Kp, U* __restrict__ Vp, const int* __restrict__ copies, const unsigned* __restrict__ count,
-                                                        int64_t layers, int64_t pages, int kv_heads, int per_row, unsigned page) {
-  const int64_t items = static_cast<int64_t>(*count) * layers, head = static_cast<int64_t>(page) * per_row;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t k = item / layers, l = item - k * layers;
+                                                        unsigned layers, int64_t pages, unsigned kv_heads, unsigned per_row, unsigned page) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t each = uint64_t{2} * kv_heads * layers, items = *count * each, head = static_cast<uint64_t>(page) * per_row;
+  for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * 4 + wave; item < items; item += static_cast<uint64_t>(gridDim.x) * 4) {
+    const uint64_t k = item / each, of = item - k * each;  // (neighbours: the heads of a page)
+    const uint64_t tensor = of / (each / 2), l = (of - tensor * (each / 2)) / kv_heads, h = of % kv_heads;
     const int from = copies[4 * k], to = copies[4 * k + 1];
-    const unsigned some = static_cast<unsigned>(copies[4 * k + 2]) * static_cast<unsigned>(per_row);
-    if (some == 0) continue;
-    const int64_t source = (l * pages + from) * kv_heads * head, sink = (l * pages + to) * kv_heads * head;
-    for (int64_t t = threadIdx.x; t < static_cast<int64_t>(some) * kv_heads; t += 256) {
-      const int64_t h = t / some, at = h * head + (t - h * some);
-      const U kv = Kp[source + at], vv = Vp[source + at];
-      Kp[sink + at] = kv;
-      Vp[sink + at] = vv;
+    const unsigned some = static_cast<unsigned>(copies[4 * k + 2]) * per_row;
+    U* base = tensor ? Vp : Kp;
+    const U* source = base + ((l * pages + from) * kv_heads + h) * head;
+    U* sink = base + ((l * pages + to) * kv_heads + h) * head;
+    constexpr int kAhead = 4;
+    unsigned t = lane;
+    for (; t + (kAhead - 1) * 64 < some; t += kAhead * 64) {
+      U v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) v[u] = source[t + u * 64];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) sink[t + u * 64] = v[u];
     }
+    U v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (t + u * 64 < some) v[u] = source[t + u * 64];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (t + u * 64 < some) sink[t + u * 64] = v[u];
   }
 }
 
@@ -447,7 +471,7 @@ extern "C" int dtas_page_reorder_f16(const void* parents, const void* table, con
                 (long long)beams, (long long)columns, (long long)kv_heads, (long long)d, (long long)pages);
   if (page < 1) return fail("page_reorder: a page holds at least one position, got %lld", (long long)page);
   if (beams > DTAS_MAX_BEAMS) return fail("page_reorder: up to %d beams, got %lld", DTAS_MAX_BEAMS, (long long)beams);
-  if (groups > INT32_MAX / DTAS_MAX_BEAMS || columns > INT32_MAX || page > INT32_MAX || pages > INT32_MAX / page || kv_heads > INT32_MAX || d > INT32_MAX ||
+  if (layers > INT32_MAX || groups > INT32_MAX / DTAS_MAX_BEAMS || columns > INT32_MAX || page > INT32_MAX || pages > INT32_MAX / page || kv_heads > INT32_MAX || d > INT32_MAX ||
       (columns > 0 && groups > kMost / DTAS_MAX_BEAMS / columns) || (d > 0 && page * d > INT32_MAX) ||
       (layers > 0 && kv_heads > 0 && d > 0 && pages > 0 && layers > kMost / kv_heads / d / (pages * page)))
     return fail("page_reorder: the extents overflow");
@@ -483,15 +507,18 @@ extern "C" int dtas_page_reorder_f16(const void* parents, const void* table, con
   a.count = reinterpret_cast<unsigned*>(room) + 6 * rows;
   a.backs = a.count + 2;
   a.back = reinterpret_cast<int*>(a.backs + groups * a.waves);
-  hipLaunchKernelGGL(page_reorder_kernel, dim3(static_cast<unsigned>(a.groups > 0 ? a.groups : 1)), dim3(64 * a.waves), 0, s, a);
+  // (whoever settles the pool has use for more threads than the columns have, where there are many groups)
+  const unsigned threads = 64u * static_cast<unsigned>(a.waves >= 8 || groups * a.waves <= 1 ? a.waves : groups * a.waves < 8 ? groups * a.waves : 8);
+  hipLaunchKernelGGL(page_reorder_kernel, dim3(static_cast<unsigned>(a.groups > 0 ? a.groups : 1)), dim3(threads), 0, s, a);
   if (check_launch("page_reorder") != 0) return -1;
-  const int64_t most = groups * (beams - 1) * layers;
-  if (beams < 2 || most <= 0 || page_bytes == 0 || page == 1) return 0;
+  if (groups == 0 || beams < 2 || page_bytes == 0 || page == 1) return 0;
+  const int64_t most = groups * (beams - 1), each = 2 * layers * kv_heads;  // copies at most, and a copy's items
+  const unsigned grid = each < 8192 / most ? static_cast<unsigned>(ceil_div(most * each, 4)) : 2048;
   const bool wide = d % 8 == 0 && aligned(K_pages, 16) && aligned(V_pages, 16);
   auto go = [&](auto* tag) {
     using U = std::remove_pointer_t<decltype(tag)>;
-    hipLaunchKernelGGL(page_copy_kernel<U>, dim3(static_cast<unsigned>(most < 4096 ? most : 4096)), dim3(256), 0, s, static_cast<U*>(K_pages), static_cast<U*>(V_pages),
-                       a.copies, a.count, layers, pages, static_cast<int>(kv_heads), static_cast<int>(wide ? d / 8 : d), static_cast<unsigned>(page));
+    hipLaunchKernelGGL(page_copy_kernel<U>, dim3(grid), dim3(256), 0, s, static_cast<U*>(K_pages), static_cast<U*>(V_pages), a.copies, a.count,
+                       static_cast<unsigned>(layers), pages, static_cast<unsigned>(kv_heads), static_cast<unsigned>(wide ? d / 8 : d), static_cast<unsigned>(page));
   };
   if (wide) go(static_cast<u32x4*>(nullptr));
   else go(static_cast<half_t*>(nullptr));
