@@ -822,7 +822,7 @@ int launch_paged(const PagedArgs& a, int64_t batch, int beams, int sub, hipStrea
   const int64_t problems = batch / grid.beams * grid.subs;
   grid.row_groups = GROUP ? 1 : static_cast<int>(ceil_div(g, 16 * RT));
   const int64_t kinds = a.kv_heads * static_cast<int64_t>(grid.row_groups), blocks = a.room < 32 ? 1 : ceil_div(a.room, 32);
-  if (problems > (int64_t{1} << 30) / blocks) return fail("attn_paged: the tables hold too many positions");
+  if (problems * grid.sub > (int64_t{1} << 30) / blocks) return fail("attn_paged: the tables hold too many positions");
   grid.problems = static_cast<int>(problems);
   grid.least = 8;
   grid.whole = 24;

@@ -4,7 +4,7 @@
 //   the `beams` best, by (score descending, w, v ascending); what is no finite number counts as -inf
 //
 // Within a beam the order is that of the logits, so one pass over them is enough: a workgroup goes through a part of one beam's logits and keeps its maximum, its sum of
-// exponentials (terms in 32 bits, each product with log2 e kept to twice that; the sum in 64) and its W best so far; whoever is last among a group's workgroups has the
+// exponentials (sixteen terms added in 32 bits, each product with log2 e kept to twice that; their sums in 64) and its W best so far; whoever is last among a group's workgroups has the
 // sums of all and compares what is left, in 64 bits.
 // The W best of many are found without sorting them: every lane has the best of its own, the W-th best of these in a wavefront is as good as W of all at least, so only what is not
 // below that can be among the W.  These few are counted out against each other; behind the first piece of a part only what beats the W-th best so far is left.

@@ -499,7 +499,7 @@ int dtas_page_append_f16(const void* K, const void* V, const void* slots, void* 
  * out[b,h,:] = sum_j softmax_j(scale * Q[b,h,:] . k_j) v_j over the positions j < lens[b] (clipped to [0, columns * page]; the token's own is among
  * them); positions in pages outside [0, pages) are not seen, a row that sees nothing is zeros.  Q and out [batch, heads, d], one layer's K_pages and V_pages
  * [pages, kv_heads, page, d]; heads is a multiple of kv_heads, query head h reads key head h / (heads / kv_heads).  Sequences in a row, `beams` of them, form a group: a
- * page that several of them name in the same column is read once for all (the result is the same with beams = 1).  batch is a multiple of beams.
+ * page that several of them name in the same column is read once for all, for d up to 128 (the definition is that of beams = 1).  batch is a multiple of beams.
  * d up to 256; d a multiple of 8, data on 16-byte boundaries and pages of a multiple of 16 positions run on the matrix cores, others element by element.  fp32 scores,
  * statistics and sums; weights in fp16 on the matrix cores, as in dtas_attn_tree_f16.  scale is a finite number up to 2e38 either way.  Uses the
  * split-K workspace, under the rules stated at the top of this file. */
@@ -511,7 +511,7 @@ int dtas_attn_paged_f16(const void* Q, const void* K_pages, const void* V_pages,
  * goes on with token eos alone, at scores[w].  What is no finite number counts as -inf.  The `beams` best candidates in their order, ties to the lower w, then the lower
  * v: parents, tokens [groups, beams] int32, new_scores [groups, beams] fp32; new_done = done of the parent, or token == eos.  done and new_done [groups, beams] int32,
  * or both NULL: no beam is done.  eos outside [0, V): none is (a beam that is done then has no candidate).  new_scores == scores and new_done == done are allowed.  beams up to DTAS_MAX_BEAMS, V up to 2^30.
- * Candidates are compared in 64 bits, sums of exponentials are in 64 bits over terms in 32.  Uses the split-K workspace. */
+ * Candidates are compared in 64 bits, sums of exponentials are in 64 bits over sums of sixteen terms in 32.  Uses the split-K workspace. */
 int dtas_beam_select_f32(const void* logits, const void* scores, const void* done, void* tokens, void* parents, void* new_scores, void* new_done,
                          int64_t groups, int64_t beams, int64_t V, int64_t eos, void* stream);
 
