@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(64) attn_paged_scalar_kernel(PagedArgs a, int6
 // wavefront's own and is read from there transposed.  The next visit's K and V are on their way in registers, and the table's entries a block further ahead.
 // In a group a block is visited once for every page that its sequences name there; rows that do not name it have their scores masked.
 // The blocks of all problems, one behind the other, are dealt out in equal shares, on the device, which knows the lengths: see Share.
+constexpr int kAgent = 16;    // loads past the L2 of an XCD (sc1), as atomic ones of the device's scope are, but 16 bytes wide: 4 beams after 32749 keys 41.5 us, 43.9 with two of 8
 constexpr int kStreamed = 2;  // loads that nobody repeats (nt): 2.3 GB in pieces of 8 KiB 6.0 TB/s without, 6.8 with
 constexpr int kNear = 8, kWhole = 2;
 constexpr unsigned kSlotsY = 65535;  // a grid's extent in y
@@ -301,7 +302,7 @@ __device__ f32x4 values_no_numbers(const PagedArgs& a, const Visited& v, int bea
 }
 
 template <int DP, int RT, int W, bool GROUP>
-__global__ void __launch_bounds__(64 * W, DP < 128 || (DP == 128 && !(RT == 2 && GROUP)) ? 2 : 1) attn_paged_kernel(PagedArgs a, PagedGrid grid) {
+__global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) attn_paged_kernel(PagedArgs a, PagedGrid grid) {
   constexpr int KS = DP / 32, DT = DP / 16, VL = DP / 16, VH = VL / 2;  // k steps, channel tiles, 16-byte pieces of V per lane, of a half
   constexpr int kRows = 16 * RT, kChunks = DP / 8, kWave = 32 * v_row_bytes(DP), kShare = kRows * (DP + 2);
   __shared__ __attribute__((aligned(16))) char lds[W * kWave];
@@ -723,15 +724,13 @@ __global__ void __launch_bounds__(64 * W, DP < 128 || (DP == 128 && !(RT == 2 &&
     while (spread * 2 * items_all <= 64 * W && spread < parts) spread *= 2;
     const int lot = tid_b / items_all, mine_of = tid_b - lot * items_all;
     f32x4 some[kAtOnce];
+    const __amdgpu_buffer_rsrc_t pieces = make_rsrc(firsts, 8u * grid.shares * kShare);
     auto request = [&](int at, int y0) {
       const int offset = at / kItems * DP + 4 * (at % kItems);
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
         const int y = y0 + u * spread < parts ? y0 + u * spread : parts - 1;
-        const uint64_t* two = reinterpret_cast<const uint64_t*>(sums_of(y) + offset);
-        const uint64_t low = __hip_atomic_load(two, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), high = __hip_atomic_load(two + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        some[u] = f32x4{__builtin_bit_cast(float, static_cast<unsigned>(low)), __builtin_bit_cast(float, static_cast<unsigned>(low >> 32)),
-                        __builtin_bit_cast(float, static_cast<unsigned>(high)), __builtin_bit_cast(float, static_cast<unsigned>(high >> 32))};
+        some[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(pieces, 4u * (((y == 0 ? grid.shares : y) + first_cut - 1) * kShare + offset), 0, kAgent));
       }
     };
     if (lot < spread) request(mine_of, lot);  // (on their way while the statistics come)
@@ -844,18 +843,19 @@ int launch_paged(const PagedArgs& a, int64_t batch, int beams, int sub, hipStrea
 template <int DP>
 int launch_paged_rows(const PagedArgs& a, int64_t batch, int beams, hipStream_t s) {
   const int g = a.heads / a.kv_heads;
-  // 32 rows at a time where their sums and the queries leave room for the keys (heads of up to 128), 16 beyond.  A problem holds as many sequences of a group as that; with
-  // heads of more than 128 the sequences of a group are read one by one.
+  // A problem holds as many sequences of a group as make sixteen rows; with heads of more than 128 they are read one by one.  (32 rows read what more of them share once, but a problem's
+  // own pages are then in fewer workgroups, and for heads of 128 in four wavefronts each, for want of registers: 45 sequences in groups of 5 after 675 keys 48.0 us / 29.2, 8 beams after
+  // 16000 on 4 heads of 80 38.3 / 25.4; only 7 such groups after 53876 gain, 104 / 125.)
   if constexpr (DP <= 128) {
     if (g <= 16) {
-      const int sub = beams > 1 ? (32 / g < beams ? 32 / g : beams) : 1;
-      if (sub * g > 16) return launch_paged<DP, 2, 4, true>(a, batch, beams, sub, s);
+      const int sub = beams > 1 ? (16 / g < beams ? 16 / g : beams) : 1;
       // Eight wavefronts where few problems are cut, four, and two workgroups per CU, where each CU has several to itself: 4 beams after 32749 keys 43.2 us / 48.6, 61 sequences after
       // up to 2047 on 8 heads 47.2 / 52.1; 64 on 32 heads of 80 after up to 300 55.4 / 30.2, 300 on 8 of 128 after up to 100 61.6 / 28.8.
       const bool many = batch / beams * ((beams + sub - 1) / sub) * a.kv_heads >= 512;
       if (beams > 1) return many ? launch_paged<DP, 1, 4, true>(a, batch, beams, sub, s) : launch_paged<DP, 1, 8, true>(a, batch, beams, sub, s);
       return many ? launch_paged<DP, 1, 4, false>(a, batch, beams, 1, s) : launch_paged<DP, 1, 8, false>(a, batch, beams, 1, s);
     }
+    // 32 rows at a time
     return launch_paged<DP, 2, 4, false>(a, batch, beams, 1, s);
   } else {
     return launch_paged<DP, 1, 4, false>(a, batch, beams, 1, s);
