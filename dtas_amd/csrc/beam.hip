@@ -6,7 +6,7 @@
 // Within a beam the order is that of the logits, so one pass over them is enough: a workgroup goes through a part of one beam's logits and keeps its maximum, its sum of
 // exponentials (sixteen terms added in 32 bits, each product with log2 e kept to twice that; their sums in 64) and its W best so far; whoever is last among a group's workgroups has the
 // sums of all and compares what is left, in 64 bits.
-// The W best of many are found without sorting them: every lane has the best of its own, the W-th best of these in a wavefront is as good as W of all at least, so only what is not
+// The W best of many are found without sorting them: every eight lanes have the best of their own, the W-th best of these is as good as W of all at least, so only what is not
 // below that can be among the W.  These few are counted out against each other; behind the first piece of a part only what beats the W-th best so far is left.
 #include "gemm_common.h"
 
@@ -58,13 +58,36 @@ __device__ __forceinline__ float max_over(float v, int width) {
   for (int k = 1; k < width; k *= 2) v = fmaxf(v, __shfl_xor(v, k));
   return v;
 }
-// The W-th largest of the lanes' values: the least of those that fewer than W are above
+// The W-th largest of the lanes' values, or a little less: the first 20 bits of it, found bit by bit (as whole numbers in the same order)
 __device__ __forceinline__ float nth_in_wave(float v, int W) {
-  int above = 0;
-#pragma unroll 16
-  for (int i = 0; i < 64; ++i) above += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)) > v ? 1 : 0;
-  return -wave_max(above < W ? -v : -INFINITY);
+  constexpr unsigned kLowest = 0x007fffffu;  // -inf
+  const unsigned bits = __builtin_bit_cast(unsigned, v), key = bits >> 31 != 0 ? ~bits : bits | 0x80000000u;
+  unsigned found = 0;
+#pragma unroll 4
+  for (int i = 31; i >= 12; --i) {
+    const unsigned next = found | 1u << i;
+    found = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= next)) >= W ? next : found;
+  }
+  return found <= kLowest ? -INFINITY : __builtin_bit_cast(float, found >> 31 != 0 ? found & 0x7fffffffu : ~found);
 }
+// the sum of all lanes, in the last
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_dpp(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const unsigned low = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(bits), CTRL, ROWS, 0xf, true));
+  const unsigned high = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), CTRL, ROWS, 0xf, true));
+  return v + __builtin_bit_cast(double, static_cast<uint64_t>(low) | static_cast<uint64_t>(high) << 32);
+}
+__device__ __forceinline__ double sum_in_last(double v) {
+  v = add_dpp<0x118, 0xf>(add_dpp<0x114, 0xf>(add_dpp<0x112, 0xf>(add_dpp<0x111, 0xf>(v))));  // row_shr:1, 2, 4, 8
+  return add_dpp<0x143, 0xc>(add_dpp<0x142, 0xa>(v));                                         // row_bcast:15, :31
+}
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float v) {
+  const int bits = __builtin_bit_cast(int, v);
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(bits, bits, CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float max_of_eight(float v) { return max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(v))); }  // quad_perm xor 1, xor 2, row_half_mirror
 
 // A candidate's place in the order: score, then the beam, then the logit, then the token (of one beam's candidates the sum may be the same where the logits are not)
 struct Key {
@@ -107,7 +130,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   };
   __shared__ Lds few;
   __shared__ Key slots[kBeamWaves];
-  __shared__ float tops[kBeamWaves], bounds[kBeamWaves], best_logit[2][DTAS_MAX_BEAMS];
+  __shared__ float tops[kBeamWaves], bounds[64], best_logit[2][DTAS_MAX_BEAMS];
   __shared__ int best_at[2][DTAS_MAX_BEAMS];
   __shared__ double sums[kBeamWaves], log_sum[DTAS_MAX_BEAMS], stat_s[kBeamThreads];
   __shared__ float top_of[DTAS_MAX_BEAMS], chosen_score[DTAS_MAX_BEAMS], stat_m[kBeamThreads];
@@ -122,6 +145,14 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
 #pragma unroll
     for (int i = 1; i < kBeamWaves; ++i) v = fmaxf(v, of[i]);
     return v;
+  };
+  // the W-th best of 64 maxima of eight threads each: as many are as good as it
+  static_assert(kBeamThreads == 64 * 8 && DTAS_MAX_BEAMS <= 64, "a lane for each");
+  auto bound_of = [&](float own) {
+    const float eight = max_of_eight(own);
+    if ((lane & 7) == 0) bounds[tid >> 3] = eight;
+    __syncthreads();
+    return nth_in_wave(bounds[lane], W);
   };
   if (plain) {
     const float* row = a.logits + (g * W + w) * a.V + from;
@@ -153,10 +184,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
 #pragma unroll
       for (int u = 0; u < kPieces; ++u) own = fmaxf(own, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
       if (have < W) {
-        const float bound = nth_in_wave(own, W);
-        if (lane == 0) bounds[wave] = bound;
-        __syncthreads();
-        limit = most(bounds);
+        limit = bound_of(own);
       }
       const float wave_top = wave_max(own);
       if (wave_top > m) {
@@ -241,9 +269,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
           }
         }
         __syncthreads();
-        if (tid == 0) counts[turn] = 0;
+        if (tid == 0) counts[turn] = 0;  // (a barrier stands before it is used again, and before the list is)
         if (have == W) limit = best_logit[side][W - 1];
-        __syncthreads();
       }
 #pragma unroll
       for (int u = 0; u < kPieces; ++u)
@@ -253,10 +280,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     if (lane == 0) tops[wave] = m;
     __syncthreads();
     const float top = most(tops);
-    s = sum_over(s, 64);
+    s = sum_in_last(s);
     if (m != -INFINITY) s *= exp(static_cast<double>(m) - static_cast<double>(top));
     if (__builtin_amdgcn_ballot_w64(strange) != 0) s = __builtin_nan("");
-    if (lane == 0) sums[wave] = s;
+    if (lane == 63) sums[wave] = s;
     __syncthreads();
     uint64_t* room = a.room + ((g * W + w) * a.parts + part) * stride;
     if (tid < have) put(room + 2 + tid, pair_of(best_logit[side][tid], static_cast<unsigned>(from + best_at[side][tid])));
@@ -359,10 +386,15 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
       own = fmaxf(own, static_cast<float>(ended_key(i).score));
     }
   }
-  const float bound = nth_in_wave(own, W);
-  if (lane == 0) bounds[wave] = bound;
-  __syncthreads();
-  const float least = most(bounds);
+  float least;
+  if (lists >= 8 * W) {  // (fewer: there are no W maxima of eight threads)
+    least = bound_of(own);
+  } else {
+    const float bound = nth_in_wave(own, W);
+    if (lane == 0) bounds[wave] = bound;
+    __syncthreads();
+    least = most(bounds);
+  }
   auto keep = [&](const Key& k) {
     const int n = atomicAdd(&counts[0], 1);
     if (n >= kFewKeys) return;
