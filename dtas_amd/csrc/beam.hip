@@ -4,7 +4,7 @@
 //   the `beams` best, by (score descending, w, v ascending); what is no finite number counts as -inf
 //
 // Within a beam the order is that of the logits, so one pass over them is enough: a workgroup goes through a part of one beam's logits and keeps its maximum, its sum of
-// exponentials (sixteen terms added in 32 bits, each product with log2 e kept to twice that; their sums in 64) and its W best so far; whoever is last among a group's workgroups has the
+// exponentials (sixteen terms added in 32 bits, their sums in 64) and its W best so far; whoever is last among a group's workgroups has the
 // sums of all and compares what is left, in 64 bits.
 // The W best of many are found without sorting them: every eight lanes have the best of their own, the W-th best of these is as good as W of all at least, so only what is not
 // below that can be among the W.  These few are counted out against each other; behind the first piece of a part only what beats the W-th best so far is left.
@@ -36,11 +36,14 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBeamThreads = 512, kBeamWaves = kBeamThreads / 64;
 
-// exp(x - m) for x <= m, nought for -inf and for what is no number: the exponent as the rounded product with log2 e and what that rounding left
+// Terms exp(x - m), x <= m, as 2^(x k - c) with k = log2 e in fp32 and c = m k rounded: in one operation x k - c = (x - m) k + (m k - c), whose last part is the same for all of
+// them, exact in fp32, and small while m is (below 2^20: 0.1).  Its own rounding and k's leave y 2^-24 and 0.23 y 2^-24 of a term, y = m - x.
+constexpr float kLog2e = 1.44269502f;
+// For m beyond: the exponent as the rounded product with log2 e and what that rounding left; nought for -inf and for what is no number
 __device__ __forceinline__ float exp_below(float x, float m) {
-  constexpr float kHigh = 1.44269502f, kLow = 1.92596299e-8f, kLn2 = 0.693147182f;
-  const float d = fmaxf(x - m, -150.f), t = d * kHigh;
-  const float e = __builtin_amdgcn_exp2f(t), r = fmaf(d, kLow, fmaf(d, kHigh, -t));
+  constexpr float kLow = 1.92596299e-8f, kLn2 = 0.693147182f;
+  const float d = fmaxf(x - m, -150.f), t = d * kLog2e;
+  const float e = __builtin_amdgcn_exp2f(t), r = fmaf(d, kLow, fmaf(d, kLog2e, -t));
   return fmaf(e, r * kLn2, e);
 }
 // the next number below (-inf: itself)
@@ -177,7 +180,6 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     int have = 0, side = 0;  // (of the best so far, in best_logit[side])
     float limit = -INFINITY, m = -INFINITY;
     double s = 0.0;
-    bool strange = false;
     for (int base = 0, turn = 0; base < here; base += kPiece, turn ^= 1) {
       if (base + kPiece < here) load(y, base + kPiece);
       float own = -INFINITY;
@@ -192,13 +194,26 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
         m = wave_top;
       }
       float terms[kPieces];
+      const float at = m == -INFINITY ? 0.f : m, c = at * kLog2e;
+      if (__builtin_amdgcn_readfirstlane(fabsf(at) < 0x1p20f)) {  // (of what is no number the sum is none)
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u) {
-        terms[u] = (exp_below(x[u][0], m) + exp_below(x[u][1], m)) + (exp_below(x[u][2], m) + exp_below(x[u][3], m));
+        for (int u = 0; u < kPieces; ++u) {
+          float e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) strange = strange || x[u][j] != x[u][j];
+          for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(x[u][j], kLog2e, -c));
+          terms[u] = (e[0] + e[1]) + (e[2] + e[3]);
+        }
+        s += static_cast<double>((terms[0] + terms[1]) + (terms[2] + terms[3])) * __builtin_amdgcn_exp2f(-fmaf(at, kLog2e, -c));
+      } else {
+        bool strange = false;
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+          terms[u] = (exp_below(x[u][0], m) + exp_below(x[u][1], m)) + (exp_below(x[u][2], m) + exp_below(x[u][3], m));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) strange = strange || x[u][j] != x[u][j];
+        }
+        s += strange ? __builtin_nan("") : static_cast<double>((terms[0] + terms[1]) + (terms[2] + terms[3]));
       }
-      s += (terms[0] + terms[1]) + (terms[2] + terms[3]);
       // (an equal one behind the best so far is no better)
       const float above = have == W ? limit : below_of(limit);
       if (own > above) {
@@ -282,7 +297,6 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     const float top = most(tops);
     s = sum_in_last(s);
     if (m != -INFINITY) s *= exp(static_cast<double>(m) - static_cast<double>(top));
-    if (__builtin_amdgcn_ballot_w64(strange) != 0) s = __builtin_nan("");
     if (lane == 63) sums[wave] = s;
     __syncthreads();
     uint64_t* room = a.room + ((g * W + w) * a.parts + part) * stride;

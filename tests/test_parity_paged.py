@@ -497,9 +497,9 @@ def check_beams(logits, scores, done=None, eos=-1, in_place=False):
     assert torch.equal(got[1], want[1]) and torch.equal(got[0], want[0]), (got[:2], want[:2])
     if done is not None:
         assert torch.equal(got[3], want[3])
-    # A term exp(-y), y its distance to the maximum, is off by y 2^-24 (the difference rounded) and 2^-22 (exp2, and what the product's rounding left); weighted by the
-    # terms the mean of y is the entropy less log(sum), at most log(V) < 13; sixteen terms are added in 32 bits, two by two: 4 2^-24; (13 + 4 + 4) 2^-24 < 2^-19 of the sum, and of its
-    # logarithm.  Storing: 2^-24 of the value.
+    # A term exp(-y), y its distance to the maximum, is off by 1.23 y 2^-24 (its exponent's rounding, and log2 e's) and 2^-22 (exp2); weighted by the terms the mean of y is the
+    # entropy less log(sum), at most log(V) < 13; sixteen terms are added in 32 bits, two by two: 4 2^-24; what all have in common is off by 2 2^-24: (16 + 4 + 4 + 2) 2^-24 < 2^-19
+    # of the sum, and of its logarithm.  Storing: 2^-24 of the value.
     same = torch.isinf(want[2])
     assert torch.equal(torch.isinf(got[2]), same)
     off = torch.where(same, 0.0, (got[2].double() - want[2]).abs() - 2.0 ** -24 * want[2].abs() - 2.0 ** -19)
