@@ -575,6 +575,22 @@ def test_logits_far_apart():
         assert torch.equal(out[0].cpu(), want[0]) and torch.equal(out[1].cpu(), want[1])
 
 
+@pytest.mark.parametrize("base", [1e5, -1e5, 2.0 ** 20 - 40, 2.0 ** 20 + 40, -2.0 ** 20, 3e6])
+def test_logits_far_from_nought(base):
+    # steps of a quarter up to 64, exact in fp32 beside the base: the differences alone count
+    g = torch.Generator().manual_seed(3)
+    logits = (torch.randint(0, 256, (3, 4, 20000), generator=g) / 4.0 + base).float()
+    check_beams(logits, -torch.rand(3, 4, generator=g))
+
+
+@pytest.mark.parametrize("W,step", [(8, 1e-3), (2, 1e-3), (32, 1e-3), (8, -1e-3), (8, 0.0)])
+def test_rising_and_falling_logits(W, step):
+    # every one beats what came before it, or none does, or all are the same; rows of several pieces each
+    G, V = 520 // W, 20001
+    logits = (torch.arange(V) * step).expand(G, W, V).contiguous()
+    check_beams(logits, -torch.arange(G * W).view(G, W) / 64.0)
+
+
 def test_many_groups():
     logits, scores, g = some_logits(700, 2, 301, 4)
     check_beams(logits, scores, (torch.rand(700, 2, generator=g) < 0.2).int(), eos=7)
