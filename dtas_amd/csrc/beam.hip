@@ -8,6 +8,9 @@
 // sums of all and compares what is left, in 64 bits.
 // The W best of many are found without sorting them: every eight lanes have the best of their own, the W-th best of these is as good as W of all at least, so only what is not
 // below that can be among the W.  These few are counted out against each other; behind the first piece of a part only what beats the W-th best so far is left.
+// Measured (vocabulary 50280): one group of 4 beams 12.1 us, 32 groups of 8 25.7 us (51 MB: 2.0 TB/s; 10 us at a copy's rate), one group of 32 21.3 us.  What binds is the chain of one
+// workgroup: its load's trip, bound, counting, the hand-over and the last one's comparison (5 to 8 us), each behind the one before.  One search after the other, W of them, took 36.7 and
+// 181 us; the W-th best lanes of each wavefront as the bound 14.4, 30.8 and 39.2.  (Candidates behind the first piece counted out behind the last alone: 24.6 for 32 groups, but 12.9 for one.)
 #include "gemm_common.h"
 
 namespace dtas {

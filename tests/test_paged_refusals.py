@@ -1,4 +1,7 @@
 """What the operators of requests in pages refuse, and what they do nothing for: decided before any launch."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -97,6 +100,20 @@ def test_page_reorder_refuses(bad, why):
                                      lambda: reorder(groups=0, left=E), lambda: reorder(beams=0, left=E)])
 def test_nothing_to_do(nothing):
     assert nothing()[0] == 0
+
+
+def test_tables_of_too_many_positions():
+    # 2^26 blocks of 32 keys to a table: sixteen of them, or of the sequences of groups, are as many as a launch counts
+    for many in (dict(batch=17), dict(batch=32, beams=32), dict(batch=34, beams=2)):
+        rc, message = paged(columns=1 << 27, table=1 << 44, **many)
+        assert rc == -1 and "too many positions" in message, message
+
+
+def test_no_kernel_keeps_registers_in_memory():
+    # what the built library says of its kernels: bytes of scratch memory per lane
+    with open(os.path.join(os.path.dirname(_lib.__file__), "libdtas_gfx950.so"), "rb") as f:
+        found = re.findall(rb"(_ZN4dtas\w*(?:attn_paged|beam_select|page_)\w+)\xbb\.private_segment_fixed_size(.)", f.read(), re.S)
+    assert len(found) >= 20 and all(size == b"\0" for _, size in found), found
 
 
 def test_tensors_on_the_host_are_refused():
