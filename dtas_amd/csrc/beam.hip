@@ -8,7 +8,7 @@
 // sums of all and compares what is left, in 64 bits.
 // The W best of many are found without sorting them: every eight lanes have the best of their own, the W-th best of these is as good as W of all at least, so only what is not
 // below that can be among the W.  These few are counted out against each other; behind the first piece of a part only what beats the W-th best so far is left.
-// Measured (vocabulary 50280): one group of 4 beams 12.1 us, 32 groups of 8 25.7 us (51 MB: 2.0 TB/s; 10 us at a copy's rate), one group of 32 21.3 us.  What binds is the chain of one
+// Measured (vocabulary 50280): one group of 4 beams 11.6 us, 32 groups of 8 25.1 us (51 MB: 2.1 TB/s; 10 us at a copy's rate), one group of 32 20.5 us.  What binds is the chain of one
 // workgroup: its load's trip, bound, counting, the hand-over and the last one's comparison (5 to 8 us), each behind the one before.  One search after the other, W of them, took 36.7 and
 // 181 us; the W-th best lanes of each wavefront as the bound 14.4, 30.8 and 39.2.  (Candidates behind the first piece counted out behind the last alone: 24.6 for 32 groups, but 12.9 for one.)
 #include "gemm_common.h"
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   const int* done = a.done ? a.done + g * W : nullptr;
   auto is_done = [&](int i) { return done && done[i] != 0; };
   auto goes_on = [&](int i) { return finite(scores[i]) && is_done(i) && a.eos >= 0 && a.eos < a.V; };
-  // A list is a part of a beam, a thread's.  Of fewer than a wavefront has lanes, though, the W-th best of their first candidates would be no bound: `depth` threads go through a list
+  // A list is a part of a beam, a thread's (there are no more than threads: beam_parts).  Of fewer than a wavefront has lanes, though, the W-th best of their first candidates would be no bound: `depth` threads go through a list
   // there, thread (list, sub) through its candidates sub, sub + depth, ..., so that a wavefront's are the first ones of all (18 groups of 32 beams over 9143 tokens 54 us, 269 without).
   // What the parts left, and a thread's first candidates, in one trip to memory (further ones, if there are more, are read when they are needed).
   constexpr int kAhead = 4;
@@ -341,22 +341,17 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     uint64_t head, sum, one[kAhead];
   };
   const int depth = lists >= 64 ? 1 : kBeamThreads / lists < W ? kBeamThreads / lists : W;
-  const int sub_of = lists >= 64 ? 0 : tid / lists, list_of = tid - sub_of * lists, step = lists >= 64 ? kBeamThreads : lists;
-  const int last_list = sub_of < depth ? lists : 0;  // (this thread's: list_of, + step, ... before this)
-  auto fetch = [&](int t) {
-    List l{};
-    const int i = t / a.parts;
-    if (t < last_list && finite(scores[i]) && !is_done(i)) {
-      const uint64_t* at = room + static_cast<int64_t>(t) * stride;
-      l.head = get(at);
-      l.sum = get(at + 1);
+  const int sub_of = lists >= 64 ? 0 : tid / lists, list_of = tid - sub_of * lists, beam_of = list_of / a.parts;
+  const bool listed = list_of < lists && sub_of < depth, sole = listed && sub_of == 0;
+  const uint64_t* from_list = room + static_cast<int64_t>(listed ? list_of : 0) * stride;
+  List mine{};
+  if (listed && finite(scores[beam_of]) && !is_done(beam_of)) {
+    mine.head = get(from_list);
+    mine.sum = get(from_list + 1);
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) l.one[u] = get(at + 2 + (sub_of + u * depth < W ? sub_of + u * depth : W - 1));
-    }
-    return l;
-  };
-  const List mine = fetch(list_of);
-  if (sub_of == 0) {
+    for (int u = 0; u < kAhead; ++u) mine.one[u] = get(from_list + 2 + (sub_of + u * depth < W ? sub_of + u * depth : W - 1));
+  }
+  if (sole) {
     stat_m[tid] = first_of(mine.head);
     stat_s[tid] = __builtin_bit_cast(double, mine.sum);
   }
@@ -372,8 +367,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     double s = 0.0;
     for (int p = first; plain_row && p < a.parts; p += 64) {  // (one lane's parts: one sum on the larger maximum)
       const int t = i * a.parts + p;
-      const float o = t < kBeamThreads ? stat_m[t] : first_of(get(room + static_cast<int64_t>(t) * stride)), both = fmaxf(m, o);
-      const double more = t < kBeamThreads ? stat_s[t] : __builtin_bit_cast(double, get(room + static_cast<int64_t>(t) * stride + 1));
+      const float o = stat_m[t], both = fmaxf(m, o);
+      const double more = stat_s[t];
       s = (m == -INFINITY ? s : s * exp(static_cast<double>(m) - static_cast<double>(both))) + (o == -INFINITY ? more : more * exp(static_cast<double>(o) - static_cast<double>(both)));
       m = both;
     }
@@ -391,18 +386,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     return Key{static_cast<double>(scores[i]) + ((static_cast<double>(x) - static_cast<double>(top_of[i])) - log_sum[i]), x, i, static_cast<int>(one >> 32)};
   };
   auto ended_key = [&](int i) { return Key{static_cast<double>(scores[i]), 0.f, i, static_cast<int>(a.eos)}; };
-  auto size_of = [](const List& l) { return static_cast<int>(l.head >> 32); };
+  const int size = static_cast<int>(mine.head >> 32);
+  const bool goes = listed && normal(beam_of), ended = sole && !goes && list_of == beam_of * a.parts && goes_on(beam_of);
   // the bound that the threads' first candidates give, rounded to 32 bits like what is held against it (a beam that is done has one candidate, in its first part's place)
   float own = -INFINITY;
-  for (int t = list_of; t < last_list; t += step) {
-    const int i = t / a.parts;
-    if (normal(i)) {
-      const List l = t == list_of ? mine : fetch(t);
-      if (size_of(l) > sub_of) own = fmaxf(own, static_cast<float>(key_of(i, l.one[0]).score));
-    } else if (sub_of == 0 && t == i * a.parts && goes_on(i)) {
-      own = fmaxf(own, static_cast<float>(ended_key(i).score));
-    }
-  }
+  if (goes && size > sub_of) own = static_cast<float>(key_of(beam_of, mine.one[0]).score);
+  if (ended) own = static_cast<float>(ended_key(beam_of).score);
   float least;
   if (lists >= 8 * W) {  // (fewer: there are no W maxima of eight threads)
     least = bound_of(own);
@@ -420,29 +409,22 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     few.all.beam[n] = k.beam;
     few.all.token[n] = k.token;
   };
-  for (int t = list_of; t < last_list; t += step) {
-    const int i = t / a.parts;
-    if (normal(i)) {
-      List l = t == list_of ? mine : fetch(t);
-      const uint64_t* at = room + static_cast<int64_t>(t) * stride;
-      const int n = size_of(l);
-      bool more = true;
-      for (int k0 = sub_of; more && k0 < n; k0 += kAhead * depth) {
-        if (k0 > sub_of) {
+  if (goes) {
+    bool more = true;
+    for (int k0 = sub_of; more && k0 < size; k0 += kAhead * depth) {
+      if (k0 > sub_of) {
 #pragma unroll
-          for (int u = 0; u < kAhead; ++u) l.one[u] = get(at + 2 + (k0 + u * depth < n ? k0 + u * depth : n - 1));
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const Key k = key_of(i, l.one[u]);
-          more = more && k0 + u * depth < n && static_cast<float>(k.score) >= least;
-          if (more) keep(k);
-        }
+        for (int u = 0; u < kAhead; ++u) mine.one[u] = get(from_list + 2 + (k0 + u * depth < size ? k0 + u * depth : size - 1));
       }
-    } else if (sub_of == 0 && t == i * a.parts && goes_on(i)) {
-      keep(ended_key(i));
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const Key k = key_of(beam_of, mine.one[u]);
+        more = more && k0 + u * depth < size && static_cast<float>(k.score) >= least;
+        if (more) keep(k);
+      }
     }
   }
+  if (ended) keep(ended_key(beam_of));
   __syncthreads();
   const int n = counts[0];
   int found = n < W ? n : W;
@@ -475,13 +457,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
       auto offer = [&](const Key& k) {
         if ((found == 0 || before(last, k)) && before(k, best)) best = k;
       };
-      for (int t = tid; t < lists; t += kBeamThreads) {
-        const int i = t / a.parts;
-        const uint64_t* at = room + static_cast<int64_t>(t) * stride;
-        const int many = normal(i) ? static_cast<int>(get(at) >> 32) : 0;
-        for (int k = 0; k < many; ++k) offer(key_of(i, get(at + 2 + k)));
-        if (t == i * a.parts && goes_on(i)) offer(ended_key(i));
-      }
+      for (int k = 0; sole && goes && k < size; ++k) offer(key_of(beam_of, get(from_list + 2 + k)));
+      if (ended) offer(ended_key(beam_of));
       best = first_in_block(best, slots);
       if (best.token == INT32_MAX) break;
       last = best;
@@ -507,18 +484,19 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   __syncthreads();
   const bool one_of = tid < W;
   const int parent = one_of ? chosen_beam[tid] : 0, token = one_of ? chosen_token[tid] : 0;
-  const bool ended = (done && done[parent] != 0) || token == a.eos;
+  const bool over = (done && done[parent] != 0) || token == a.eos;
   __syncthreads();  // (scores and done may be the outputs: they have been read)
   if (!one_of) return;
   a.parents[g * W + tid] = parent;
   a.tokens[g * W + tid] = token;
   a.new_scores[g * W + tid] = chosen_score[tid];
-  if (a.new_done) a.new_done[g * W + tid] = ended ? 1 : 0;
+  if (a.new_done) a.new_done[g * W + tid] = over ? 1 : 0;
 }
 
 constexpr int64_t kBeamWords = int64_t{1} << 25, kLeastPart = 2048;  // 64-bit words of a launch's lists; logits of a part
-// Parts of a row: two workgroups per CU, of 2048 logits at least (4096: 13.6 us instead of 14.1 for one group of 4 beams, 44.0 instead of 38.6 for one of 32, even for the others).
+// Parts of a row: two workgroups per CU (and so a group's never more than a workgroup has threads), of 2048 logits at least (4096: 13.6 us instead of 14.1 for one group of 4 beams, 44.0 instead of 38.6 for one of 32, even for the others).
 inline int64_t beam_parts(int64_t rows, int64_t V) {
+  static_assert(kBeamThreads >= 512 && kBeamThreads >= DTAS_MAX_BEAMS, "a thread for each part of a group");
   int64_t parts = rows < 512 ? 512 / rows : 1;
   if (parts > ceil_div(V, kLeastPart)) parts = ceil_div(V, kLeastPart);
   const int64_t per = ceil_div(ceil_div(V, parts), 4) * 4;

@@ -57,6 +57,27 @@ def test_the_last_value_is_no_number(B, Hkv, group, d, page, beams, offset, leng
     assert bool(((got[B - 1] - want[0]).abs() <= tolerance[0])[:group, others].all()) and bool(((got[B - 1] - want[0]).abs() <= tolerance[0])[group:].all())
 
 
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+@pytest.mark.parametrize("B,Hkv,group,d,page,beams,offset,length", [c for c in CASES if c[-1] in (33, 97, 2049)])
+def test_a_query_that_is_no_number_is_its_rows_own(B, Hkv, group, d, page, beams, offset, length, value):
+    host = made(B, Hkv, group, d, page, beams, length)
+    want, tolerance = expected(host)
+    host["Q"][B - 1, group - 1, 2] = value
+    got = launch(host, offset=offset, beams=beams).double()
+    assert bool(torch.isnan(got[B - 1, group - 1]).all())
+    # (the others' bits may change: the rows of a problem move their running maxima together, which rounds their weights at other places; the bound of the error is the same)
+    got[B - 1, group - 1] = want[B - 1, group - 1]
+    assert bool(((got - want).abs() <= tolerance).all())
+
+
+@pytest.mark.parametrize("beams", [1, 3])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_no_columns_no_pages_no_keys(beams, offset):
+    host = make(3, 2, 2, 64, 16, [5, 0, 20], beams=beams)
+    for change in (dict(table=host["table"][:, :0]), dict(K=host["K"][:0], V=host["V"][:0]), dict(lens=ints([0, 0, -3]))):
+        assert bool((launch({**host, **change}, offset=offset, beams=beams) == 0).all())
+
+
 @pytest.mark.parametrize("at", [0, 5, 40, -1])
 @pytest.mark.parametrize("B,Hkv,group,d,page,beams,offset,length", [c for c in CASES if c[-1] in (47, 97, 2049)])
 def test_a_key_that_is_no_number_wherever_it_stands(B, Hkv, group, d, page, beams, offset, length, at):

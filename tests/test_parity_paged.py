@@ -594,3 +594,5 @@ def test_rising_and_falling_logits(W, step):
 def test_many_groups():
     logits, scores, g = some_logits(700, 2, 301, 4)
     check_beams(logits, scores, (torch.rand(700, 2, generator=g) < 0.2).int(), eos=7)
+    logits, scores, g = some_logits(70001, 1, 3, 4)  # (more than a grid holds)
+    check_beams(logits, scores, (torch.rand(70001, 1, generator=g) < 0.2).int(), eos=1, in_place=True)
