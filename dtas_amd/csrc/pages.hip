@@ -200,10 +200,14 @@ __device__ __forceinline__ T get(const T* at) { return __hip_atomic_load(at, __A
 constexpr int kReorderThreads = 1024;
 __device__ void settle_pool(const ReorderArgs& a) {
   __shared__ unsigned slots[kReorderThreads / 64], before[kReorderThreads];
+  __shared__ int top[kReorderThreads];  // (what was put down last, by its place in the stack)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nwaves = blockDim.x >> 6;
   const int64_t threads = blockDim.x;
   const int stack = *a.free_count;
-  uint64_t height = stack < 0 ? 0 : stack > a.pages ? a.pages : stack;
+  const uint64_t old_height = stack < 0 ? 0 : stack > a.pages ? a.pages : stack;
+  uint64_t height = old_height;
+  const int64_t rows = a.groups * a.beams;
+  const uint64_t first_wanted = tid < rows ? get(a.wanted + tid) : ~uint64_t{0};  // (with the lists' sizes, in one trip)
   auto upto = [&](unsigned v, unsigned& total) {  // (a workgroup of any number of wavefronts)
     v = upto_in_wave(v);
     __syncthreads();
@@ -233,26 +237,39 @@ __device__ void settle_pool(const ReorderArgs& a) {
         if (before[mid] <= j) low = mid;
         else high = mid;
       }
-      if (height + j < static_cast<uint64_t>(a.pages)) put(a.free + height + j, get(a.back + (c + low) * a.share + (j - before[low])));
+      if (height + j < static_cast<uint64_t>(a.pages)) {
+        const int page = get(a.back + (c + low) * a.share + (j - before[low]));
+        put(a.free + height + j, page);
+        if (total - j <= kReorderThreads) top[(height + j) % kReorderThreads] = page;
+      }
     }
     height += total;
     __syncthreads();
   }
-  if (height > static_cast<uint64_t>(a.pages)) height = a.pages;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  const int64_t rows = a.groups * a.beams;
+  bool drained = false;
+  auto drain = [&] {
+    if (drained) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    drained = true;
+  };
+  if (height > static_cast<uint64_t>(a.pages)) {  // (more pages than there are: some table names one that is not its own)
+    height = a.pages;
+    drain();
+  }
   uint64_t taken = 0;
   for (int64_t c = 0; c < rows; c += threads) {
     const int64_t r = c + tid;
-    const uint64_t one = r < rows ? get(a.wanted + r) : ~uint64_t{0};
+    if (taken + threads > kReorderThreads) drain();
+    const uint64_t one = c == 0 ? first_wanted : r < rows ? get(a.wanted + r) : ~uint64_t{0};
     const bool copy = one != ~uint64_t{0};
     unsigned total;
     const unsigned behind = upto(copy ? 1u : 0u, total);
     if (copy) {
       const uint64_t k = taken + behind - 1;
       const unsigned len = static_cast<unsigned>(one >> 32);
-      const int to = k < height ? get(a.free + (height - 1 - k)) : -1;
+      const uint64_t place = height - 1 - k;
+      const int to = k >= height ? -1 : drained || place < old_height ? get(a.free + place) : top[place % kReorderThreads];
       const bool good = to >= 0 && to < a.pages;
       a.new_lens[r] = good ? static_cast<int>(len) : -1;
       if (good) a.new_table[r * a.columns + len / a.page] = to;

@@ -466,6 +466,18 @@ def test_many_requests_let_go():
     check_reorder(parents, table, lens, free, 10, page, layers=(), Hkv=1, d=8, in_place=True)
 
 
+@pytest.mark.parametrize("G,W,shared,extra,height", [(200, 8, 0, 3, 3), (200, 8, 2, 1500, 1500), (200, 8, 2, 700, 700), (3, 32, 0, 2, 2), (600, 4, 1, 40, 40), (130, 32, 1, 0, 0)])
+def test_many_copies(G, W, shared, extra, height):
+    # copies take what is given back in the same call, what was there before, some of both, or there are too few; more of them than a workgroup has threads
+    g = torch.Generator().manual_seed(G)
+    page, columns = 4, 3
+    lens = torch.randint(9, 12, (G, 1), generator=g).expand(G, W).tolist()
+    table, free = beam_tables(G, W, columns, lens, page, shared, extra, g)
+    for parents in (torch.randint(0, 2, (G, W), generator=g).tolist(), torch.randint(0, W, (G, W), generator=g).tolist()):
+        check_reorder(parents, table, lens, free, height, page, layers=(), Hkv=1, d=8)
+        check_reorder(parents, table, lens, free, height, page, layers=(), Hkv=1, d=8, in_place=True)
+
+
 # ---- the choice of beams
 
 def chosen(logits, scores, done, eos):
