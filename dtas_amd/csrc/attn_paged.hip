@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(64) attn_paged_scalar_kernel(PagedArgs a, int6
 constexpr int kAgent = 16;    // loads past the L2 of an XCD (sc1), as atomic ones of the device's scope are, but 16 bytes wide: 4 beams after 32749 keys 41.5 us, 43.9 with two of 8
 constexpr int kStreamed = 2;  // loads that nobody repeats (nt): 2.3 GB in pieces of 8 KiB 6.0 TB/s without, 6.8 with
 constexpr int kNear = 8, kWhole = 2;
+constexpr int kLong = 48;
+constexpr int kCounted = 512;  // sequences that are looked at for that
 constexpr unsigned kSlotsY = 65535;  // a grid's extent in y
 constexpr int most_shares(int RT) { return 256 / RT; }
 __device__ __forceinline__ uint64_t pair_of(float a, float b) { return static_cast<uint64_t>(__builtin_bit_cast(unsigned, a)) | static_cast<uint64_t>(__builtin_bit_cast(unsigned, b)) << 32; }
@@ -92,6 +94,7 @@ struct PagedGrid {
   int shares, row_groups;          // workgroups per key head and row group that may share
   float one_of;                    // 1 / shares, and a little
   int least, whole;                // a share's blocks, if there are as many; blocks up to which a problem is in one piece
+  int batch, worth;                // sequences; blocks of all of them from which on groups are read together (kLong of them in one at least)
   float* ws;
   unsigned* arrivals;
 };
@@ -115,6 +118,17 @@ __device__ __forceinline__ unsigned problem_length(const PagedArgs& a, const Pag
 }
 // its blocks of 32 keys (one, to write its noughts, where it is empty)
 __device__ __forceinline__ int blocks_of(unsigned len) { return len < 32 ? 1 : static_cast<int>((len + 31) / 32); }
+// Whether groups are read together: what that saves, with pages that are all shared, is more than its longer way costs (launch_paged_rows has the figures)
+__device__ __forceinline__ bool together(const PagedArgs& a, const PagedGrid& grid, int lane) {
+  const int some = grid.batch < kCounted ? grid.batch : kCounted;
+  int total = 0, top = 0;
+  for (int c = 0; c < some; c += 64) {
+    const int blocks = c + lane < some ? blocks_of(length_of(a, c + lane)) : 0, most = wave_most(blocks);
+    total += wave_total(blocks);
+    top = top > most ? top : most;
+  }
+  return top >= kLong && static_cast<float>(total) * (static_cast<float>(grid.batch) / static_cast<float>(some)) >= static_cast<float>(grid.worth);
+}
 // Where the longest problem is not much longer than an even share of all blocks, or short, each workgroup has a problem.  Otherwise workgroup s has the blocks from s * per up to
 // (s + 1) * per, but for a boundary less than `near` from the end of a problem, which moves there: a problem is cut into pieces only where that is worth handing its sums over.
 // Every workgroup finds out for itself which problem its share begins in (p, of length len, whose blocks begin at `at`), and what pieces there are of a problem follows from where
@@ -306,6 +320,13 @@ __device__ f32x4 values_no_numbers(const PagedArgs& a, const Visited& v, int bea
 
 template <int DP, int RT, int W, bool GROUP>
 __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) attn_paged_kernel(PagedArgs a, PagedGrid grid) {
+  if constexpr (GROUP) {
+    if (!together(a, grid, threadIdx.x & 63)) {
+      grid.problems = grid.batch;
+      grid.sub = 1;
+      grid.subs = grid.beams;
+    }
+  }
   constexpr int KS = DP / 32, DT = DP / 16, VL = DP / 16, VH = VL / 2;  // k steps, channel tiles, 16-byte pieces of V per lane, of a half
   constexpr int kRows = 16 * RT, kChunks = DP / 8, kWave = 32 * v_row_bytes(DP), kShare = kRows * (DP + 2);
   __shared__ __attribute__((aligned(16))) char lds[W * kWave];
@@ -814,6 +835,13 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) attn_paged_kernel(P
   }
 }
 
+// Blocks of all sequences on all key heads whose reading once per sequence instead of once per group would cost each CU kSaved bytes
+constexpr double kSaved = 200e3;
+inline int64_t worth_grouping(const PagedArgs& a, int sub) {
+  const double bytes = 128.0 * a.d * a.kv_heads * (1.0 - 1.0 / sub) / 256.0, blocks = sub > 1 ? kSaved / bytes : 1e9;
+  return static_cast<int64_t>(blocks < 1e9 ? blocks : 1e9);
+}
+
 template <int DP, int RT, int W, bool GROUP>
 int launch_paged(const PagedArgs& a, int64_t batch, int beams, int sub, hipStream_t s) {
   const int64_t g = a.heads / a.kv_heads;
@@ -823,21 +851,23 @@ int launch_paged(const PagedArgs& a, int64_t batch, int beams, int sub, hipStrea
   grid.subs = static_cast<int>(ceil_div(grid.beams, grid.sub));
   const int64_t problems = batch / grid.beams * grid.subs;
   grid.row_groups = GROUP ? 1 : static_cast<int>(ceil_div(g, 16 * RT));
-  const int64_t kinds = a.kv_heads * static_cast<int64_t>(grid.row_groups), blocks = a.room < 32 ? 1 : ceil_div(a.room, 32);
+  const int64_t kinds = a.kv_heads * static_cast<int64_t>(grid.row_groups), blocks = a.room < 32 ? 1 : ceil_div(a.room, 32), most = GROUP ? batch : problems;
   if (problems * grid.sub > (int64_t{1} << 30) / blocks) return fail("attn_paged: the tables hold too many positions");
   grid.problems = static_cast<int>(problems);
+  grid.batch = static_cast<int>(batch);
+  grid.worth = GROUP ? static_cast<int>(worth_grouping(a, grid.sub)) : 0;
   grid.least = 8;
   grid.whole = 24;
   constexpr int64_t kWorkgroups = 256;
   int64_t shares = kinds < kWorkgroups ? kWorkgroups / kinds : 1;
   shares = shares < most_shares(RT) ? shares : most_shares(RT);
   if (blocks <= grid.whole) shares = 1;  // (nothing that could be cut)
-  const int64_t slots = problems > shares ? problems : shares;
+  const int64_t slots = most > shares ? most : shares;
   if (slots > INT32_MAX / kinds || slots > int64_t{kSlotsY} * 65535) return fail("attn_paged: the launch has too many workgroups");
   grid.shares = static_cast<int>(shares);
   grid.one_of = 1.000001f / static_cast<float>(shares);
   std::unique_lock<std::recursive_mutex> lock;
-  if (shares > 1 && split_scratch(s, static_cast<size_t>(kinds * 2 * shares) * 16 * RT * (DP + 2) * sizeof(float), static_cast<size_t>(kinds * problems), static_cast<int>(shares),
+  if (shares > 1 && split_scratch(s, static_cast<size_t>(kinds * 2 * shares) * 16 * RT * (DP + 2) * sizeof(float), static_cast<size_t>(kinds * most), static_cast<int>(shares),
                                   &grid.ws, &grid.arrivals, &lock) != 0)
     return -1;
   hipLaunchKernelGGL((attn_paged_kernel<DP, RT, W, GROUP>), dim3(static_cast<unsigned>(kinds), static_cast<unsigned>(slots < kSlotsY ? slots : kSlotsY), static_cast<unsigned>(ceil_div(slots, kSlotsY))), dim3(64 * W), 0, s, a, grid);
@@ -851,7 +881,11 @@ int launch_paged_rows(const PagedArgs& a, int64_t batch, int beams, hipStream_t 
   // 16000 on 4 heads of 80 38.3 / 25.4; only 7 such groups after 53876 gain, 104 / 125.)
   if constexpr (DP <= 128) {
     if (g <= 16) {
-      const int sub = beams > 1 ? (16 / g < beams ? 16 / g : beams) : 1;
+      int sub = beams > 1 ? (16 / g < beams ? 16 / g : beams) : 1;
+      // Read together where that saves each CU 200 KB at least, in sequences of 1536 keys or more (the tables say it could, and the lengths then that it does): groups on their way have four
+      // trips to memory more and fewer, longer problems.  Apart / together: 32 sequences in groups of 4, 32 heads on 8 of 128, after 500 keys 11.1 us / 17.0, 2000 26.6 / 28.4, 8000 89.1 / 46.7;
+      // 8 beams on 32 heads of 128 after 120 7.2 / 21.8, 1000 16.6 / 22.4, 4000 48.2 / 30.3; 4 beams, 32 heads on 8, after 2000 16.8 / 17.1, 16000 41.5 / 28.2.
+      if (a.room < 32u * kLong || batch * ceil_div(a.room, 32) < worth_grouping(a, sub)) sub = beams = 1;
       // Eight wavefronts where few problems are cut, four, and two workgroups per CU, where each CU has several to itself: 4 beams after 32749 keys 43.2 us / 48.6, 61 sequences after
       // up to 2047 on 8 heads 47.2 / 52.1; 64 on 32 heads of 80 after up to 300 55.4 / 30.2, 300 on 8 of 128 after up to 100 61.6 / 28.8.
       const bool many = batch / beams * ((beams + sub - 1) / sub) * a.kv_heads >= 512;

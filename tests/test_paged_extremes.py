@@ -11,16 +11,17 @@ pytestmark = pytest.mark.gpu
 
 INF, NAN = float("inf"), float("nan")
 # (sequences, key heads, query heads to each, d, page, beams, elements off an aligned address): eight wavefronts to a sequence, four where there are many, 32 rows, heads
-# of more than 128; groups of 16 rows with eight and four, of 32 rows, of more than a problem's rows; element by element (an odd address, a page of 10)
+# of more than 128; groups too short to be read together; element by element (an odd address, a page of 10); groups read together where they are long, by eight wavefronts and by four
 FORMS = [(2, 2, 1, 64, 16, 1, 0), (1, 3, 9, 80, 48, 1, 0), (1, 1, 4, 128, 32, 1, 0), (256, 2, 1, 64, 16, 1, 0), (2, 1, 17, 96, 16, 1, 0), (2, 2, 2, 256, 16, 1, 0), (1, 1, 20, 192, 32, 1, 0),
          (4, 2, 2, 64, 16, 2, 0), (4, 1, 4, 128, 32, 4, 0), (512, 2, 1, 64, 16, 2, 0), (8, 2, 4, 80, 16, 8, 0), (10, 1, 9, 128, 16, 5, 0), (4, 2, 2, 256, 16, 4, 0),
-         (2, 2, 2, 64, 16, 1, 1), (4, 1, 3, 40, 10, 2, 0)]
+         (2, 2, 2, 64, 16, 1, 1), (4, 1, 3, 40, 10, 2, 0),
+         (8, 32, 1, 128, 16, 8, 0), (4, 32, 4, 96, 32, 4, 0), (16, 64, 1, 64, 16, 2, 0)]  # (long: groups read together)
 LENGTHS = (1, 16, 31, 32, 33, 47, 97, 2049)
 
 
 def few(form, length):
-    """Many sequences stay short."""
-    return form[0] < 100 or length <= 97
+    """Many sequences stay short, many heads long."""
+    return length == 2049 if form[1] >= 32 else form[0] < 100 or length <= 97
 
 
 CASES = [(*f, n) for f in FORMS for n in LENGTHS if few(f, n)]
@@ -135,7 +136,7 @@ def test_an_infinite_value_of_a_small_weight(B, Hkv, group, d, page, beams, offs
 
 
 @pytest.mark.parametrize("value", [INF, NAN, 65504.0])
-@pytest.mark.parametrize("B,Hkv,group,d,beams,lens", [(4, 2, 2, 64, 2, [70, 70, 200, 181]), (8, 1, 4, 128, 8, [700 + i for i in range(8)]), (3, 3, 1, 80, 3, [97, 1500, 1501]), (5, 2, 9, 128, 5, [40, 41, 47, 39, 33])])
+@pytest.mark.parametrize("B,Hkv,group,d,beams,lens", [(4, 2, 2, 64, 2, [70, 70, 200, 181]), (4, 32, 2, 128, 4, [1700, 1710, 1721, 1701]), (8, 1, 4, 128, 8, [700 + i for i in range(8)]), (3, 3, 1, 80, 3, [97, 1500, 1501]), (5, 2, 9, 128, 5, [40, 41, 47, 39, 33])])
 def test_what_a_beam_does_not_see_does_not_reach_it(B, Hkv, group, d, beams, lens, value):
     # the beams share their first two pages and grow apart behind them; what is wrong with one's own page, or lies behind its length, is not the others'
     host = make(B, Hkv, group, d, 16, lens, beams=beams, shared=2)
@@ -168,7 +169,7 @@ def test_what_a_beam_does_not_see_does_not_reach_it(B, Hkv, group, d, beams, len
 
 
 @pytest.mark.parametrize("gap", [9.0, 13.875, 15.0, 16.5])
-@pytest.mark.parametrize("B,Hkv,group,d,page,beams", [(1, 2, 1, 64, 16, 1), (10, 32, 4, 128, 16, 1), (4, 2, 2, 80, 32, 4), (8, 2, 4, 64, 64, 8), (2, 1, 17, 96, 16, 1), (2, 2, 2, 256, 16, 1), (64, 32, 1, 64, 16, 2)])
+@pytest.mark.parametrize("B,Hkv,group,d,page,beams", [(1, 2, 1, 64, 16, 1), (10, 32, 4, 128, 16, 1), (4, 2, 2, 80, 32, 4), (8, 2, 4, 64, 64, 8), (2, 1, 17, 96, 16, 1), (2, 2, 2, 256, 16, 1), (64, 32, 1, 64, 16, 2), (8, 32, 2, 128, 16, 8)])
 def test_a_long_flat_tail_behind_few_large_weights(B, Hkv, group, d, page, beams, gap):
     """Eight keys of no value whose scores lead those of all others by `gap`: what is left are the others' values, weighted by exp(-gap) each.
 
@@ -229,8 +230,8 @@ def test_sharp_rows(spread, beams):
 
 
 def test_nothing_behind_the_lengths_is_used():
-    for beams, lens in ((1, [0, 33, 64, 2000]), (4, [50, 33, 64, 49]), (2, [700, 689, 1, 15])):
-        host = make(4, 2, 3, 80, 32, lens, beams=beams)
+    for beams, lens, Hkv in ((1, [0, 33, 64, 2000], 2), (4, [50, 33, 64, 49], 2), (2, [700, 689, 1, 15], 2), (4, [1700, 1689, 1600, 15], 32)):
+        host = make(4, Hkv, 3, 80, 32, lens, beams=beams)
         want = launch(host, beams=beams)
         for value in (NAN, INF, -65504.0):
             for b, n in enumerate(lens):

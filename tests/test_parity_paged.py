@@ -310,6 +310,26 @@ def test_beams_that_share_here_and_there(page):
     check(host, beams=1)
 
 
+@pytest.mark.parametrize("beams,B,Hkv,group,d,page,shared,lens", [
+    (8, 8, 32, 1, 128, 16, 120, [2060 + i for i in range(8)]), (4, 8, 16, 4, 128, 32, 0, [2100] * 4 + [1, 0, 2080, 700]), (4, 4, 16, 4, 80, 48, 40, [3000, 2999, 2990, 3001]),
+    (5, 10, 32, 3, 64, 16, 60, [1700 + 9 * i for i in range(10)]), (33, 33, 16, 2, 64, 128, 15, [2000 - 3 * i for i in range(33)]), (2, 4, 32, 8, 96, 64, 20, [2500, 1400, 0, 2499]),
+    (7, 7, 64, 2, 72, 80, 24, [-1, 2000, 1999, 30, 2 ** 31 - 1, 1936, 1905]), (2, 16, 64, 1, 64, 16, 97, [1700, 1600, 1555, 1556] + [50 * i for i in range(12)])])
+def test_long_groups_read_together(beams, B, Hkv, group, d, page, shared, lens):
+    # long enough, and enough of them, that pages are read once for all; the last with more problems than four wavefronts each need
+    host = make(B, Hkv, group, d, page, lens, beams=beams, shared=shared, columns=up(max(n for n in lens if n < 2 ** 31 - 1), page))
+    if page == 32:  # the same page here and there, and pages outside the pool
+        t = host["table"]
+        t[2, 5:9], t[3, 20:] = t[0, 5:9], t[1, 20:]
+        t[1, 30], t[2, 31], t[0, 64] = -1, host["K"].shape[0], -5
+    check(host, beams=beams)
+
+
+def test_short_groups_in_long_tables():
+    # the tables have room for much more: the lengths decide
+    for lens in ([5, 40, 33, 0, 1, 64, 300, 299], [900] * 8, [2100, 5, 3, 2, 1, 0, 7, 9]):
+        check(make(8, 32, 2, 64, 16, lens, beams=4, shared=1, columns=140), beams=4)
+
+
 def test_many_sequences():
     check(make(300, 1, 2, 64, 16, [(37 * b) % 150 for b in range(300)]))
     check(make(96, 8, 1, 64, 16, [(37 * b) % 90 for b in range(96)], beams=4, shared=1), beams=4)
