@@ -895,7 +895,9 @@ int launch_paged_rows(const PagedArgs& a, int64_t batch, int beams, hipStream_t 
     // 32 rows at a time
     return launch_paged<DP, 2, 4, false>(a, batch, beams, 1, s);
   } else {
-    return launch_paged<DP, 1, 4, false>(a, batch, beams, 1, s);
+    // Registers leave room for one wavefront per SIMD: four to a problem, or two where there are many: heads of 256, 52 sequences on 32 after 3 keys 40.3 us / 24.0, after 1000 164 / 151, 64 on 8 of 192
+    // after 60 12.5 / 8.0; but 40 on 8 of 192 after 3000 71.4 / 89.6, one on 8 after 8000 21.0 / 23.4.
+    return batch * a.kv_heads >= 512 ? launch_paged<DP, 1, 2, false>(a, batch, beams, 1, s) : launch_paged<DP, 1, 4, false>(a, batch, beams, 1, s);
   }
 }
 

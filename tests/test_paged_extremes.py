@@ -11,10 +11,10 @@ pytestmark = pytest.mark.gpu
 
 INF, NAN = float("inf"), float("nan")
 # (sequences, key heads, query heads to each, d, page, beams, elements off an aligned address): eight wavefronts to a sequence, four where there are many, 32 rows, heads
-# of more than 128; groups too short to be read together; element by element (an odd address, a page of 10); groups read together where they are long, by eight wavefronts and by four
+# of more than 128, and many of those; groups too short to be read together; element by element (an odd address, a page of 10); groups read together where they are long, by eight wavefronts and by four
 FORMS = [(2, 2, 1, 64, 16, 1, 0), (1, 3, 9, 80, 48, 1, 0), (1, 1, 4, 128, 32, 1, 0), (256, 2, 1, 64, 16, 1, 0), (2, 1, 17, 96, 16, 1, 0), (2, 2, 2, 256, 16, 1, 0), (1, 1, 20, 192, 32, 1, 0),
          (4, 2, 2, 64, 16, 2, 0), (4, 1, 4, 128, 32, 4, 0), (512, 2, 1, 64, 16, 2, 0), (8, 2, 4, 80, 16, 8, 0), (10, 1, 9, 128, 16, 5, 0), (4, 2, 2, 256, 16, 4, 0),
-         (2, 2, 2, 64, 16, 1, 1), (4, 1, 3, 40, 10, 2, 0),
+         (128, 4, 1, 256, 16, 1, 0), (2, 2, 2, 64, 16, 1, 1), (4, 1, 3, 40, 10, 2, 0),
          (8, 32, 1, 128, 16, 8, 0), (4, 32, 4, 96, 32, 4, 0), (16, 64, 1, 64, 16, 2, 0)]  # (long: groups read together)
 LENGTHS = (1, 16, 31, 32, 33, 47, 97, 2049)
 

@@ -330,6 +330,13 @@ def test_short_groups_in_long_tables():
         check(make(8, 32, 2, 64, 16, lens, beams=4, shared=1, columns=140), beams=4)
 
 
+@pytest.mark.parametrize("d", [160, 192, 200, 256])
+def test_many_sequences_of_large_heads(d):
+    lens = [(53 * b) % 200 for b in range(64)]
+    check(make(64, 8, 2, d, 16, lens))
+    check(make(64, 8, 17, d, 32, lens[:62] + [1500, 700], columns=47))
+
+
 def test_many_sequences():
     check(make(300, 1, 2, 64, 16, [(37 * b) % 150 for b in range(300)]))
     check(make(96, 8, 1, 64, 16, [(37 * b) % 90 for b in range(96)], beams=4, shared=1), beams=4)
