@@ -8,7 +8,7 @@
 // sums of all and compares what is left, in 64 bits.
 // The W best of many are found without sorting them: every eight lanes have the best of their own, the W-th best of these is as good as W of all at least, so only what is not
 // below that can be among the W.  These few are counted out against each other; behind the first piece of a part only what beats the W-th best so far is left.
-// Measured (vocabulary 50280): one group of 4 beams 11.6 us, 32 groups of 8 25.1 us (51 MB: 2.1 TB/s; 10 us at a copy's rate), one group of 32 20.5 us.  What binds is the chain of one
+// Measured (vocabulary 50280): one group of 4 beams 11.6 us, 32 groups of 8 23.4 us (51 MB: 2.2 TB/s; 10 us at a copy's rate), one group of 32 20.5 us.  What binds is the chain of one
 // workgroup: its load's trip, bound, counting, the hand-over and the last one's comparison (5 to 8 us), each behind the one before.  One search after the other, W of them, took 36.7 and
 // 181 us; the W-th best lanes of each wavefront as the bound 14.4, 30.8 and 39.2.  (Candidates behind the first piece counted out behind the last alone: 24.6 for 32 groups, but 12.9 for one.)
 #include "gemm_common.h"
@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   };
   __shared__ Lds few;
   __shared__ Key slots[kBeamWaves];
-  __shared__ float tops[kBeamWaves], bounds[64], best_logit[2][DTAS_MAX_BEAMS];
+  __shared__ float tops[kBeamWaves], bounds[64];
+  __shared__ __attribute__((aligned(16))) float best_logit[2][DTAS_MAX_BEAMS];
   __shared__ int best_at[2][DTAS_MAX_BEAMS];
   __shared__ double sums[kBeamWaves], log_sum[DTAS_MAX_BEAMS], stat_s[kBeamThreads];
   __shared__ float top_of[DTAS_MAX_BEAMS], chosen_score[DTAS_MAX_BEAMS], stat_m[kBeamThreads];
@@ -245,18 +246,23 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
             const float mine = i < n ? few.piece.logit[i] : old_logit[i - n];
             const int at = i < n ? few.piece.at[i] : old_at[i - n];
             int rank = 0, level = 0;
-            for (int k = 0; k < n; k += 4) {
-              const f32x4 some = *reinterpret_cast<const f32x4*>(few.piece.logit + k);
+            auto count = [&](const float* of, int many) {
+              for (int k = 0; k < many; k += 4) {
+                const f32x4 some = *reinterpret_cast<const f32x4*>(of + k);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const bool in = k + j < n;
-                rank += in && some[j] > mine ? 1 : 0;
-                level += in && some[j] == mine ? 1 : 0;
+                for (int j = 0; j < 4; ++j) {
+                  const bool in = k + j < many;
+                  rank += in && some[j] > mine ? 1 : 0;
+                  level += in && some[j] == mine ? 1 : 0;
+                }
               }
-            }
-            if (level > (i < n ? 1 : 0))  // (equal ones go by their places)
+            };
+            count(few.piece.logit, n);
+            count(old_logit, old);
+            if (level > 1) {  // (equal ones, but for itself, go by their places)
               for (int k = 0; k < n; ++k) rank += few.piece.logit[k] == mine && few.piece.at[k] < at ? 1 : 0;
-            for (int k = 0; k < old; ++k) rank += old_logit[k] > mine || (old_logit[k] == mine && old_at[k] < at) ? 1 : 0;
+              for (int k = 0; k < old; ++k) rank += old_logit[k] == mine && old_at[k] < at ? 1 : 0;
+            }
             if (rank < W) {
               best_logit[side][rank] = mine;
               best_at[side][rank] = at;
