@@ -684,7 +684,7 @@ def attn_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, ta
     heads, d), one layer's K_pages and V_pages (pages, kv_heads, page, d), fp16; table int32 (B, columns), lens int32 (B).  heads is a
     multiple of kv_heads; scale 1 / sqrt(d) if None.  Positions in pages outside the pool are not seen; a row that sees nothing is zeros.
     With ``beams`` > 1 every so many sequences in a row form a group, whose pages of the same column are read once for all that name
-    them (heads of up to 128); the definition is that of beams = 1.  Pages of a multiple of 16 positions, d a multiple of 8 and data on 16-byte boundaries run on the
+    them where that saves more than it costs (long sequences, heads of up to 128); the definition is that of beams = 1.  Pages of a multiple of 16 positions, d a multiple of 8 and data on 16-byte boundaries run on the
     matrix cores, others element by element."""
     if _fastcall._attn_paged(Q, K_pages, V_pages, table, lens, out, scale, beams):
         return
