@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) page_append_kernel(const U* __restrict__ 
 // parent's from that lane, and compares its own with all that are taken: what nobody takes goes onto the stack, once.  Where on the stack is known when all groups have
 // counted: the pages wait in the workspace, and whoever is last among the workgroups puts them down in their order, and takes the pages for copies from the top
 // (in this order: a pool that has a page too few for the moment would lose a row otherwise).  The copies are a second launch.
-// What binds are trips to memory, one behind the other: lengths, entries, the arrival, what was given back, what is wanted: 6.2 us for one group of 4 beams, 9.8 for 24 of 8 (18.8 with a
+// What binds are trips to memory, one behind the other: lengths, entries, the arrival, the lists' sizes, the lists: 5.5 us for one group of 4 beams, 9.7 for 24 of 8 (18.8 with a
 // wavefront per list of pages in settle_pool instead of a thread per page).
 struct ReorderArgs {
   const int *parents, *table, *lens;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
 }
 
 // The copies: a wavefront per copy, layer, key head and K or V, four pieces per lane on their way at a time.  24 groups of 8 beams, 16 layers of 8 heads of 128, pages of 32 (95 MB
-// read and written): 24 us of the call's 33.7 (eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
+// read and written): 24 us of the call's 33 (when that was 33.7, eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
 template <typename U>
 __global__ void __launch_bounds__(256) page_copy_kernel(U* __restrict__ Kp, U* __restrict__ Vp, const int* __restrict__ copies, const unsigned* __restrict__ count,
                                                         unsigned layers, int64_t pages, unsigned kv_heads, unsigned per_row, unsigned page) {
