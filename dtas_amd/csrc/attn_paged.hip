@@ -882,8 +882,8 @@ int launch_paged_rows(const PagedArgs& a, int64_t batch, int beams, hipStream_t 
   if constexpr (DP <= 128) {
     if (g <= 16) {
       int sub = beams > 1 ? (16 / g < beams ? 16 / g : beams) : 1;
-      // Read together where that saves each CU 200 KB at least, in sequences of 1536 keys or more (the tables say it could, and the lengths then that it does): groups on their way have four
-      // trips to memory more and fewer, longer problems.  Apart / together: 32 sequences in groups of 4, 32 heads on 8 of 128, after 500 keys 11.1 us / 17.0, 2000 26.6 / 28.4, 8000 89.1 / 46.7;
+      // Read together where that saves each CU 200 KB at least, in sequences of 1536 keys or more (the tables say it could, and the lengths then that it does): groups on their way have
+      // more trips to memory and fewer, longer problems.  Apart / together: 32 sequences in groups of 4, 32 heads on 8 of 128, after 500 keys 11.1 us / 17.0, 2000 26.6 / 28.4, 8000 89.1 / 46.7;
       // 8 beams on 32 heads of 128 after 120 7.2 / 21.8, 1000 16.6 / 22.4, 4000 48.2 / 30.3; 4 beams, 32 heads on 8, after 2000 16.8 / 17.1, 16000 41.5 / 28.2.
       if (a.room < 32u * kLong || batch * ceil_div(a.room, 32) < worth_grouping(a, sub)) sub = beams = 1;
       // Eight wavefronts where few problems are cut, four, and two workgroups per CU, where each CU has several to itself: 4 beams after 32749 keys 43.2 us / 48.6, 61 sequences after

@@ -170,10 +170,10 @@ __global__ void __launch_bounds__(256) page_append_kernel(const U* __restrict__ 
 
 // ---- tables of the beams that were chosen --------------------------------------------------------------------------------
 // A workgroup per group, its wavefronts with a range of columns each, S >= beams lanes (a power of two) to a column: lane w reads the old entry of row w, takes its
-// parent's from that lane, and compares its own with all that are taken: what nobody takes goes onto the stack, once.  Where on the stack is known when all groups have
+// parent's from that lane, and compares its own with all others: what no parent names goes onto the stack, once.  Where on the stack is known when all groups have
 // counted: the pages wait in the workspace, and whoever is last among the workgroups puts them down in their order, and takes the pages for copies from the top
 // (in this order: a pool that has a page too few for the moment would lose a row otherwise).  The copies are a second launch.
-// What binds are trips to memory, one behind the other: lengths, entries, the arrival, the lists' sizes, the lists: 5.5 us for one group of 4 beams, 9.7 for 24 of 8 (18.8 with a
+// What binds are trips to memory, one behind the other: lengths, entries, the arrival, the lists' sizes, the lists: 5.3 us for one group of 4 beams, 7.8 for 24 of 8 (18.8 with a
 // wavefront per list of pages in settle_pool instead of a thread per page).
 struct ReorderArgs {
   const int *parents, *table, *lens;
@@ -197,7 +197,18 @@ __device__ __forceinline__ void put(T* at, T v) { __hip_atomic_store(at, v, __AT
 template <typename T>
 __device__ __forceinline__ T get(const T* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned most_dpp(unsigned v) {
+  const unsigned o = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true));
+  return v > o ? v : o;
+}
+__device__ __forceinline__ unsigned most_in_wave(unsigned v) {
+  v = most_dpp<0x118, 0xf>(most_dpp<0x114, 0xf>(most_dpp<0x112, 0xf>(most_dpp<0x111, 0xf>(v))));  // row_shr:1, 2, 4, 8
+  return static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(most_dpp<0x143, 0xc>(most_dpp<0x142, 0xa>(v))), 63));
+}
+
 constexpr int kReorderThreads = 1024;
+static_assert(DTAS_MAX_BEAMS <= 32, "a bit of a word for each");
 __device__ void settle_pool(const ReorderArgs& a) {
   __shared__ unsigned slots[kReorderThreads / 64], before[kReorderThreads];
   __shared__ int top[kReorderThreads];  // (what was put down last, by its place in the stack)
@@ -290,7 +301,7 @@ __device__ void settle_pool(const ReorderArgs& a) {
 
 __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderArgs a) {
   __shared__ uint64_t copy[DTAS_MAX_BEAMS];
-  __shared__ int flag;
+  __shared__ int flag, front[DTAS_MAX_BEAMS];  // (the first row of each parent)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S = 1 << a.shift, w = lane & (S - 1), sub = lane >> a.shift, first = lane - w;
   const int64_t g = blockIdx.x, room = a.columns * a.page;
@@ -301,20 +312,17 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
   const bool has = parent >= 0 && parent < a.beams;
   const int from = first + (has ? parent : 0);
   const unsigned their_len = __shfl(len, from), their_named = __shfl(named, from), new_len = has ? their_len : 0u, new_named = has ? their_named : 0u;
-  bool later = false;  // (a row of the same parent stands in front)
-#pragma unroll 4
-  for (int i = 0; i < a.beams; ++i) {  // (every lane shuffles)
-    const int one = __shfl(parent, first + i);
-    later = later || (one == parent && i < w);
+  if (tid < DTAS_MAX_BEAMS) {
+    copy[tid] = ~uint64_t{0};
+    front[tid] = DTAS_MAX_BEAMS;
   }
-  const bool part_filled = has && later && new_len % a.page != 0;
-  unsigned most = 0;
-  for (int i = 0; i < a.beams; ++i) {
-    const unsigned n = __builtin_amdgcn_readlane(named, i);
-    most = most > n ? most : n;
-  }
-  if (tid < DTAS_MAX_BEAMS) copy[tid] = ~uint64_t{0};
+  __syncthreads();
+  if (wave == 0 && sub == 0 && has) atomicMin(&front[parent], w);
   __syncthreads();  // (also: the lengths have been read)
+  const bool later = has && front[parent] < w;  // (a row of the same parent stands in front)
+  const unsigned followed = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(row && front[w] < DTAS_MAX_BEAMS)) & (S == 32 ? ~0u : (1u << S) - 1u);  // rows that are a parent
+  const bool part_filled = has && later && new_len % a.page != 0;
+  const unsigned most = most_in_wave(named);
   // this wavefront's columns
   const unsigned per = (most + a.waves - 1) / a.waves, lo = per * wave < most ? per * wave : most, hi = lo + per < most ? lo + per : most;
   const int* old = a.table + (g * a.beams + (row ? w : 0)) * a.columns;
@@ -329,13 +337,12 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
     const int next = read(c + step);
     const int theirs = __shfl(entry, from);
     const bool mine = has && c < hi && c < new_named;
-    const int take = mine ? theirs : -1;
-    bool kept = false, again = false;
+    bool kept = false, again = false;  // (a row that is a parent names the same page; a row in front does)
 #pragma unroll 4
     for (int i = 0; i < a.beams; ++i) {
-      const int some = __shfl(take, first + i), one = __shfl(entry, first + i);
-      kept = kept || some == entry;
-      again = again || (one == entry && i < w);
+      const bool same = __shfl(entry, first + i) == entry;
+      kept = kept || (same && ((followed >> i) & 1) != 0);
+      again = again || (same && i < w);
     }
     const bool give = entry >= 0 && entry < a.pages && !kept && !again;
     const uint64_t all = __builtin_amdgcn_ballot_w64(give);
@@ -367,7 +374,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
 }
 
 // The copies: a wavefront per copy, layer, key head and K or V, four pieces per lane on their way at a time.  24 groups of 8 beams, 16 layers of 8 heads of 128, pages of 32 (95 MB
-// read and written): 24 us of the call's 33 (when that was 33.7, eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
+// read and written): 24 us of the call's 31.3 (when that was 33.7, eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
 template <typename U>
 __global__ void __launch_bounds__(256) page_copy_kernel(U* __restrict__ Kp, U* __restrict__ Vp, const int* __restrict__ copies, const unsigned* __restrict__ count,
                                                         unsigned layers, int64_t pages, unsigned kv_heads, unsigned per_row, unsigned page) {
@@ -492,10 +499,10 @@ extern "C" int dtas_page_reorder_f16(const void* parents, const void* table, con
       (columns > 0 && groups > kMost / DTAS_MAX_BEAMS / columns) || (d > 0 && page * d > INT32_MAX) ||
       (layers > 0 && kv_heads > 0 && d > 0 && pages > 0 && layers > kMost / kv_heads / d / (pages * page)))
     return fail("page_reorder: the extents overflow");
-  // two steps of a wavefront's columns at least, and the 32-bit words of the workspace: wanted, copies, backs, back, the count
+  // a step of a wavefront's columns, two from eight wavefronts on, and the 32-bit words of the workspace: wanted, copies, backs, back, the count
   int shift = 0;
   while ((1 << shift) < beams) ++shift;
-  const int64_t steps = ceil_div(columns << shift, 64), waves = steps < 4 ? 1 : steps / 2 < kReorderThreads / 64 ? steps / 2 : kReorderThreads / 64;
+  const int64_t steps = ceil_div(columns << shift, 64), waves = steps < 2 ? 1 : steps < 8 ? steps : steps < 16 ? 8 : steps / 2 < kReorderThreads / 64 ? steps / 2 : kReorderThreads / 64;
   const int64_t share = ceil_div(columns, waves) * beams, lists = groups * beams * 6 + groups * waves * (share + 1) + 2;
   if (lists > (int64_t{1} << 28)) return fail("page_reorder: tables of %lld entries are too large", (long long)(groups * beams * columns));
   const int64_t rows = groups * beams, page_bytes = layers * pages * kv_heads * page * d * 2;
