@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(64) attn_paged_scalar_kernel(PagedArgs a, int6
 // and four trips to memory, one behind the other (length, table, keys, the answer).
 constexpr int kAgent = 16;    // loads past the L2 of an XCD (sc1), as atomic ones of the device's scope are, but 16 bytes wide: 4 beams after 32749 keys 41.5 us, 43.9 with two of 8
 constexpr int kStreamed = 2;  // loads that nobody repeats (nt): 2.3 GB in pieces of 8 KiB 6.0 TB/s without, 6.8 with
-constexpr int kNear = 8, kWhole = 2;
+constexpr int kNear = 8;
+constexpr int kLonger = 32;    // blocks by which a problem may be longer than an even share
 constexpr int kLong = 48;
 constexpr int kCounted = 512;  // sequences that are looked at for that
 constexpr unsigned kSlotsY = 65535;  // a grid's extent in y
@@ -122,14 +123,18 @@ __device__ __forceinline__ int blocks_of(unsigned len) { return len < 32 ? 1 : s
 __device__ __forceinline__ bool together(const PagedArgs& a, const PagedGrid& grid, int lane) {
   const int some = grid.batch < kCounted ? grid.batch : kCounted;
   int total = 0, top = 0;
-  for (int c = 0; c < some; c += 64) {
-    const int blocks = c + lane < some ? blocks_of(length_of(a, c + lane)) : 0, most = wave_most(blocks);
-    total += wave_total(blocks);
-    top = top > most ? top : most;
+#pragma unroll 4
+  for (int c = lane; c < some; c += 64) {
+    const int blocks = blocks_of(length_of(a, c));
+    total += blocks;
+    top = top > blocks ? top : blocks;
   }
+  total = wave_total(total);
+  top = wave_most(top);
   return top >= kLong && static_cast<float>(total) * (static_cast<float>(grid.batch) / static_cast<float>(some)) >= static_cast<float>(grid.worth);
 }
-// Where the longest problem is not much longer than an even share of all blocks, or short, each workgroup has a problem.  Otherwise workgroup s has the blocks from s * per up to
+// Where the longest problem is not much longer than an even share of all blocks (7 sequences on 32 heads of 80 after 6550 .. 26209 keys: cut 176 us, whole 265; 10 after up to 2000 27.6 / 26.3), or
+// short, each workgroup has a problem.  Otherwise workgroup s has the blocks from s * per up to
 // (s + 1) * per, but for a boundary less than `near` from the end of a problem, which moves there: a problem is cut into pieces only where that is worth handing its sums over.
 // Every workgroup finds out for itself which problem its share begins in (p, of length len, whose blocks begin at `at`), and what pieces there are of a problem follows from where
 // its blocks begin and end.
@@ -142,7 +147,7 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, const PagedGrid&
   auto deal = [&](int total, int longest) {
     int per = static_cast<int>(static_cast<float>(total) * grid.one_of) + 1;  // (a little more than an even share: all of them hold everything)
     per = per > grid.least ? per : grid.least;
-    if ((longest + kWhole - 1) / kWhole <= per || longest <= grid.whole) return Share{s < grid.problems ? s : -1, 0, 0, 0, 1 << 30, 1, 0};
+    if (longest - kLonger <= per || longest <= grid.whole) return Share{s < grid.problems ? s : -1, 0, 0, 0, 1 << 30, 1, 0};
     const int64_t from = static_cast<int64_t>(s) * per;
     return Share{s < grid.shares && from < total ? 0 : -1, 0, static_cast<int>(from), total - from > per ? static_cast<int>(from + per) : total, per, per / kNear + 1, 0};
   };
@@ -172,11 +177,14 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, const PagedGrid&
   __shared__ int totals[W], tops[W], found[2];
   const int range = (grid.problems + 64 * W - 1) / (64 * W) * 64, first = wave * range, last = first + range < grid.problems ? first + range : grid.problems;
   int total = 0, top = 0;
-  for (int c = first; c < last; c += 64) {
-    const int blocks = c + lane < last ? blocks_of(problem_length<GROUP>(a, grid, c + lane)) : 0, most = wave_most(blocks);
-    total += wave_total(blocks);
-    top = top > most ? top : most;
+#pragma unroll 4
+  for (int c = first + lane; c < last; c += 64) {
+    const int blocks = blocks_of(problem_length<GROUP>(a, grid, c));
+    total += blocks;
+    top = top > blocks ? top : blocks;
   }
+  total = wave_total(total);
+  top = wave_most(top);
   if (lane == 0) {
     totals[wave] = total;
     tops[wave] = top;
@@ -858,10 +866,11 @@ int launch_paged(const PagedArgs& a, int64_t batch, int beams, int sub, hipStrea
   grid.worth = GROUP ? static_cast<int>(worth_grouping(a, grid.sub)) : 0;
   grid.least = 8;
   grid.whole = 24;
-  constexpr int64_t kWorkgroups = 256;
+  // workgroups of four wavefronts share a CU, but for those of large heads: 16 sequences on 32 heads of 80 after up to 10000 keys 148 us, with 256 of them 174
+  constexpr int64_t kWorkgroups = DP <= 128 && W == 4 ? 512 : 256;
   int64_t shares = kinds < kWorkgroups ? kWorkgroups / kinds : 1;
   shares = shares < most_shares(RT) ? shares : most_shares(RT);
-  if (blocks <= grid.whole) shares = 1;  // (nothing that could be cut)
+  if (blocks <= grid.whole || most > 4096) shares = 1;  // (nothing that could be cut; so many sequences that reading all their lengths in each workgroup costs more than it gives: 8192 after 30 keys, in tables of 4096, 326 us, 543 without)
   const int64_t slots = most > shares ? most : shares;
   if (slots > INT32_MAX / kinds || slots > int64_t{kSlotsY} * 65535) return fail("attn_paged: the launch has too many workgroups");
   grid.shares = static_cast<int>(shares);

@@ -253,6 +253,19 @@ def test_many_sequences_some_of_them_cut(lens):
     assert bool(((got - want).abs() <= tolerance).all())
 
 
+@pytest.mark.parametrize("beams", [1, 2])
+def test_more_sequences_than_are_cut(beams):
+    # thousands of them, one of them long; all tables name pages of a small pool
+    B, page = 4100, 16
+    host = make(2, 2, 2, 64, page, [3000, 3000])
+    g = torch.Generator().manual_seed(beams)
+    host["Q"] = torch.randn(B, 4, 64, generator=g).half()
+    host["table"] = host["table"][:1].expand(B, -1).contiguous()
+    host["lens"] = ints([5 + b % 30 for b in range(B - 2)] + [3000, 0])
+    got, (want, tolerance) = launch(host, beams=beams).double(), expected(host)
+    assert bool(((got - want).abs() <= tolerance).all())
+
+
 @pytest.mark.parametrize("group,d", [(17, 64), (33, 128), (40, 80), (70, 64), (20, 256)])
 def test_many_rows_of_a_key_head_cut(group, d):
     host = make(2, 1, group, d, 32, [3001, 65])
