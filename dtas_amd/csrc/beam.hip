@@ -64,17 +64,25 @@ __device__ __forceinline__ float max_over(float v, int width) {
   for (int k = 1; k < width; k *= 2) v = fmaxf(v, __shfl_xor(v, k));
   return v;
 }
-// The W-th largest of the lanes' values, or a little less: the first 20 bits of it, found bit by bit (as whole numbers in the same order)
+// Numbers as whole ones in the same order, and back (what is not above -inf: -inf)
+__device__ __forceinline__ unsigned key_bits(float v) {
+  const unsigned bits = __builtin_bit_cast(unsigned, v);
+  return bits >> 31 != 0 ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float of_key_bits(unsigned key) {
+  return key <= 0x007fffffu ? -INFINITY : __builtin_bit_cast(float, key >> 31 != 0 ? key & 0x7fffffffu : ~key);
+}
+constexpr int kLastBit = 12;  // of a bound: 20 bits are near enough
+// The W-th largest of the lanes' values, or a little less: its first bits, found one by one
 __device__ __forceinline__ float nth_in_wave(float v, int W) {
-  constexpr unsigned kLowest = 0x007fffffu;  // -inf
-  const unsigned bits = __builtin_bit_cast(unsigned, v), key = bits >> 31 != 0 ? ~bits : bits | 0x80000000u;
+  const unsigned key = key_bits(v);
   unsigned found = 0;
 #pragma unroll 4
-  for (int i = 31; i >= 12; --i) {
+  for (int i = 31; i >= kLastBit; --i) {
     const unsigned next = found | 1u << i;
     found = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= next)) >= W ? next : found;
   }
-  return found <= kLowest ? -INFINITY : __builtin_bit_cast(float, found >> 31 != 0 ? found & 0x7fffffffu : ~found);
+  return of_key_bits(found);
 }
 // the sum of all lanes, in the last
 template <int CTRL, int ROWS>
@@ -126,6 +134,7 @@ __device__ Key first_in_block(Key k, Key* slots) {
   return k;
 }
 
+constexpr int kManyKeys = 96;  // candidates from which on a sharper bound is looked for (2 groups of 32 beams over 92931 tokens, scores up to 20 apart: 27.4 us, 144 without)
 constexpr int kFew = 1024, kFewKeys = 512;  // candidates that are counted out; more (many equal ones, hardly any numbers) are taken one after the other
 constexpr int kPieces = 4, kPiece = kBeamThreads * 4 * kPieces;  // 16 logits per thread at a time
 
@@ -142,7 +151,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   __shared__ double sums[kBeamWaves], log_sum[DTAS_MAX_BEAMS], stat_s[kBeamThreads];
   __shared__ float top_of[DTAS_MAX_BEAMS], chosen_score[DTAS_MAX_BEAMS], stat_m[kBeamThreads];
   __shared__ int chosen_beam[DTAS_MAX_BEAMS], chosen_token[DTAS_MAX_BEAMS];
-  __shared__ int flag, counts[2];  // (of one piece and of the next: a wavefront may be that far ahead of another)
+  __shared__ int above[2][kBeamWaves], flag, counts[2];  // (of one piece and of the next: a wavefront may be that far ahead of another)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x, w = blockIdx.y, W = a.beams;
   const int64_t g = blockIdx.z, from = static_cast<int64_t>(part) * a.per;
   const int here = static_cast<int>(a.V - from < a.per ? a.V - from : a.per), stride = 2 + W;
@@ -346,8 +355,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
   struct List {
     uint64_t head, sum, one[kAhead];
   };
-  const int depth = lists >= 64 ? 1 : kBeamThreads / lists < W ? kBeamThreads / lists : W;
-  const int sub_of = lists >= 64 ? 0 : tid / lists, list_of = tid - sub_of * lists, beam_of = list_of / a.parts;
+  const int wanted = lists >= 64 ? (W + kAhead - 1) / kAhead : W, depth = kBeamThreads / lists < wanted ? kBeamThreads / lists : wanted;
+  const int sub_of = depth == 1 ? 0 : tid / lists, list_of = tid - sub_of * lists, beam_of = list_of / a.parts;
   const bool listed = list_of < lists && sub_of < depth, sole = listed && sub_of == 0;
   const uint64_t* from_list = room + static_cast<int64_t>(listed ? list_of : 0) * stride;
   List mine{};
@@ -415,24 +424,45 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
     few.all.beam[n] = k.beam;
     few.all.token[n] = k.token;
   };
-  if (goes) {
-    bool more = true;
+  auto collect = [&] {
+    bool more = goes;
     for (int k0 = sub_of; more && k0 < size; k0 += kAhead * depth) {
-      if (k0 > sub_of) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) mine.one[u] = get(from_list + 2 + (k0 + u * depth < size ? k0 + u * depth : size - 1));
-      }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const Key k = key_of(beam_of, mine.one[u]);
+        const uint64_t one = k0 == sub_of ? mine.one[u] : get(from_list + 2 + (k0 + u * depth < size ? k0 + u * depth : size - 1));
+        const Key k = key_of(beam_of, one);
         more = more && k0 + u * depth < size && static_cast<float>(k.score) >= least;
         if (more) keep(k);
       }
     }
+    if (ended) keep(ended_key(beam_of));
+    __syncthreads();
+    return counts[0];
+  };
+  int n = collect();
+  if (n > kManyKeys) {
+    // some beams lead the others by far, and the bound is what these have: the W-th best of all that the threads hold, bit by bit
+    unsigned keys[kAhead], best = 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) keys[u] = goes && sub_of + u * depth < size ? key_bits(static_cast<float>(key_of(beam_of, mine.one[u]).score)) : 0u;
+    if (ended) keys[0] = key_bits(static_cast<float>(ended_key(beam_of).score));
+    for (int i = 31; i >= kLastBit; --i) {
+      const unsigned next = best | 1u << i;
+      int some = 0;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) some += __builtin_popcountll(__builtin_amdgcn_ballot_w64(keys[u] >= next));
+      if (lane == 0) above[i & 1][wave] = some;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int k = 0; k < kBeamWaves; ++k) all += above[i & 1][k];
+      best = all >= W ? next : best;
+    }
+    least = fmaxf(least, of_key_bits(best));
+    if (tid == 0) counts[0] = 0;
+    __syncthreads();
+    n = collect();
   }
-  if (ended) keep(ended_key(beam_of));
-  __syncthreads();
-  const int n = counts[0];
   int found = n < W ? n : W;
   if (n <= kFewKeys) {
     for (int i = tid; i < n; i += kBeamThreads) {

@@ -630,6 +630,15 @@ def test_rising_and_falling_logits(W, step):
     check_beams(logits, -torch.arange(G * W).view(G, W) / 64.0)
 
 
+@pytest.mark.parametrize("W", [3, 8, 16, 32])
+@pytest.mark.parametrize("G,V", [(1, 3000), (2, 20000), (2, 92931), (20, 3157)])
+@pytest.mark.parametrize("apart", [0.0, 0.3, 2.0, 50.0])
+def test_some_beams_lead_the_others(W, G, V, apart):
+    # most of the best, or all of them, are one beam's
+    logits, scores, g = some_logits(G, W, V, W + G, spread=1.0)
+    check_beams(logits, (-apart * torch.randperm(W, generator=g)).expand(G, W).contiguous(), (torch.arange(W) % 5 == 4).int().expand(G, W).contiguous(), eos=2)
+
+
 def test_many_groups():
     logits, scores, g = some_logits(700, 2, 301, 4)
     check_beams(logits, scores, (torch.rand(700, 2, generator=g) < 0.2).int(), eos=7)
