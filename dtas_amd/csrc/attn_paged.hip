@@ -75,11 +75,13 @@ __global__ void __launch_bounds__(64) attn_paged_scalar_kernel(PagedArgs a, int6
 // The query heads that share a key head, of all sequences of a group, form one problem of R rows: S^T = K Q^T and O^T = V^T P^T, 16 keys or channels by 16 rows to an
 // instruction, as the tree's attention has them (attn_rows.h).  A wavefront takes a visit at a time: two halves of 16 keys, each from one page, so that
 // all its addresses are a scalar and a lane's constant.  K comes as the matrix cores take it, straight from memory; V passes through a piece of the LDS that is the
-// wavefront's own and is read from there transposed.  The next visit's K and V are on their way in registers, and the table's entries a block further ahead.
+// wavefront's own and is read from there transposed.  A weight goes into the product with V as two fp16 numbers of 11 bits, itself and what its rounding left, so that the answer has
+// the bits of weights in fp32, as element by element (with the first alone it was off by up to 2^-12 of the sum of |v|): 1 after 127 keys 5.46 us with one, 5.54 with both, 4 beams after 32749 41.9 / 42.3,
+// 61 after up to 2047 47.5 / 47.8, 16 after up to 65533 level.  The next visit's K and V are on their way in registers, and the table's entries a block further ahead.
 // In a group a block is visited once for every page that its sequences name there; rows that do not name it have their scores masked.
 // The blocks of all problems, one behind the other, are dealt out in equal shares, on the device, which knows the lengths: see Share.
 // Memory bounds it: 16 sequences after up to 65533 keys (32 heads on 8 of 128, 2.34 GB) 360 us, 6.5 TB/s, where a kernel that only reads pieces of 8 .. 32 KiB in no order reaches 6.7 .. 6.9;
-// 61 after up to 2047 (284 MB) 47.9 us, 5.9 TB/s; 4 beams after 32749 (175 MB) 41.5 us, of which handing the pieces' sums over takes 6 .. 8.  One sequence after 127 keys takes 5.4 us: a launch
+// 61 after up to 2047 (284 MB) 47.8 us, 5.9 TB/s; 4 beams after 32749 (175 MB) 42.3 us, of which handing the pieces' sums over takes 6 .. 8.  One sequence after 127 keys takes 5.5 us: a launch
 // and four trips to memory, one behind the other (length, table, keys, the answer).
 constexpr int kAgent = 16;    // loads past the L2 of an XCD (sc1), as atomic ones of the device's scope are, but 16 bytes wide: 4 beams after 32749 keys 41.5 us, 43.9 with two of 8
 constexpr int kStreamed = 2;  // loads that nobody repeats (nt): 2.3 GB in pieces of 8 KiB 6.0 TB/s without, 6.8 with
@@ -277,8 +279,8 @@ __device__ __forceinline__ int common_blocks(const PagedArgs& a, const int* name
   return l == 0 ? 0 : static_cast<int>(static_cast<unsigned>(static_cast<uint64_t>(columns) * (l - 1) / 64) * a.page / 32);
 }
 
-// A value may be infinite where its weight is too small for fp16 (below 2^-36 of the largest): zero times infinity, though the weight is a number in fp32 and the channel
-// infinite.  Such a channel shows in the sums, as NaN where the sum of the weights is a number (rare); what visits of a group took out is known as well.  What it is instead depends
+// An infinite value may meet a weight too small for fp16 (below 2^-36 of the largest), or one whose rounding left nothing, or less than nothing: zero times infinity, or infinities
+// of both signs, though the weight is a number in fp32 and the channel infinite.  Such a channel shows in the sums, as NaN where the sum of the weights is a number (rare); what visits of a group took out is known as well.  What it is instead depends
 // on the keys alone whose values are no numbers: a thread looks for them in four channels of a row, among what its workgroup visited of the row's sequence (items first .. last), and
 // sums them with their weights in fp32.
 struct Visited {
@@ -629,29 +631,34 @@ __global__ void __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) attn_paged_kernel(P
         *reinterpret_cast<u32x4*>(mine + row * v_row_bytes(DP) + c * 16) = vf[n];
       }
       load_v(next);
-      f16x8 p[RT];
+      f16x8 p[RT], rest[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         weigh<2, DT>(s[rt], all, shown[rt], quarter, a.scale_log2, top[rt], sum[rt], o[rt]);
         p[rt] = weights_f16(s[rt][0], s[rt][1]);
+        rest[rt] = weights_rest(s[rt][0], s[rt][1], p[rt]);
       }
-      auto add = [&](int dt, const f16x4& lo, const f16x4& hi) {
-        const f16x8 vt = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      auto add = [&](int dt0, auto& lo, auto& hi) {
+        constexpr int N = sizeof(lo) / sizeof(lo[0]);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p[rt], o[rt][dt], 0, 0, 0);
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int u = 0; u < N; ++u) {
+            const f16x8 vt = {lo[u][0], lo[u][1], lo[u][2], lo[u][3], hi[u][0], hi[u][1], hi[u][2], hi[u][3]};
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[rt][dt0 + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, part == 0 ? p[rt] : rest[rt], o[rt][dt0 + u], 0, 0, 0);
+          }
       };
 #pragma unroll
       for (int dt = 0; dt + 4 <= DT; dt += 4) {
         f16x4 lo[4], hi[4];
         read_v<DP>(tr_at + dt * 32, lo, hi);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) add(dt + u, lo[u], hi[u]);
+        add(dt, lo, hi);
       }
       if constexpr (DT % 4 == 2) {
         f16x4 lo[2], hi[2];
         read_v<DP>(tr_at + (DT - 2) * 32, lo, hi);
-        add(DT - 2, lo[0], hi[0]);
-        add(DT - 1, lo[1], hi[1]);
+        add(DT - 2, lo, hi);
       }
     };
     Visit here{}, next{};

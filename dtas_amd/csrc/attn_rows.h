@@ -1,5 +1,5 @@
 // What the kernels have in common that attend with few query rows per key head (attn_tree.hip, attn_paged.hip): 16 keys or rows to a matrix instruction, P and O^T as
-// the lanes hold them, weights in fp16, parts of the keys joined through the workspace.  Internal to libdtas_gfx950.so.
+// the lanes hold them, weights in fp16 (one or two of them), parts of the keys joined through the workspace.  Internal to libdtas_gfx950.so.
 #pragma once
 #include "gemm_common.h"
 
@@ -153,6 +153,16 @@ __device__ __forceinline__ void weigh(f32x4 (&s)[NK], bool all, uint64_t shown, 
 __device__ __forceinline__ f16x8 weights_f16(const f32x4& a, const f32x4& b) {
   return f16x8{static_cast<half_t>(a[0]), static_cast<half_t>(a[1]), static_cast<half_t>(a[2]), static_cast<half_t>(a[3]),
                static_cast<half_t>(b[0]), static_cast<half_t>(b[1]), static_cast<half_t>(b[2]), static_cast<half_t>(b[3])};
+}
+// ... and what is left of them beside that, in fp16 as well: the two together have 22 bits, and steps of 2^-36 of the maximum's weight at least
+__device__ __forceinline__ f16x8 weights_rest(const f32x4& a, const f32x4& b, const f16x8& p) {
+  f16x8 rest;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    rest[j] = static_cast<half_t>(a[j] - static_cast<float>(p[j]));
+    rest[4 + j] = static_cast<half_t>(b[j] - static_cast<float>(p[4 + j]));
+  }
+  return rest;
 }
 __device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1; }
 

@@ -501,7 +501,7 @@ int dtas_page_append_f16(const void* K, const void* V, const void* slots, void* 
  * [pages, kv_heads, page, d]; heads is a multiple of kv_heads, query head h reads key head h / (heads / kv_heads).  Sequences in a row, `beams` of them, form a group: a
  * page that several of them name in the same column is read once for all where that saves more than it costs (long sequences, d up to 128; the definition is that of beams = 1).  batch is a multiple of beams.
  * d up to 256; d a multiple of 8, data on 16-byte boundaries and pages of a multiple of 16 positions run on the matrix cores, others element by element.  fp32 scores,
- * statistics and sums; weights in fp16 on the matrix cores, as in dtas_attn_tree_f16.  scale is a finite number up to 2e38 either way.  Uses the
+ * statistics, weights and sums (on the matrix cores a weight is two fp16 numbers: 22 bits, and 2^-36 of its row's largest at least).  scale is a finite number up to 2e38 either way.  Uses the
  * split-K workspace, under the rules stated at the top of this file. */
 int dtas_attn_paged_f16(const void* Q, const void* K_pages, const void* V_pages, const void* table, const void* lens, void* out, int64_t batch,
                         int64_t heads, int64_t kv_heads, int64_t d, int64_t page, int64_t pages, int64_t columns, int64_t beams, float scale, void* stream);
