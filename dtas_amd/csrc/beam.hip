@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_select_kernel(BeamArgs a) {
       }
       const float wave_top = wave_max(own);
       if (wave_top > m) {
-        s = m == -INFINITY ? 0.0 : s * exp(static_cast<double>(m) - static_cast<double>(wave_top));
+        s = m == -INFINITY ? s : s * exp(static_cast<double>(m) - static_cast<double>(wave_top));  // (before the first number: nought, or NaN where one was among them, which stays)
         m = wave_top;
       }
       float terms[kPieces];
