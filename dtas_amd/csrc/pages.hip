@@ -373,6 +373,12 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(ReorderAr
   if (flag) settle_pool(a);
 }
 
+// without a row the stack's height is handed on, as far as the stack can be that high
+__global__ void stack_height_kernel(const int* free_count, int* left, int pages) {
+  const int stack = *free_count;
+  *left = stack < 0 ? 0 : stack > pages ? pages : stack;
+}
+
 // The copies: a wavefront per copy, layer, key head and K or V, four pieces per lane on their way at a time.  24 groups of 8 beams, 16 layers of 8 heads of 128, pages of 32 (95 MB
 // read and written): 24 us of the call's 31.3 (when that was 33.7, eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
 template <typename U>
@@ -515,14 +521,15 @@ extern "C" int dtas_page_reorder_f16(const void* parents, const void* table, con
   ReorderArgs a{static_cast<const int*>(parents), static_cast<const int*>(table), static_cast<const int*>(lens), static_cast<int*>(free),
                 static_cast<const int*>(free_count), static_cast<int*>(new_table), static_cast<int*>(new_lens), static_cast<int*>(left), groups, columns,
                 static_cast<int>(beams), 0, static_cast<unsigned>(page), static_cast<int>(pages), 1, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
-  if (rows == 0) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows == 0) {  // (nothing to sort out, and no workspace to do it in)
     if (left == free_count) return 0;
-    a.groups = a.beams = 0;  // (a workgroup without a row hands the stack's height on)
+    hipLaunchKernelGGL(stack_height_kernel, dim3(1), dim3(1), 0, s, a.free_count, a.left, a.pages);
+    return check_launch("page_reorder");
   }
   a.shift = shift;
   a.waves = static_cast<int>(waves);
   a.share = share;
-  hipStream_t s = static_cast<hipStream_t>(stream);
   float* room = nullptr;
   std::unique_lock<std::recursive_mutex> lock;
   if (split_scratch(s, static_cast<size_t>(lists) * 4, 1, 1, &room, &a.arrivals, &lock) != 0) return -1;
@@ -533,9 +540,9 @@ extern "C" int dtas_page_reorder_f16(const void* parents, const void* table, con
   a.back = reinterpret_cast<int*>(a.backs + groups * a.waves);
   // (whoever settles the pool has use for more threads than the columns have, where there are many groups)
   const unsigned threads = 64u * static_cast<unsigned>(a.waves >= 8 || groups * a.waves <= 1 ? a.waves : groups * a.waves < 8 ? groups * a.waves : 8);
-  hipLaunchKernelGGL(page_reorder_kernel, dim3(static_cast<unsigned>(a.groups > 0 ? a.groups : 1)), dim3(threads), 0, s, a);
+  hipLaunchKernelGGL(page_reorder_kernel, dim3(static_cast<unsigned>(groups)), dim3(threads), 0, s, a);
   if (check_launch("page_reorder") != 0) return -1;
-  if (groups == 0 || beams < 2 || page_bytes == 0 || page == 1) return 0;
+  if (beams < 2 || page_bytes == 0 || page == 1) return 0;
   const int64_t most = groups * (beams - 1), each = 2 * layers * kv_heads;  // copies at most, and a copy's items
   const unsigned grid = each < 8192 / most ? static_cast<unsigned>(ceil_div(most * each, 4)) : 2048;
   const bool wide = d % 8 == 0 && aligned(K_pages, 16) && aligned(V_pages, 16);
