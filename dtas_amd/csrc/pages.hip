@@ -479,16 +479,23 @@ extern "C" int dtas_page_append_f16(const void* K, const void* V, const void* sl
   if (check_spans("page_append", in, out, {nullptr, nullptr}) != 0) return -1;
   const bool wide = d % 8 == 0 && aligned(K, 16) && aligned(V, 16) && aligned(K_pages, 16) && aligned(V_pages, 16);
   const int64_t per_row = wide ? d / 8 : d, row = kv_heads * per_row, run = row >= 256 ? 1 : 256 / row, runs = ceil_div(rows, run);
-  if (layers * runs > INT32_MAX) return fail("page_append: the launch has too many workgroups");
+  // as many layers, or runs of one layer, to a launch as a grid holds: less than 2^32 threads
+  constexpr int64_t kMostRuns = int64_t{1} << 23;
+  const int64_t some_layers = runs < kMostRuns ? kMostRuns / runs : 1, some_rows = runs < kMostRuns ? rows : kMostRuns * run;
   auto go = [&](auto* tag) {
     using U = std::remove_pointer_t<decltype(tag)>;
-    hipLaunchKernelGGL(page_append_kernel<U>, dim3(static_cast<unsigned>(layers * runs)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const U*>(K),
-                       static_cast<const U*>(V), static_cast<const int*>(slots), static_cast<U*>(K_pages), static_cast<U*>(V_pages), rows, static_cast<int>(kv_heads),
-                       static_cast<int>(per_row), static_cast<unsigned>(page), pages, static_cast<int>(run), static_cast<unsigned>(runs));
+    for (int64_t l = 0; l < layers; l += some_layers)
+      for (int64_t n = 0; n < rows; n += some_rows) {
+        const int64_t here = layers - l < some_layers ? layers - l : some_layers, rows_here = rows - n < some_rows ? rows - n : some_rows, runs_here = ceil_div(rows_here, run);
+        const int64_t from = (l * rows + n) * row, to = l * pages * page * row;
+        hipLaunchKernelGGL(page_append_kernel<U>, dim3(static_cast<unsigned>(here * runs_here)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const U*>(K) + from,
+                           static_cast<const U*>(V) + from, static_cast<const int*>(slots) + n, static_cast<U*>(K_pages) + to, static_cast<U*>(V_pages) + to, rows_here,
+                           static_cast<int>(kv_heads), static_cast<int>(per_row), static_cast<unsigned>(page), pages, static_cast<int>(run), static_cast<unsigned>(runs_here));
+        if (check_launch("page_append") != 0) return -1;
+      }
+    return 0;
   };
-  if (wide) go(static_cast<u32x4*>(nullptr));
-  else go(static_cast<half_t*>(nullptr));
-  return check_launch("page_append");
+  return wide ? go(static_cast<u32x4*>(nullptr)) : go(static_cast<half_t*>(nullptr));
 }
 
 extern "C" int dtas_page_reorder_f16(const void* parents, const void* table, const void* lens, void* free, const void* free_count, void* new_table, void* new_lens,
