@@ -545,8 +545,10 @@ extern "C" int dtas_page_reorder_f16(const void* parents, const void* table, con
   a.count = reinterpret_cast<unsigned*>(room) + 6 * rows;
   a.backs = a.count + 2;
   a.back = reinterpret_cast<int*>(a.backs + groups * a.waves);
-  // (whoever settles the pool has use for more threads than the columns have, where there are many groups)
-  const unsigned threads = 64u * static_cast<unsigned>(a.waves >= 8 || groups * a.waves <= 1 ? a.waves : groups * a.waves < 8 ? groups * a.waves : 8);
+  // Whoever settles the pool has use for more wavefronts than the columns have, where there are many groups; but a launch has less than 2^32 threads.  (Those of the columns always fit: n of them, n > 1, take
+  // more than 32 (n - 1) entries of a group's lists, one takes 8 words, and the lists are limited above.)
+  const int64_t useful = groups * waves < 8 ? groups * waves : 8, fit = ((int64_t{1} << 32) - 1) / groups / 64, spare = useful < fit ? useful : fit;
+  const unsigned threads = 64u * static_cast<unsigned>(waves > spare ? waves : spare);
   hipLaunchKernelGGL(page_reorder_kernel, dim3(static_cast<unsigned>(groups)), dim3(threads), 0, s, a);
   if (check_launch("page_reorder") != 0) return -1;
   if (beams < 2 || page_bytes == 0 || page == 1) return 0;
