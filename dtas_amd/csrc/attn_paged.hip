@@ -121,13 +121,14 @@ __device__ __forceinline__ unsigned problem_length(const PagedArgs& a, const Pag
 }
 // its blocks of 32 keys (one, to write its noughts, where it is empty)
 __device__ __forceinline__ int blocks_of(unsigned len) { return len < 32 ? 1 : static_cast<int>((len + 31) / 32); }
-// Whether groups are read together: what that saves, with pages that are all shared, is more than its longer way costs (launch_paged_rows has the figures)
+// Whether groups are read together: what that saves, with pages that are all shared, is more than its longer way costs (launch_paged_rows has the figures).  Of more than kCounted
+// sequences as many are looked at, evenly over the batch
 __device__ __forceinline__ bool together(const PagedArgs& a, const PagedGrid& grid, int lane) {
   const int some = grid.batch < kCounted ? grid.batch : kCounted;
   int total = 0, top = 0;
 #pragma unroll 4
   for (int c = lane; c < some; c += 64) {
-    const int blocks = blocks_of(length_of(a, c));
+    const int blocks = blocks_of(length_of(a, some < kCounted ? c : static_cast<int64_t>(c) * grid.batch / kCounted));
     total += blocks;
     top = top > blocks ? top : blocks;
   }

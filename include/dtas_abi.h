@@ -499,7 +499,8 @@ int dtas_page_append_f16(const void* K, const void* V, const void* slots, void* 
  * out[b,h,:] = sum_j softmax_j(scale * Q[b,h,:] . k_j) v_j over the positions j < lens[b] (clipped to [0, columns * page]; the token's own is among
  * them); positions in pages outside [0, pages) are not seen, a row that sees nothing is zeros.  Q and out [batch, heads, d], one layer's K_pages and V_pages
  * [pages, kv_heads, page, d]; heads is a multiple of kv_heads, query head h reads key head h / (heads / kv_heads).  Sequences in a row, `beams` of them, form a group: a
- * page that several of them name in the same column is read once for all where that saves more than it costs (long sequences, d up to 128; the definition is that of beams = 1).  batch is a multiple of beams.
+ * page that several of them name in the same column is read once for all where that saves more than it costs (long sequences, d up to 128: the lengths say, of more than 512 sequences those of 512 evenly over
+ * the batch; the definition is that of beams = 1).  batch is a multiple of beams.
  * d up to 256; d a multiple of 8, data on 16-byte boundaries and pages of a multiple of 16 positions run on the matrix cores, others element by element.  fp32 scores,
  * statistics, weights and sums (on the matrix cores a weight is two fp16 numbers: 22 bits, and 2^-36 of its row's largest at least).  scale is a finite number up to 2e38 either way.  Uses the
  * split-K workspace, under the rules stated at the top of this file. */
