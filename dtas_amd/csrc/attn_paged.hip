@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(64) attn_paged_scalar_kernel(PagedArgs a, int6
 // all its addresses are a scalar and a lane's constant.  K comes as the matrix cores take it, straight from memory; V passes through a piece of the LDS that is the
 // wavefront's own and is read from there transposed.  A weight goes into the product with V as two fp16 numbers of 11 bits, itself and what its rounding left, so that the answer has
 // the bits of weights in fp32, as element by element (with the first alone it was off by up to 2^-12 of the sum of |v|): 1 after 127 keys 5.46 us with one, 5.54 with both, 4 beams after 32749 41.9 / 42.3,
-// 61 after up to 2047 47.5 / 47.8, 16 after up to 65533 level.  The next visit's K and V are on their way in registers, and the table's entries a block further ahead.
+// 61 after up to 2047 47.5 / 47.8, 16 after up to 65533 level, other forms 0.3 to 2 %.  The next visit's K and V are on their way in registers, and the table's entries a block further ahead.
 // In a group a block is visited once for every page that its sequences name there; rows that do not name it have their scores masked.
 // The blocks of all problems, one behind the other, are dealt out in equal shares, on the device, which knows the lengths: see Share.
 // Memory bounds it: 16 sequences after up to 65533 keys (32 heads on 8 of 128, 2.34 GB) 360 us, 6.5 TB/s, where a kernel that only reads pieces of 8 .. 32 KiB in no order reaches 6.7 .. 6.9;

@@ -42,7 +42,7 @@ __device__ __forceinline__ unsigned upto_in_block(unsigned v, unsigned* slots, u
 // A thread per sequence finds out what it needs and, from the sums over the sequences before it, whether the pool has it; then a thread per row looks up its sequence
 // (packed rows: by halving the starts, which lie in the LDS) and its slot.  The row that begins a page writes it into the table, so that no two threads write one entry,
 // and nobody reads an entry that this launch writes.  Every workgroup repeats the sums for itself: no hand-over between workgroups, whose
-// trip through memory costs more than the sums of a thousand sequences.  3.4 us, a launch's time, for 64 sequences of a row; 5.7 for 16384 packed rows.
+// trip through memory costs more than the sums of a thousand sequences.  3.5 to 4.2 us, a launch's time, for 64 sequences of a row; 5.7 for 16384 packed rows of 37.
 struct AssignArgs {
   const int *lens, *count;
   int* table;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(THREADS) page_assign_kernel(AssignArgs a, bool
 
 // ---- rows into their slots ----------------------------------------------------------------------------------------------
 // A workgroup has `run` rows of one layer, of K and of V, in 16-byte pieces (or elements): a row of all key heads at least, two pieces per thread and turn.
-// 2047 packed rows of 32 heads of 80 (42 MB read and written): 8.4 us, 5.0 TB/s, the rate of a large copy; 64 rows: 3.75 us, a launch's time.
+// 2047 packed rows of 32 heads of 80 (42 MB read and written): 8.4 us, 5.0 TB/s, the rate of a large copy; 64 rows: 3.2 to 3.8 us, a launch's time.
 template <typename U>
 __global__ void __launch_bounds__(256) page_append_kernel(const U* __restrict__ K, const U* __restrict__ V, const int* __restrict__ slots, U* __restrict__ Kp,
                                                           U* __restrict__ Vp, int64_t rows, int kv_heads, int per_row, unsigned page, int64_t pages, int run, unsigned runs) {
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) page_append_kernel(const U* __restrict__ 
 // parent's from that lane, and compares its own with all others: what no parent names goes onto the stack, once.  Where on the stack is known when all groups have
 // counted: the pages wait in the workspace, and whoever is last among the workgroups puts them down in their order, and takes the pages for copies from the top
 // (in this order: a pool that has a page too few for the moment would lose a row otherwise).  The copies are a second launch.
-// What binds are trips to memory, one behind the other: lengths, entries, the arrival, the lists' sizes, the lists: 5.3 us for one group of 4 beams, 7.8 for 24 of 8 (18.8 with a
+// What binds are trips to memory, one behind the other: lengths, entries, the arrival, the lists' sizes, the lists: 4.9 us for one group of 4 beams, 7.8 for 24 of 8 (18.8 with a
 // wavefront per list of pages in settle_pool instead of a thread per page).
 struct ReorderArgs {
   const int *parents, *table, *lens;
@@ -380,7 +380,7 @@ __global__ void stack_height_kernel(const int* free_count, int* left, int pages)
 }
 
 // The copies: a wavefront per copy, layer, key head and K or V, four pieces per lane on their way at a time.  24 groups of 8 beams, 16 layers of 8 heads of 128, pages of 32 (95 MB
-// read and written): 24 us of the call's 31.3 (when that was 33.7, eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
+// read and written): 24 us of the call's 31 to 34 (when that was 33.7, eight pieces: 35.3; four times the workgroups: 1 us more; loads and stores past the L2: 2 more; a workgroup for all heads of K and V: 29).
 template <typename U>
 __global__ void __launch_bounds__(256) page_copy_kernel(U* __restrict__ Kp, U* __restrict__ Vp, const int* __restrict__ copies, const unsigned* __restrict__ count,
                                                         unsigned layers, int64_t pages, unsigned kv_heads, unsigned per_row, unsigned page) {
