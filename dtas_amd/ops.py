@@ -708,7 +708,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: Optional[torch
     with token ``eos`` alone, at scores[w].  The best, as many as there are beams, in their order (ties: the lower w, then the lower v): parents
     w and tokens v int32, new_scores; new_done where the parent was done or the token is eos.  logits (requests, beams, V) and scores
     (requests, beams) fp32, done int32 (requests, beams) or None with new_done None: no beam is done.  new_scores and new_done may be scores
-    and done themselves.  What is no finite number counts as -inf (a request begins with scores (0, -inf, ...)).  Up to 32 beams.
+    and done themselves.  What is no finite number counts as -inf (a request begins with scores (0, -inf, ...);
+    of a beam with a NaN or +inf among its logits that is every candidate).  Up to 32 beams.
     ``page_reorder`` takes the parents."""
     if _fastcall._beam_select(logits, scores, done, tokens, parents, new_scores, new_done, eos):
         return

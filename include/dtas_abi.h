@@ -509,7 +509,7 @@ int dtas_attn_paged_f16(const void* Q, const void* K_pages, const void* V_pages,
 
 /* ---- the best continuations of each request's beams ----
  * logits [groups, beams, V], scores [groups, beams], fp32.  Candidate (w, v) of a group has scores[w] + log_softmax(logits[w])[v]; a beam that is done (done[w] != 0)
- * goes on with token eos alone, at scores[w].  What is no finite number counts as -inf.  The `beams` best candidates in their order, ties to the lower w, then the lower
+ * goes on with token eos alone, at scores[w].  What is no finite number counts as -inf (of a beam with a NaN or +inf among its logits that is every candidate: their sum is none).  The `beams` best candidates in their order, ties to the lower w, then the lower
  * v: parents, tokens [groups, beams] int32, new_scores [groups, beams] fp32; new_done = done of the parent, or token == eos.  done and new_done [groups, beams] int32,
  * or both NULL: no beam is done.  eos outside [0, V): none is (a beam that is done then has no candidate).  new_scores == scores and new_done == done are allowed.  beams up to DTAS_MAX_BEAMS, V up to 2^30.
  * Candidates are compared in 64 bits, sums of exponentials are in 64 bits over sums of sixteen terms in 32.  Uses the split-K workspace. */
